@@ -26,7 +26,8 @@
  *     aborts or prints. wattn_last_error() gives the calling thread's last
  *     error message. All entry points are thread-safe and re-entrant.
  *   - Kernel-side waits are bounded; a wait that runs out sets a per-device
- *     status word, read (and cleared) by wattn_device_status().
+ *     status word, read (and cleared) by wattn_device_status(). So do device
+ *     arrays that a kernel finds out of range (wattn_paged_attend).
  */
 #ifndef WATTN_H
 #define WATTN_H
@@ -63,8 +64,9 @@ const char *wattn_status_string(int status);
 int wattn_last_error(char *buf, size_t len);
 
 /* Reads and clears the device status word of `device` (the current device
- * if device < 0): WATTN_OK, or WATTN_ERR_TIMEOUT if a kernel's bounded wait
- * ran out since the last call. Synchronises that device. */
+ * if device < 0): WATTN_OK, WATTN_ERR_TIMEOUT if a kernel's bounded wait ran
+ * out since the last call, or WATTN_ERR_RANGE if a kernel found a device array
+ * out of range (the first of them is kept). Synchronises that device. */
 int wattn_device_status(int device, int *status);
 
 /* ======================================================================
@@ -331,6 +333,122 @@ int wattn_kv_read_slot(wattn_kv_cache *cache, int layer, int slot, int which,
 /* Pool statistics: pages in use and pool size. */
 int wattn_kv_stats(const wattn_kv_cache *cache, int *pages_used,
                    int *pages_total);
+
+/* ======================================================================
+ * Device-planned paged cache
+ *
+ * The cache above keeps its page lists on the host and builds each launch's
+ * table there. Here the whole state lives in the caller's device arrays, so a
+ * decode step makes no host decision: one captured graph serves requests of
+ * every length, and a step may check a tree of drafted tokens per request
+ * (speculative decoding). These entry points have no counterpart in the
+ * reference; the attention is multi_head_attention_with_cache's
+ * (crates/whisper/src/decoder.rs:835-892) with a tree in the place of the
+ * causal rule. A step:
+ *
+ *   wattn_paged_plan     once: pages, row slots, positions, tree masks
+ *   wattn_paged_write    per layer: the new rows' K/V into their slots
+ *   wattn_paged_attend   per layer: attention of the new rows
+ *   wattn_paged_accept   once: the verified path kept, the lengths advanced
+ *
+ * All arrays are device memory of the current device, 4-byte integers, 4-byte
+ * aligned; none may overlap another. Request s has seq_lens[s] cached tokens
+ * and n_new[s] new ones in this step. The new rows of all requests are packed,
+ * request after request: those of s are rows row_start[s] .. row_start[s+1]-1.
+ * Row buffers hold max_rows rows; rows behind the last request's are padding
+ * (slot -1, position -1, mask 0), whose outputs are left as they are.
+ *
+ * Pool: the layout of wattn_kv_create, [n_pages][n_layers][K|V][n_heads]
+ * [page_rows][64] elements of `dtype`, 16-byte aligned, page_rows a multiple
+ * of 16, fewer than 2^31 head rows in all (n_pages * n_layers * 2 * n_heads *
+ * page_rows). A slot is page * page_rows + row in the page; token t of request
+ * s lives at row t % page_rows of page block_table[s * table_stride + t /
+ * page_rows]. Pages belong to one request each.
+ * ====================================================================== */
+
+/* Block tables, slot maps and tree masks from the requests' lengths.
+ * Request s ends up holding exactly ceil((seq_lens[s] + n_new[s]) / page_rows)
+ * pages: entries from there to n_held[s] go back on the free stack (and become
+ * -1 in the table), then missing ones are taken from it, and n_held[s] is set.
+ * The stack is free_pages[0 .. n_free-1], its top the last; free_pages has room
+ * for n_pages entries. Counted in the order of requests and of pages, the g-th
+ * page given back is put where the g-th page taken is taken from, so a plan
+ * that undoes another restores the stack. (A request of length 0 without new
+ * rows gives back all it held.)
+ *   row_start [n_seqs+1]  first packed row of each request, and the total
+ *   row_slot  [max_rows]  slot of each packed row
+ *   row_pos   [max_rows]  its position: seq_lens[s] + its index in the request,
+ *                         with a tree seq_lens[s] + its depth
+ *   row_mask  [max_rows][mask_words]  with a tree: bit j of the words (bit j % 32
+ *                         of word j / 32) is set where the request's new row j is
+ *                         the row itself or an ancestor
+ * parents [max_rows], packed as the rows: the index within its request of each
+ * new row's parent, -1 for a root. Parents come before their children; a row
+ * for which this fails, or whose ancestor it fails for, is dead: position -1,
+ * mask 0 (it keeps its slot, where an accepted row may land). parents and row_mask are both given or both NULL (the
+ * new rows then follow each other).
+ * status [1] receives WATTN_OK; WATTN_ERR_INVALID (negative lengths, n_held
+ * outside [0, max_pages], a stack that would overflow), WATTN_ERR_RANGE (a
+ * request needs more than max_pages pages or, with a tree, has more than
+ * 32 * mask_words new rows, or the rows exceed max_rows) or WATTN_ERR_NOMEM
+ * (too few free pages). A plan that is refused leaves tables, counts and stack
+ * as they are and describes no rows: row_start all 0, every row padding. */
+int wattn_paged_plan(const int *seq_lens, const int *n_new, int n_seqs, int page_rows,
+                     int n_pages, int *block_table, int64_t table_stride, int max_pages,
+                     int *n_held, int *free_pages, int *n_free, const int *parents,
+                     int *row_start, int *row_pos, int *row_slot, int *row_mask,
+                     int mask_words, int max_rows, int *status, void *stream);
+
+/* K/V rows into the slots of a plan: row r of k_rows / v_rows ([n_rows]
+ * [n_heads*64], type src_dtype, row stride row_stride elements, aligned to the
+ * element size) goes to row_slot[r] of `layer`, rounded to the pool's type.
+ * Rows whose slot is outside the pool (-1) are skipped. No slot may be named
+ * twice. */
+int wattn_paged_write(void *pool, int dtype, int n_pages, int n_layers, int n_heads,
+                      int page_rows, int layer, const int *row_slot, int n_rows,
+                      const void *k_rows, const void *v_rows, int src_dtype,
+                      int64_t row_stride, void *stream);
+
+/* Attention of the new rows over their request's pages in `layer`: row i of
+ * request s attends positions 0 .. seq_lens[s]-1 and those positions
+ * seq_lens[s] + j whose bit j is set in its row of row_mask (row_mask NULL:
+ * j <= i). Positions the mask leaves out have no influence, whatever they
+ * hold; a row that sees nothing gives 0. q and o: packed rows [max_rows]
+ * [n_heads*64], q of the pool's type, o of out_dtype (WATTN_F32 or the pool's
+ * type), 16-byte aligned with row strides (elements) that are multiples of 16
+ * bytes. A table entry outside the pool, lengths beyond max_pages pages or row
+ * starts outside [0, max_rows] make that request's rows unspecified, and
+ * wattn_device_status() reports WATTN_ERR_RANGE. workspace as for
+ * wattn_decode_fwd (wattn_paged_attend_workspace_bytes(), zero-filled before
+ * its first use), or NULL; calls that may overlap, captured graphs among them,
+ * need one each. */
+size_t wattn_paged_attend_workspace_bytes(int n_seqs, int max_rows, int n_heads);
+int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, int n_heads,
+                       int page_rows, int layer, const int *block_table, int64_t table_stride,
+                       int max_pages, const int *seq_lens, const int *row_start, int n_seqs,
+                       const int *row_mask, int mask_words, const void *q,
+                       int64_t q_row_stride, void *o, int out_dtype, int64_t o_row_stride,
+                       int max_rows, float scale, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/* Keeps the drafts that the model agrees with. tokens [max_rows]: each packed
+ * row's token; picked [max_rows]: the token the model picks after that row.
+ * Row 0 of a request (a root) is accepted; after an accepted row r the next is
+ * the lowest child of r whose token is picked[r]. The accepted rows' K/V move,
+ * in every layer, to the slots of the request's first rows, and
+ *   n_accepted [n_seqs]  their number
+ *   path [max_rows]      their indices, packed at row_start[s]; -1 behind them
+ *   next_token [n_seqs]  picked[] of the last one, the request's next token
+ *   seq_lens [n_seqs]    += n_accepted
+ * A request without new rows, or whose row 0 is no root, accepts nothing
+ * (next_token -1). parents, row_start, row_slot as in wattn_paged_plan
+ * (parents NULL: each row's parent is the one before it). The pages beyond the
+ * new length are given back or used by the next plan. */
+int wattn_paged_accept(void *pool, int dtype, int n_pages, int n_layers, int n_heads,
+                       int page_rows, const int *row_start, int n_seqs, int max_rows,
+                       const int *parents, const int *row_slot, const int *tokens,
+                       const int *picked, int *seq_lens, int *n_accepted, int *path,
+                       int *next_token, void *stream);
 
 /* ======================================================================
  * Host-buffer entry points (the reference-facing calls)

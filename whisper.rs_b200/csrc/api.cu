@@ -260,7 +260,10 @@ int consume_status() {
     const int zero[2] = {WATTN_OK, 0};
     cudaMemcpy(sp, zero, sizeof(zero), cudaMemcpyHostToDevice);
     reset_split_counters();
-    return set_error(s[0], "a kernel's bounded wait ran out (site 0x%08x)", s[1]);
+    return set_error(s[0], "%s (site 0x%08x)",
+                     s[0] == WATTN_ERR_RANGE ? "a kernel found a device array out of range"
+                                             : "a kernel's bounded wait ran out",
+                     s[1]);
   }
   return WATTN_OK;
 }
@@ -601,7 +604,8 @@ int wattn_device_status(int device, int *status) {
   if (device >= 0 && device != prev) cudaSetDevice(prev);
   *status = s[0];
   if (rc == WATTN_OK && s[0] != WATTN_OK)
-    set_error(s[0], "bounded wait ran out at site 0x%08x", s[1]);
+    set_error(s[0], "%s at site 0x%08x",
+              s[0] == WATTN_ERR_RANGE ? "device array out of range" : "bounded wait ran out", s[1]);
   return rc;
 }
 

@@ -209,6 +209,14 @@ int launch_decode_paged(const CUtensorMap &map_k, const CUtensorMap &map_v, cons
 // ranges span at most max_keys rows.
 size_t paged_workspace_bytes(int n_rows, int n_heads, int max_keys);
 
+// ----------------------------------------------------------- device-planned pages
+// Pages of the device-planned cache (paged.cu, paged_attend.cu) hold a
+// multiple of this many rows: the smallest TMA box.
+constexpr int kPageRowsUnit = 16;
+// Type, sizes and alignment of a page pool, shared by the paged entry points.
+int check_page_pool(const char *what, const void *pool, int dtype, int n_pages, int n_layers,
+                    int n_heads, int page_rows);
+
 // Library-owned, zero-initialised decode workspace of the calling thread on
 // the current device (grown on demand). Returns NULL on allocation failure.
 void *thread_workspace(size_t bytes, cudaStream_t stream);

@@ -9,7 +9,7 @@
 use std::{env, fs, path::PathBuf, process::Command};
 
 /// Every CUDA source of the library (csrc/<name>.cu).
-const SOURCES: [&str; 7] = [
+const SOURCES: [&str; 9] = [
     "api",
     "attn_f32",
     "attn_tc",
@@ -17,6 +17,8 @@ const SOURCES: [&str; 7] = [
     "decode_noalloc",
     "kv_cache",
     "linear_tc",
+    "paged",
+    "paged_attend",
 ];
 
 const ARCH: [&str; 2] = ["-gencode", "arch=compute_100a,code=sm_100a"];

@@ -15,6 +15,10 @@
 //!   per-layer `append` / `attend` of `decode_batch_inner`
 //!   (decoder.rs:616-647) and `advance` (:765-767).
 //!
+//! The `wattn_paged_*` entry points of [`sys`] (a paged cache whose state is in
+//! the caller's device arrays, for steps that check a tree of drafted tokens)
+//! take device pointers only and have no safe wrapper.
+//!
 //! There is no CPU fallback: head dimensions other than 64 are refused by
 //! the library (`WATTN_ERR_UNSUPPORTED`), which panics here.
 
@@ -151,6 +155,37 @@ pub mod sys {
                                   stream: *mut c_void) -> c_int;
         pub fn wattn_kv_stats(cache: *const wattn_kv_cache, pages_used: *mut c_int,
                               pages_total: *mut c_int) -> c_int;
+
+        pub fn wattn_paged_plan(seq_lens: *const c_int, n_new: *const c_int, n_seqs: c_int,
+                                page_rows: c_int, n_pages: c_int, block_table: *mut c_int,
+                                table_stride: i64, max_pages: c_int, n_held: *mut c_int,
+                                free_pages: *mut c_int, n_free: *mut c_int, parents: *const c_int,
+                                row_start: *mut c_int, row_pos: *mut c_int, row_slot: *mut c_int,
+                                row_mask: *mut c_int, mask_words: c_int, max_rows: c_int,
+                                status: *mut c_int, stream: *mut c_void) -> c_int;
+        pub fn wattn_paged_write(pool: *mut c_void, dtype: c_int, n_pages: c_int, n_layers: c_int,
+                                 n_heads: c_int, page_rows: c_int, layer: c_int,
+                                 row_slot: *const c_int, n_rows: c_int, k_rows: *const c_void,
+                                 v_rows: *const c_void, src_dtype: c_int, row_stride: i64,
+                                 stream: *mut c_void) -> c_int;
+        pub fn wattn_paged_attend_workspace_bytes(n_seqs: c_int, max_rows: c_int,
+                                                  n_heads: c_int) -> usize;
+        pub fn wattn_paged_attend(pool: *const c_void, dtype: c_int, n_pages: c_int,
+                                  n_layers: c_int, n_heads: c_int, page_rows: c_int, layer: c_int,
+                                  block_table: *const c_int, table_stride: i64, max_pages: c_int,
+                                  seq_lens: *const c_int, row_start: *const c_int, n_seqs: c_int,
+                                  row_mask: *const c_int, mask_words: c_int, q: *const c_void,
+                                  q_row_stride: i64, o: *mut c_void, out_dtype: c_int,
+                                  o_row_stride: i64, max_rows: c_int, scale: f32,
+                                  workspace: *mut c_void, workspace_bytes: usize,
+                                  stream: *mut c_void) -> c_int;
+        pub fn wattn_paged_accept(pool: *mut c_void, dtype: c_int, n_pages: c_int, n_layers: c_int,
+                                  n_heads: c_int, page_rows: c_int, row_start: *const c_int,
+                                  n_seqs: c_int, max_rows: c_int, parents: *const c_int,
+                                  row_slot: *const c_int, tokens: *const c_int,
+                                  picked: *const c_int, seq_lens: *mut c_int,
+                                  n_accepted: *mut c_int, path: *mut c_int, next_token: *mut c_int,
+                                  stream: *mut c_void) -> c_int;
 
         pub fn wattn_flash_attention_2(q: *const f32, k: *const f32, v: *const f32, t_q: usize,
                                        t_kv: usize, n_heads: usize, d_model: usize,

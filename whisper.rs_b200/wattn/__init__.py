@@ -10,8 +10,9 @@ Mirrors the reference interface of whisper.rs's attention hot path:
 The four reference-signature functions take host f32 arrays (numpy) in the
 reference layout ``[t, n_heads*64]`` and write ``output`` in place, as the
 Rust functions do; argument errors raise ``WattnError`` where the reference
-panics. ``attention_fwd`` / ``decode_fwd`` and ``DeviceKvCache`` work on CUDA
-tensors (torch) on the caller's current stream.
+panics. ``attention_fwd`` / ``decode_fwd``, ``DeviceKvCache`` and the ``paged_*``
+functions (the cache whose state is on the device) work on CUDA tensors (torch)
+on the caller's current stream.
 
 There is no fallback: if libwattn.so is missing or fails to load, importing
 this module raises.
@@ -28,6 +29,7 @@ __all__ = [
     "flash_attention_2", "multi_head_attention", "single_token_mha_d64",
     "multi_head_attention_with_cache", "attention_host", "decode_host",
     "attention_fwd", "decode_fwd", "decode_fwd_noalloc", "decode_workspace_bytes", "DeviceKvCache",
+    "paged_plan", "paged_write", "paged_attend", "paged_attend_workspace_bytes", "paged_accept",
     "device_status", "selftest_bounded_wait", "EXPORTED_SYMBOLS",
 ]
 
@@ -92,6 +94,14 @@ _SIGS = {
                              _vp]),
     "wattn_kv_read_slot": (_i, [_vp, _i, _i, _i, _vp, _i, _vp]),
     "wattn_kv_stats": (_i, [_vp, _ip, _ip]),
+    "wattn_paged_plan": (_i, [_vp, _vp, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _vp, _vp, _i, _i, _vp, _vp]),
+    "wattn_paged_write": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _i, _i64, _vp]),
+    "wattn_paged_attend_workspace_bytes": (_sz, [_i, _i, _i]),
+    "wattn_paged_attend": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _i64, _i, _vp, _vp, _i, _vp, _i,
+                                _vp, _i64, _vp, _i, _i64, _i, _f, _vp, _sz, _vp]),
+    "wattn_paged_accept": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp,
+                                _vp, _vp, _vp, _vp]),
     "wattn_flash_attention_2": (_i, [_fp, _fp, _fp, _sz, _sz, _sz, _sz, _i, _fp]),
     "wattn_multi_head_attention": (_i, [_fp, _fp, _fp, _sz, _sz, _sz, _sz, _i, _fp]),
     "wattn_single_token_mha_d64": (_i, [_fp, _fp, _fp, _sz, _sz, _sz, _fp]),
@@ -494,3 +504,134 @@ class DeviceKvCache:
         used, total = ctypes.c_int(0), ctypes.c_int(0)
         _check(lib.wattn_kv_stats(self._h, ctypes.byref(used), ctypes.byref(total)), "kv_stats")
         return used.value, total.value
+
+
+# ---------------------------------------------------------------- device-planned paged cache
+# (include/wattn.h, "Device-planned paged cache": the meaning of every array)
+
+def _ints(t, shape, name, device):
+    """Address of an int32 CUDA tensor whose last dimension is dense; None passes."""
+    if t is None:
+        return None
+    if not getattr(t, "is_cuda", False):
+        raise TypeError(f"{name}: device entry points take CUDA tensors")
+    if str(t.dtype) != "torch.int32":
+        raise TypeError(f"{name} must be int32, not {t.dtype}")
+    if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
+        raise WattnError(ERR_INVALID, f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if not t.is_contiguous() and (t.dim() != 2 or name != "block_table" or t.stride(1) != 1):
+        raise WattnError(ERR_INVALID, f"{name} must be contiguous")
+    if t.device != device:
+        raise WattnError(ERR_INVALID, f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr()
+
+
+def _rows(t, n_rows, width, name, device):
+    """(address, row stride) of a 2-D CUDA tensor of dense rows."""
+    if not getattr(t, "is_cuda", False):
+        raise TypeError(f"{name}: device entry points take CUDA tensors")
+    if t.dim() != 2 or t.shape[0] != n_rows or t.shape[1] != width or t.stride(1) != 1:
+        raise WattnError(ERR_INVALID, f"{name} must be [{n_rows}][{width}] with dense rows, not "
+                                      f"{tuple(t.shape)} with strides {tuple(t.stride())}")
+    if t.device != device:
+        raise WattnError(ERR_INVALID, f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr(), t.stride(0) if n_rows > 1 else width
+
+
+def _pool(pool):
+    """(address, dtype, n_pages, n_layers, n_heads, page_rows) of a page pool."""
+    if not getattr(pool, "is_cuda", False):
+        raise TypeError("pool: device entry points take CUDA tensors")
+    if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[5] != 64 or not pool.is_contiguous():
+        raise WattnError(ERR_INVALID, "pool must be contiguous [n_pages][n_layers][2][n_heads]"
+                                      f"[page_rows][64], not {tuple(pool.shape)}")
+    n_pages, n_layers, _, n_heads, page_rows, _ = pool.shape
+    return pool.data_ptr(), _dt_of(pool), n_pages, n_layers, n_heads, page_rows
+
+
+def _call_on(device, stream, fn, *args):
+    """fn(*args, stream) with `device` current."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return fn(*args, _stream_ptr(stream))
+    with torch.cuda.device(device):
+        return fn(*args, _stream_ptr(stream))
+
+
+def paged_plan(seq_lens, n_new, block_table, n_held, free_pages, n_free, row_start, row_pos,
+               row_slot, status, *, page_rows, parents=None, row_mask=None, stream=None) -> None:
+    """``wattn_paged_plan``: block tables, slot maps and (with ``parents`` and
+    ``row_mask`` [max_rows][mask_words]) tree masks from the requests'
+    lengths. Updates block_table, n_held, free_pages and n_free in place and
+    fills row_start, row_pos, row_slot, row_mask and status; all int32."""
+    dev, n, rows = seq_lens.device, seq_lens.shape[0], row_pos.shape[0]
+    table = _ints(block_table, (n, None), "block_table", dev)
+    words = 0 if row_mask is None else row_mask.shape[-1]
+    _check(_call_on(
+        dev, stream, lib.wattn_paged_plan, _ints(seq_lens, (n,), "seq_lens", dev),
+        _ints(n_new, (n,), "n_new", dev), n, page_rows, free_pages.shape[0], table,
+        block_table.stride(0) if n > 1 else block_table.shape[1], block_table.shape[1],
+        _ints(n_held, (n,), "n_held", dev), _ints(free_pages, (None,), "free_pages", dev),
+        _ints(n_free, (1,), "n_free", dev), _ints(parents, (rows,), "parents", dev),
+        _ints(row_start, (n + 1,), "row_start", dev), _ints(row_pos, (rows,), "row_pos", dev),
+        _ints(row_slot, (rows,), "row_slot", dev),
+        _ints(row_mask, (rows, None), "row_mask", dev), words, rows,
+        _ints(status, (1,), "status", dev)), "paged_plan")
+
+
+def paged_write(pool, layer, row_slot, k_rows, v_rows, *, stream=None) -> None:
+    """``wattn_paged_write``: the new rows' K/V ([n_rows][n_heads*64], one row
+    stride) into their slots of ``layer``."""
+    p = _pool(pool)
+    dev, n = pool.device, row_slot.shape[0]
+    k, k_rs = _rows(k_rows, n, p[4] * 64, "k_rows", dev)
+    v, v_rs = _rows(v_rows, n, p[4] * 64, "v_rows", dev)
+    if k_rs != v_rs or k_rows.dtype != v_rows.dtype:
+        raise WattnError(ERR_INVALID, "k_rows and v_rows must have one type and one row stride")
+    _check(_call_on(dev, stream, lib.wattn_paged_write, *p, layer,
+                    _ints(row_slot, (n,), "row_slot", dev), n, k, v, _dt_of(k_rows), k_rs),
+           "paged_write")
+
+
+def paged_attend_workspace_bytes(n_seqs, max_rows, n_heads) -> int:
+    return lib.wattn_paged_attend_workspace_bytes(n_seqs, max_rows, n_heads)
+
+
+def paged_attend(pool, layer, block_table, seq_lens, row_start, q, o, *, row_mask=None,
+                 scale=0.125, workspace=None, stream=None) -> None:
+    """``wattn_paged_attend``: attention of the packed rows ``q`` over their
+    requests' pages and, as ``row_mask`` says (None: causally), each other.
+    ``workspace``: a zero-filled CUDA tensor of at least
+    paged_attend_workspace_bytes() bytes, or None."""
+    p = _pool(pool)
+    dev, n, rows = pool.device, seq_lens.shape[0], q.shape[0]
+    if q.dtype != pool.dtype:
+        raise WattnError(ERR_INVALID, f"q is {q.dtype}, the pool {pool.dtype}")
+    qp, q_rs = _rows(q, rows, p[4] * 64, "q", dev)
+    op, o_rs = _rows(o, rows, p[4] * 64, "o", dev)
+    table = _ints(block_table, (n, None), "block_table", dev)
+    ws_ptr = _dev(workspace) if workspace is not None else None
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _check(_call_on(
+        dev, stream, lib.wattn_paged_attend, *p, layer, table,
+        block_table.stride(0) if n > 1 else block_table.shape[1], block_table.shape[1],
+        _ints(seq_lens, (n,), "seq_lens", dev), _ints(row_start, (n + 1,), "row_start", dev), n,
+        _ints(row_mask, (rows, None), "row_mask", dev),
+        0 if row_mask is None else row_mask.shape[1], qp, q_rs, op, _dt_of(o), o_rs, rows, scale,
+        ws_ptr, ws_bytes), "paged_attend")
+
+
+def paged_accept(pool, row_start, row_slot, tokens, picked, seq_lens, n_accepted, path,
+                 next_token, *, parents=None, stream=None) -> None:
+    """``wattn_paged_accept``: the longest path of drafts the model agrees
+    with: its K/V rows moved together in ``pool``, ``seq_lens`` advanced,
+    n_accepted, path and next_token filled; all int32."""
+    p = _pool(pool)
+    dev, n, rows = pool.device, seq_lens.shape[0], row_slot.shape[0]
+    _check(_call_on(
+        dev, stream, lib.wattn_paged_accept, *p, _ints(row_start, (n + 1,), "row_start", dev), n,
+        rows, _ints(parents, (rows,), "parents", dev), _ints(row_slot, (rows,), "row_slot", dev),
+        _ints(tokens, (rows,), "tokens", dev), _ints(picked, (rows,), "picked", dev),
+        _ints(seq_lens, (n,), "seq_lens", dev), _ints(n_accepted, (n,), "n_accepted", dev),
+        _ints(path, (rows,), "path", dev), _ints(next_token, (n,), "next_token", dev)),
+        "paged_accept")
