@@ -666,8 +666,10 @@ def test_bad_tables_are_reported_and_harmless(W):
     the other requests are right and the status word says so."""
     for what in ("page", "page_low", "len", "len_low", "start", "start_back"):
         b = Batch(41, "f16", [100, 40, 70], [3, 2, 4], 2, 16)
-        want = b.attend(W, 1, "f32")
-        assert W.device_status() == 0
+        ref, mag, top = (x[:3] for x in P.attend(
+            b.pool.float().cpu().numpy(), 1, b.st.table, b.lens, b.start,
+            b.q.float().cpu().numpy()[:9], 2, 0.125))
+        lim = bound("f16", "f32", ref, mag, top, 110, 6.0)
         if what == "page":
             b.st.table[1, 0] = b.n_pages
         elif what == "page_low":
@@ -686,7 +688,8 @@ def test_bad_tables_are_reported_and_harmless(W):
         W.paged_attend(b.pool, 1, table, lens, start, b.q, o)
         torch.cuda.synchronize()
         assert W.device_status() == -6, what
-        assert np.array_equal(o[:3].cpu().numpy(), want[:3].astype(np.float32)), what
+        # (not bit for bit: the lengths of the others move the cuts of the keys)
+        assert (np.abs(o[:3].cpu().numpy() - ref) <= lim).all(), what
 
 
 def test_refusals(W):
