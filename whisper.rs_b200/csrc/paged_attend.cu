@@ -3,13 +3,16 @@
 // cached positions and those of the request's new rows that its mask names
 // (without masks: rows 0..i, the causal rule of decoder.rs:864).
 //
-// 16-bit pools: a persistent grid streams K and V once per tile of 64 rows.
-// The unit of work is a 64-key sub-tile of one (request, head, row tile). The
-// lengths are on the device, so every CTA adds up the requests' units itself
-// and takes an equal share of them in order, wherever that cuts a row
-// tile's keys (the parts of a cut one are merged by log-sum-exp, in order,
-// by the CTA that finishes last: same inputs, same bits).
-
+// 16-bit pools. Bound: HBM (each key's K and V, 256 bytes, meet up to 32
+// query rows: 4 * 64 * 32 products on the tensor cores for 256 bytes). Every
+// warp streams for itself: it has its own ring of two 32-key stages, loads
+// them by TMA through the block table and multiplies with mma.sync; warps
+// meet only when they are done. The unit of work is one stage of one item
+// (request, head, tile of up to 32 rows). The lengths are on the device, so
+// each CTA adds up the requests' units itself and each warp takes an equal
+// share of them, in order, wherever that cuts an item's keys. The parts of a
+// cut item are merged by log-sum-exp in the order of the keys, by its CTA or,
+// where it spans several, by the last of them: same inputs, same bits.
 #include <algorithm>
 
 #include "wattn_common.cuh"
@@ -36,22 +39,22 @@ struct PagedAttendParams {
   float scale_log2;
   int cap;       // positions that the table can hold
   int box_rows;  // rows of a TMA box of whole sub-tiles
-  float *part;   // partials of cut items, two per CTA
-  int *count;    // finished shares of the item that each CTA's share starts
+  float *part;   // partials of cut items, two per warp
+  int *count;    // finished CTAs of the item that each CTA starts and another ends
   int *status;
 };
 
 // ---------------------------------------------------------------- shares of the work
 
-constexpr int kPaSub = 64;        // keys of a sub-tile
+constexpr int kPaKeys = 32;       // keys of a stage
 constexpr int kPaTail = 16;       // rows of a tail box: the pool's unit of page rows
-constexpr int kPaRows = 64;       // rows of a row tile
-constexpr int kPaStages = 3;      // sub-tiles of the K/V ring: three CTAs to an SM
-constexpr int kPaWarps = 4;       // compute warps; one more warp issues the loads
-constexpr int kPaThreads = (kPaWarps + 1) * 32;
+constexpr int kPaRows = 32;       // rows of a row tile
+constexpr int kPaStages = 2;      // stages of a warp's ring
+constexpr int kPaWarps = 4;
+constexpr int kPaThreads = kPaWarps * 32;
 constexpr int kPaCtasPerSm = 3;
-constexpr int kPaMinUnits = 4;    // units of a share below which fewer CTAs work
-constexpr int kPaRedStride = 72;  // floats per row of the merge buffer: no bank met twice
+constexpr int kPaMinUnits = 4;    // units of a share below which fewer warps work
+constexpr int kPaQueue = 4;       // items a warp may have loads for, and one more
 constexpr int kPaPartStride = 68; // floats per row of a partial: acc[64], m, l
 
 // One request as the kernel sees it, its arrays' values forced into range.
@@ -82,9 +85,9 @@ WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
              ? q.end
              : (int)min((int64_t)q.len + min(q.n, kPaRows * (rt + 1)), (int64_t)q.end);
 }
-// Units of one row tile: its sub-tiles, and one for what an item costs besides.
+// Units of one row tile: its stages, and one for what an item costs besides.
 WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return (pa_end(p, q, rt) + kPaSub - 1) / kPaSub + 1;
+  return (pa_end(p, q, rt) + kPaKeys - 1) / kPaKeys + 1;
 }
 // Units of one head of a request.
 WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
@@ -94,53 +97,54 @@ WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q)
   return u;
 }
 
-// A walk over the items (request, head, row tile) of one CTA's share
-// [lo, hi) of the units; `at` is the unit at which the current item starts.
-struct PaWalk {
-  PaSeq q;
-  int s, head, rt, units;
-  long long at, lo, hi;
-};
-WATTN_DEVINL bool pa_more(const PaWalk &w) { return w.at < w.hi; }
-WATTN_DEVINL void pa_next(const PagedAttendParams &p, PaWalk &w) {
-  w.at += w.units;
-  if (w.at >= w.hi) return;
-  if (++w.rt == w.q.row_tiles) {
-    w.rt = 0;
-    if (++w.head == p.n_heads) {
-      w.head = 0;
-      do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
-    }
-  }
-  w.units = pa_units(p, w.q, w.rt);
-}
-// The current item's sub-tiles of this share.
-WATTN_DEVINL int pa_from(const PaWalk &w) { return (int)max(0ll, w.lo - w.at); }
-WATTN_DEVINL int pa_to(const PaWalk &w) { return (int)min((long long)w.units - 1, w.hi - w.at); }
-
 // The share that unit u belongs to, of `parts` shares of `total` units:
 // share c is [c * total / parts, (c + 1) * total / parts).
 WATTN_DEVINL int pa_owner(long long u, long long total, int parts) {
   return (int)(((u + 1) * parts - 1) / total);
 }
 
-struct PaShare {
-  long long total;
-  int parts;
+// Where a warp's share [lo, hi) begins: in units `at` .. `at` + units of the
+// item (s, head, rt).
+struct PaStart {
+  PaSeq q;
+  int s, head, rt, units;
+  long long at, lo, hi;
 };
 
-// The CTA's share, found by all its threads: each adds up the units of a
-// run of requests, the sums are scanned, and the thread whose run holds the
-// share's first unit walks to the item that holds it.
-WATTN_DEVINL void pa_find_share(const PagedAttendParams &p, PaWalk &walk, PaShare &share,
-                                long long *warp_sums, PaWalk *s_walk) {
+// An item of a warp's share, as the loads announce it to the products.
+struct PaItem {
+  int row0, nr;      // packed rows of the tile
+  int row, n;        // the tile's first row in the request, the request's rows
+  int len, end;      // cached positions, positions that some row may see
+  int head;
+  int from, to, stages;  // stages of this share, of the item
+  long long at;      // the item's first unit
+};
+
+struct PaSmem {
+  uint8_t k[kPaWarps][kPaStages][kPaKeys * 128];
+  uint8_t v[kPaWarps][kPaStages][kPaKeys * 128];
+  uint64_t full[kPaWarps][kPaStages];
+  PaItem queue[kPaWarps][kPaQueue];
+  PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
+  PaStart start[kPaWarps];
+  long long warp_sums[kPaWarps];
+  long long total;
+  int parts;
+  int abort, last;
+};
+
+// The warps' shares, found by all threads of the CTA: each adds up the units
+// of a run of requests, the sums are scanned, and the thread whose run holds
+// a share's first unit walks to the item that holds it.
+WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.n_seqs + kPaThreads - 1) / kPaThreads;
   const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
   long long mine = 0;
-  for (int s = s0; s < s1; ++s) {
+  for (int i = s0; i < s1; ++i) {
     bool bad;
-    const PaSeq q = pa_seq(p, s, &bad);
+    const PaSeq q = pa_seq(p, i, &bad);
     if (bad) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
     mine += pa_head_units(p, q) * p.n_heads;
   }
@@ -150,45 +154,50 @@ WATTN_DEVINL void pa_find_share(const PagedAttendParams &p, PaWalk &walk, PaShar
     const long long y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  if (lane == 31) warp_sums[warp] = inc;
+  if (lane == 31) s.warp_sums[warp] = inc;
   __syncthreads();
   long long before = inc - mine, total = 0;
 #pragma unroll
-  for (int w = 0; w < kPaWarps + 1; ++w) {
-    if (w < warp) before += warp_sums[w];
-    total += warp_sums[w];
+  for (int w = 0; w < kPaWarps; ++w) {
+    if (w < warp) before += s.warp_sums[w];
+    total += s.warp_sums[w];
   }
-  share.total = total;
-  share.parts = (int)max(1ll, min((long long)gridDim.x, total / kPaMinUnits));
-  const long long lo = blockIdx.x * total / share.parts;
-  const long long hi = (int)blockIdx.x < share.parts ? (blockIdx.x + 1) * total / share.parts : lo;
-  if (lo < hi && before <= lo && lo < before + mine) {
-    PaWalk w;
-    w.lo = lo;
-    w.hi = hi;
-    w.at = before;
-    for (w.s = s0;; ++w.s) {
-      w.q = pa_seq(p, w.s, nullptr);
-      const long long u = pa_head_units(p, w.q);
-      if (lo < w.at + u * p.n_heads) {
-        w.head = (int)((lo - w.at) / u);
-        w.at += w.head * u;
-        break;
+  const int parts = (int)max(1ll, min((long long)gridDim.x * kPaWarps, total / kPaMinUnits));
+  if (tid == 0) {
+    s.total = total;
+    s.parts = parts;
+  }
+#pragma unroll 1
+  for (int k = 0; k < kPaWarps; ++k) {
+    const int c = blockIdx.x * kPaWarps + k;
+    const long long lo = c < parts ? c * total / parts : 0;
+    const long long hi = c < parts ? (c + 1) * total / parts : 0;
+    if (lo >= hi) {
+      if (tid == 0) s.start[k].lo = s.start[k].hi = 0;
+    } else if (before <= lo && lo < before + mine) {
+      PaStart w;
+      w.lo = lo;
+      w.hi = hi;
+      w.at = before;
+      for (w.s = s0;; ++w.s) {
+        w.q = pa_seq(p, w.s, nullptr);
+        const long long u = pa_head_units(p, w.q);
+        if (lo < w.at + u * p.n_heads) {
+          w.head = (int)((lo - w.at) / u);
+          w.at += w.head * u;
+          break;
+        }
+        w.at += u * p.n_heads;
       }
-      w.at += u * p.n_heads;
+      for (w.rt = 0;; ++w.rt) {
+        w.units = pa_units(p, w.q, w.rt);
+        if (lo < w.at + w.units) break;
+        w.at += w.units;
+      }
+      s.start[k] = w;
     }
-    for (w.rt = 0;; ++w.rt) {
-      w.units = pa_units(p, w.q, w.rt);
-      if (lo < w.at + w.units) break;
-      w.at += w.units;
-    }
-    *s_walk = w;
-  }
-  if (tid == 0 && lo >= hi) {
-    s_walk->lo = s_walk->hi = s_walk->at = 0;
   }
   __syncthreads();
-  walk = *s_walk;
 }
 
 // ---------------------------------------------------------------- 16-bit pools
@@ -201,17 +210,6 @@ template <> struct PaType<__half> {
 template <> struct PaType<__nv_bfloat16> {
   static constexpr uint32_t kOne = 0x3f80u, kInf = 0x7f80u;
   static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
-};
-
-struct PaSmem {
-  uint8_t k[kPaStages][kPaSub * 128];
-  uint8_t v[kPaStages][kPaSub * 128];
-  float red[kPaWarps][16][kPaRedStride];
-  float wm[kPaWarps][16], wl[kPaWarps][16];
-  uint64_t kfull[kPaStages], vfull[kPaStages], empty[kPaStages];
-  long long warp_sums[kPaWarps + 1];
-  PaWalk walk;
-  int abort, last;
 };
 
 template <typename T>
@@ -232,17 +230,19 @@ WATTN_DEVINL void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uin
 WATTN_DEVINL void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
 WATTN_DEVINL void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+               : "r"(addr)
+               : "memory");
 }
-WATTN_DEVINL void pa_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // Which of the 32 positions from seq_lens + off on row i sees, as bits: all
-// of the cached ones (off < 0), then the row's mask, or the rows up to itself.
+// of the cached ones (off < 0), then the row's mask, or the rows up to itself;
+// `left` positions of them exist.
 WATTN_DEVINL uint32_t pa_mask_word(const PagedAttendParams &p, int packed, int i, int w) {
   if (w < 0) return 0xffffffffu;
   if (p.row_mask == nullptr) {
@@ -252,10 +252,9 @@ WATTN_DEVINL uint32_t pa_mask_word(const PagedAttendParams &p, int packed, int i
   return w < p.mask_words ? (uint32_t)p.row_mask[(int64_t)packed * p.mask_words + w] : 0u;
 }
 WATTN_DEVINL uint32_t pa_visible(const PagedAttendParams &p, int packed, int i, int off, int left) {
-  if (left <= 0) return 0u;
   const int w = off >> 5;
-  uint32_t bits = __funnelshift_r(pa_mask_word(p, packed, i, w), pa_mask_word(p, packed, i, w + 1),
-                                  off & 31);
+  const uint32_t bits = __funnelshift_r(pa_mask_word(p, packed, i, w),
+                                        pa_mask_word(p, packed, i, w + 1), off & 31);
   return left >= 32 ? bits : bits & ((1u << left) - 1u);
 }
 
@@ -265,194 +264,13 @@ template <typename T> WATTN_DEVINL uint32_t pa_not_finite(uint32_t w) {
   return __vcmpeq2(w & kInf2, kInf2);
 }
 
-// State of a warp's 16 query rows over an item: this lane's rows are g and g + 8.
-struct PaAcc {
-  float o[8][4];
-  float m[2], l[2];
-};
-
-// One sub-tile's SL 16-key slices of this warp (slices kg, kg + 4 / SL, ...).
-// few: at most 8 query rows in the tile of 16; its rows 8..15 then carry the
-// weights' rounding residuals and cost no further products.
-template <typename T, int SL>
-WATTN_DEVINL void pa_sub_tile(const PagedAttendParams &p, const uint32_t (&qa)[4][4], PaAcc &a,
-                              uint32_t ktile, uint32_t vtile, uint64_t *vbar, uint32_t ph,
-                              volatile int *abort, int kg, bool few, int packed, int row, int n,
-                              int off, int left, int lane) {
-  constexpr int KG = kPaWarps / SL;
-  const int g = lane >> 2, t4 = lane & 3;
-  float sc[SL][2][4];
-#pragma unroll
-  for (int i = 0; i < SL; ++i) {
-    const int j = kg + KG * i;
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      sc[i][nb][0] = sc[i][nb][1] = sc[i][nb][2] = sc[i][nb][3] = 0.f;
-      const int key = j * 16 + nb * 8 + (lane & 7);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        uint32_t r[4];
-        pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r);
-        pa_mma<T>(sc[i][nb], qa[2 * ks], r[0], r[1]);
-        pa_mma<T>(sc[i][nb], qa[2 * ks + 1], r[2], r[3]);
-      }
-    }
-  }
-  // off: first position of the sub-tile less seq_lens; left: positions of it
-  // that any row may see.
-  const bool drafts = off + kPaSub > 0;
-  if (drafts || left < kPaSub) {
-#pragma unroll
-    for (int i = 0; i < SL; ++i) {
-      const int j16 = (kg + KG * i) * 16;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t vis =
-            row + 8 * h < n ? pa_visible(p, packed + 8 * h, row + 8 * h, off + j16, left - j16) : 0u;
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!(vis >> (nb * 8 + 2 * t4 + e) & 1u)) sc[i][nb][2 * h + e] = -INFINITY;
-      }
-    }
-  }
-  float mu[2] = {0.f, 0.f};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (few && h == 1) break;  // no rows there
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < SL; ++i)
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb) mx = fmaxf(mx, fmaxf(sc[i][nb][2 * h], sc[i][nb][2 * h + 1]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float mc = mx * p.scale_log2;
-    if (mc > a.m[h] + 8.0f) {  // rescale only when the running max grows by more than 2^8
-      const float alpha = ex2(a.m[h] - mc);
-      a.l[h] *= alpha;
-#pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        a.o[db][2 * h] *= alpha;
-        a.o[db][2 * h + 1] *= alpha;
-      }
-      if (few)  // rows 8..15 hold the residuals of rows 0..7
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-          a.o[db][2] *= alpha;
-          a.o[db][3] *= alpha;
-        }
-      a.m[h] = mc;
-    }
-    mu[h] = a.m[h] == -INFINITY ? 0.f : a.m[h];
-  }
-  mbar_wait(vbar, ph, abort, p.status, (4 << 24) | (2 << 16));
-#pragma unroll
-  for (int i = 0; i < SL; ++i) {
-    const int j16 = (kg + KG * i) * 16;
-    float pe[2][4];
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        pe[nb][e] = ex2(fmaf(sc[i][nb][e], p.scale_log2, -mu[e >> 1]));
-    uint32_t pa[4], pr[4];
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      a.l[0] += pe[nb][0] + pe[nb][1];
-      pa[2 * nb] = pack2<T>(pe[nb][0], pe[nb][1]);
-      const float2 r0 = unpack2<T>(pa[2 * nb]);
-      const uint32_t lo = pack2<T>(pe[nb][0] - r0.x, pe[nb][1] - r0.y);
-      if (few) {
-        pa[2 * nb + 1] = lo;
-      } else {
-        a.l[1] += pe[nb][2] + pe[nb][3];
-        pa[2 * nb + 1] = pack2<T>(pe[nb][2], pe[nb][3]);
-        if constexpr (PaType<T>::kResidual) {
-          const float2 r1 = unpack2<T>(pa[2 * nb + 1]);
-          pr[2 * nb] = lo;
-          pr[2 * nb + 1] = pack2<T>(pe[nb][2] - r1.x, pe[nb][3] - r1.y);
-        }
-      }
-    }
-    // Value rows behind the last position hold anything: zero for the product.
-    const bool part = left - j16 < 16;
-    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-    if (part) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int k0 = j16 + b * 8 + 2 * t4;
-        keep[b] = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
-      }
-    }
-    const int key = j16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-    uint32_t vr[4][4];
-    uint32_t odd = 0;
-#pragma unroll
-    for (int d2 = 0; d2 < 4; ++d2)
-      pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr[d2]);
-    if (part) {
-#pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vr[d2][e] &= keep[e & 1];
-    }
-    if (drafts) {
-      // A draft's value that is infinite or NaN reaches the rows that see
-      // it and, as 0 times it, would spoil those that do not.
-#pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= pa_not_finite<T>(vr[d2][e]);
-      if (__any_sync(0xffffffffu, odd != 0)) {
-        uint32_t sees[4];
-        constexpr uint32_t one = PaType<T>::kOne;
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            sees[2 * nb + h] = (sc[i][nb][2 * h] != -INFINITY ? one : 0u) |
-                               (sc[i][nb][2 * h + 1] != -INFINITY ? one << 16 : 0u);
-        if (few) sees[1] = sees[3] = 0u;
-        constexpr uint32_t inf2 = PaType<T>::kInf * 0x10001u;
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-          uint32_t *v = &vr[db >> 1][(db & 1) * 2];
-          // counts of +inf, -inf and NaN values that each row sees
-          float np[4] = {0, 0, 0, 0}, nm[4] = {0, 0, 0, 0}, nn[4] = {0, 0, 0, 0};
-          uint32_t up[2], down[2], nan[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            up[b] = __vcmpeq2(v[b], inf2) & (one * 0x10001u);
-            down[b] = __vcmpeq2(v[b], inf2 | 0x80008000u) & (one * 0x10001u);
-            nan[b] = __vcmpgtu2(v[b] & 0x7fff7fffu, inf2) & (one * 0x10001u);
-            v[b] &= ~pa_not_finite<T>(v[b]);
-          }
-          pa_mma<T>(np, sees, up[0], up[1]);
-          pa_mma<T>(nm, sees, down[0], down[1]);
-          pa_mma<T>(nn, sees, nan[0], nan[1]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (np[e] > 0.f) a.o[db][e] += INFINITY;
-            if (nm[e] > 0.f) a.o[db][e] -= INFINITY;
-            if (nn[e] > 0.f) a.o[db][e] = NAN;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      const uint32_t b0 = vr[db >> 1][(db & 1) * 2], b1 = vr[db >> 1][(db & 1) * 2 + 1];
-      pa_mma<T>(a.o[db], pa, b0, b1);
-      if constexpr (PaType<T>::kResidual)
-        if (!few) pa_mma<T>(a.o[db], pr, b0, b1);
-    }
-  }
+template <typename OutT> WATTN_DEVINL void pa_store2(void *o, int64_t at, float x, float y) {
+  if constexpr (sizeof(OutT) == 4)
+    *reinterpret_cast<float2 *>(reinterpret_cast<float *>(o) + at) = make_float2(x, y);
+  else
+    *reinterpret_cast<uint32_t *>(reinterpret_cast<OutT *>(o) + at) = pack2<OutT>(x, y);
 }
-
-template <typename OutT>
-WATTN_DEVINL void pa_store4(void *o, int64_t at, float4 x) {
+template <typename OutT> WATTN_DEVINL void pa_store4(void *o, int64_t at, float4 x) {
   if constexpr (sizeof(OutT) == 4)
     *reinterpret_cast<float4 *>(reinterpret_cast<float *>(o) + at) = x;
   else
@@ -460,61 +278,368 @@ WATTN_DEVINL void pa_store4(void *o, int64_t at, float4 x) {
         make_uint2(pack2<OutT>(x.x, x.y), pack2<OutT>(x.z, x.w));
 }
 
-// The partial of share c for an item that share c0 starts.
-WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, int c0) {
-  return p.part + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * kPaRows * kPaPartStride;
+// The partial of share c for a cut item that share c0 starts.
+WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, bool starts) {
+  return p.part + ((int64_t)c * 2 + (starts ? 1 : 0)) * kPaRows * kPaPartStride;
 }
 
-// An item's rows from the merged sums in `red`: stored, or, for an item cut
-// by a share's end, left as a partial and merged with the others by the last
-// of its shares to finish. KG warps share each tile of 16 rows.
+// The loads of a warp's share, running ahead of its products.
+struct PaLoads {
+  PaStart w;
+  int t, to;             // next stage and end within the current item
+  uint32_t issued;       // stages issued
+  uint32_t announced;    // items announced
+  int have_s, base, entry;  // lane i holds table entry base + i of request have_s
+  bool more;
+};
+
+// Announces the next item of the share that has stages in it.
+template <typename T>
+WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, int warp, int lane,
+                              bool first) {
+  PaStart &w = ld.w;
+  for (;;) {
+    if (!first) {
+      w.at += w.units;
+      if (w.at >= w.hi) {
+        ld.more = false;
+        return;
+      }
+      if (++w.rt == w.q.row_tiles) {
+        w.rt = 0;
+        if (++w.head == p.n_heads) {
+          w.head = 0;
+          do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
+        }
+      }
+      w.units = pa_units(p, w.q, w.rt);
+    }
+    first = false;
+    ld.t = (int)max(0ll, w.lo - w.at);
+    ld.to = (int)min((long long)w.units - 1, w.hi - w.at);
+    if (ld.t < ld.to) break;
+  }
+  const int row = w.rt * kPaRows, row0 = w.q.first + row, nr = min(kPaRows, w.q.n - row);
+  if (lane == 0) {
+    PaItem &it = s.queue[warp][ld.announced % kPaQueue];
+    it.row0 = row0;
+    it.nr = nr;
+    it.row = row;
+    it.n = w.q.n;
+    it.len = w.q.len;
+    it.end = pa_end(p, w.q, w.rt);
+    it.head = w.head;
+    it.from = ld.t;
+    it.to = ld.to;
+    it.stages = w.units - 1;
+    it.at = w.at;
+  }
+  if (lane < nr)  // the products will want the query rows soon
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const T *>(p.q) +
+                                                  (int64_t)(row0 + lane) * p.q_rs + w.head * 64));
+  ++ld.announced;
+}
+
+// Issues the next stage's loads into the ring slot that the products have left.
+template <typename T>
+WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
+                           const CUtensorMap &map_tail, int warp, int lane) {
+  if (!ld.more) return;
+  const int slot = ld.issued % kPaStages;
+  const int key = ld.t * kPaKeys;
+  const int rows = min(kPaKeys, pa_end(p, ld.w.q, ld.w.rt) - key);
+  const bool tail = rows < kPaKeys;
+  const int step = tail ? kPaTail : p.box_rows;
+  const int boxes = (rows + step - 1) / step;
+  uint64_t *bar = &s.full[warp][slot];
+  if (lane == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);
+#pragma unroll 1
+  for (int b = 0; b < boxes; ++b) {
+    const int at = key + b * step;
+    const int pi = at / p.page_rows;
+    if (ld.have_s != ld.w.s || pi < ld.base || pi >= ld.base + 32) {
+      ld.have_s = ld.w.s;
+      ld.base = pi;
+      ld.entry = pi + lane < p.max_pages ? p.table[ld.w.s * p.table_stride + pi + lane] : 0;
+    }
+    int page = __shfl_sync(0xffffffffu, ld.entry, pi - ld.base);
+    if (page < 0 || page >= p.n_pages) {
+      if (lane == 0) report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
+      page = 0;
+    }
+    if (lane == 0) {
+      const int rk = ((page * p.n_layers + p.layer) * 2 * p.n_heads + ld.w.head) * p.page_rows + at -
+                     pi * p.page_rows;
+      const int rv = rk + p.n_heads * p.page_rows;
+      const CUtensorMap *m = tail ? &map_tail : &map;
+      tma_load_2d(s.k[warp][slot] + b * step * 128, m, bar, 0, rk);
+      tma_load_2d(s.v[warp][slot] + b * step * 128, m, bar, 0, rv);
+    }
+  }
+  ++ld.issued;
+  if (++ld.t == ld.to) pa_announce<T>(p, s, ld, warp, lane, false);
+  __syncwarp();
+}
+
+// The products of one item's stages: MT tiles of 16 query rows against 32
+// keys a stage. FEW (at most 8 rows): rows 8..15 of the tile carry the
+// weights' rounding residuals and cost no further products.
+template <typename T, typename OutT, int MT, bool FEW>
+WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
+                          const CUtensorMap &map_tail, const PaItem &it, uint32_t &pos, int warp,
+                          int lane) {
+  const int g = lane >> 2, t4 = lane & 3;
+  uint32_t qa[MT][4][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = mt * 16 + h * 8 + g;
+      const uint32_t *q = reinterpret_cast<const uint32_t *>(
+          reinterpret_cast<const T *>(p.q) + (int64_t)(it.row0 + r) * p.q_rs + it.head * 64);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        qa[mt][ks][h] = !(FEW && h) && r < it.nr ? q[ks * 8 + t4] : 0u;
+        qa[mt][ks][2 + h] = !(FEW && h) && r < it.nr ? q[ks * 8 + 4 + t4] : 0u;
+      }
+    }
+  float o[MT][8][4], m[MT][2], l[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int db = 0; db < 8; ++db) o[mt][db][0] = o[mt][db][1] = o[mt][db][2] = o[mt][db][3] = 0.f;
+    m[mt][0] = m[mt][1] = -INFINITY;
+    l[mt][0] = l[mt][1] = 0.f;
+  }
+#pragma unroll 1
+  for (int t = it.from; t < it.to; ++t, ++pos) {
+    const int slot = pos % kPaStages;
+    mbar_wait(&s.full[warp][slot], (pos / kPaStages) & 1, &s.abort, p.status,
+              (4 << 24) | (1 << 16) | ((pos & 0xff) << 8));
+    const uint32_t ktile = smem_u32(s.k[warp][slot]), vtile = smem_u32(s.v[warp][slot]);
+    float sc[MT][4][4];
+#pragma unroll
+    for (int nb = 0; nb < 4; ++nb) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sc[mt][nb][0] = sc[mt][nb][1] = sc[mt][nb][2] = sc[mt][nb][3] = 0.f;
+      const int key = nb * 8 + (lane & 7);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t r[4];
+        pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          pa_mma<T>(sc[mt][nb], qa[mt][2 * ks], r[0], r[1]);
+          pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + 1], r[2], r[3]);
+        }
+      }
+    }
+    const int off = t * kPaKeys - it.len, left = it.end - t * kPaKeys;
+    const bool drafts = off + kPaKeys > 0;       // the stage reaches past the cached positions
+    const bool special = drafts || left < kPaKeys;
+    if (special) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+          const int r = mt * 16 + h * 8 + g;
+          const uint32_t vis = r < it.nr ? pa_visible(p, it.row0 + r, it.row + r, off, left) : 0u;
+#pragma unroll
+          for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!(vis >> (nb * 8 + 2 * t4 + e) & 1u)) sc[mt][nb][2 * h + e] = -INFINITY;
+        }
+    }
+    float mu[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb) mx = fmax3(mx, sc[mt][nb][2 * h], sc[mt][nb][2 * h + 1]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mc = mx * p.scale_log2;
+        if (mc > m[mt][h] + 8.0f) {  // rescale only when the running max grows by more than 2^8
+          const float alpha = ex2(m[mt][h] - mc);
+          l[mt][h] *= alpha;
+#pragma unroll
+          for (int db = 0; db < 8; ++db) {
+            o[mt][db][2 * h] *= alpha;
+            o[mt][db][2 * h + 1] *= alpha;
+            if (FEW) {
+              o[mt][db][2] *= alpha;
+              o[mt][db][3] *= alpha;
+            }
+          }
+          m[mt][h] = mc;
+        }
+        mu[mt][h] = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
+      }
+    // Value rows behind the last position hold anything: zero for the
+    // product. A draft's value that is infinite or NaN belongs to the rows
+    // that see it and would, as 0 times it, spoil those that do not.
+    uint32_t odd = 0;
+    if (drafts) {
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+        for (int d2 = 0; d2 < 4; ++d2) {
+          const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+          uint32_t vr[4];
+          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k0 = sl * 16 + (e & 1) * 8 + 2 * t4;
+            odd |= pa_not_finite<T>(vr[e]) &
+                   ((k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u));
+          }
+        }
+      odd = __any_sync(0xffffffffu, odd != 0);
+    }
+    if (__builtin_expect(odd != 0, 0)) {
+      constexpr uint32_t one2 = PaType<T>::kOne * 0x10001u, inf2 = PaType<T>::kInf * 0x10001u;
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {
+        uint32_t sees[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int nb = sl * 2 + (e >> 1), h = e & 1;
+            sees[mt][e] = FEW && h ? 0u
+                                   : ((sc[mt][nb][2 * h] != -INFINITY ? 0xffffu : 0u) |
+                                      (sc[mt][nb][2 * h + 1] != -INFINITY ? 0xffff0000u : 0u)) & one2;
+          }
+#pragma unroll
+        for (int d2 = 0; d2 < 4; ++d2) {
+          const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+          uint32_t vr[4];
+          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k0 = sl * 16 + (e & 1) * 8 + 2 * t4;
+            vr[e] &= (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              // how many +inf, -inf and NaN values each row sees
+              float np[4] = {0, 0, 0, 0}, nm[4] = {0, 0, 0, 0}, nn[4] = {0, 0, 0, 0};
+              const uint32_t v0 = vr[2 * half], v1 = vr[2 * half + 1];
+              pa_mma<T>(np, sees[mt], __vcmpeq2(v0, inf2) & one2, __vcmpeq2(v1, inf2) & one2);
+              pa_mma<T>(nm, sees[mt], __vcmpeq2(v0, inf2 | 0x80008000u) & one2,
+                        __vcmpeq2(v1, inf2 | 0x80008000u) & one2);
+              pa_mma<T>(nn, sees[mt], __vcmpgtu2(v0 & 0x7fff7fffu, inf2) & one2,
+                        __vcmpgtu2(v1 & 0x7fff7fffu, inf2) & one2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float &x = o[mt][2 * d2 + half][e];
+                if (np[e] > 0.f) x += INFINITY;
+                if (nm[e] > 0.f) x -= INFINITY;
+                if (nn[e] > 0.f) x = NAN;
+              }
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int sl = 0; sl < 2; ++sl) {
+      uint32_t pa[MT][4], pr[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2) {
+          const float *x = sc[mt][sl * 2 + n2];
+#pragma unroll
+          for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+            const float e0 = ex2(fmaf(x[2 * h], p.scale_log2, -mu[mt][h]));
+            const float e1 = ex2(fmaf(x[2 * h + 1], p.scale_log2, -mu[mt][h]));
+            l[mt][h] += e0 + e1;
+            const uint32_t hi = pack2<T>(e0, e1);
+            pa[mt][2 * n2 + h] = hi;
+            if (FEW || PaType<T>::kResidual) {
+              const float2 r = unpack2<T>(hi);
+              const uint32_t lo = pack2<T>(e0 - r.x, e1 - r.y);
+              if (FEW) pa[mt][2 * n2 + 1] = lo; else pr[mt][2 * n2 + h] = lo;
+            }
+          }
+        }
+      const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+      for (int d2 = 0; d2 < 4; ++d2) {
+        uint32_t vr[4];
+        pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+        if (special) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k0 = sl * 16 + (e & 1) * 8 + 2 * t4;
+            vr[e] &= (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
+            if (odd) vr[e] &= ~pa_not_finite<T>(vr[e]);
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            pa_mma<T>(o[mt][2 * d2 + half], pa[mt], vr[2 * half], vr[2 * half + 1]);
+            if constexpr (!FEW && PaType<T>::kResidual)
+              pa_mma<T>(o[mt][2 * d2 + half], pr[mt], vr[2 * half], vr[2 * half + 1]);
+          }
+      }
+    }
+    __syncwarp();  // every lane has read the stage
+    pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
+  }
+  const bool whole = it.from == 0 && it.to == it.stages;
+  const bool starts = it.from == 0;
+  if (!whole && lane == 0) s.cut[warp][starts ? 1 : 0] = it;
+  float *part = whole ? nullptr : pa_part(p, blockIdx.x * kPaWarps + warp, starts);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+      float sum = l[mt][h];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      const int r = mt * 16 + h * 8 + g;
+      if (r >= it.nr) continue;
+      const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        float x = o[mt][db][2 * h], y = o[mt][db][2 * h + 1];
+        if (FEW) {
+          x += o[mt][db][2];
+          y += o[mt][db][3];
+        }
+        x *= inv;
+        y *= inv;
+        if (whole)
+          pa_store2<OutT>(p.o, (int64_t)(it.row0 + r) * p.o_rs + it.head * 64 + db * 8 + 2 * t4, x, y);
+        else
+          *reinterpret_cast<float2 *>(part + r * kPaPartStride + db * 8 + 2 * t4) = make_float2(x, y);
+      }
+      if (!whole && t4 == 0)
+        *reinterpret_cast<float2 *>(part + r * kPaPartStride + 64) = make_float2(m[mt][h], sum);
+    }
+}
+
+// Merges the partials of shares w0 .. w1 of a cut item, all threads of a CTA.
 template <typename OutT>
-WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, const PaWalk &w,
-                            const PaShare &share, int KG, int nr) {
-  const int tid = threadIdx.x;
-  const int row0 = w.q.first + w.rt * kPaRows;
-  const int T = w.units - 1;
-  const bool whole = pa_from(w) == 0 && pa_to(w) == T;
-  const int c0 = pa_owner(w.at, share.total, share.parts);
-  const int c1 = pa_owner(w.at + T - 1, share.total, share.parts);
-  float *mine = whole ? nullptr : pa_part(p, blockIdx.x, c0);
-  for (int i = tid; i < nr * 16; i += kPaWarps * 32) {
-    const int r = i >> 4, d = (i & 15) * 4, w0 = (r >> 4) * KG;
-    float M = -INFINITY, L = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < KG; ++k) M = fmaxf(M, s.wm[w0 + k][r & 15]);
-    for (int k = 0; k < KG; ++k) {
-      const float4 y = *reinterpret_cast<const float4 *>(&s.red[w0 + k][r & 15][d]);
-      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-      L += s.wl[w0 + k][r & 15];
-    }
-    if (whole) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      pa_store4<OutT>(p.o, (int64_t)(row0 + r) * p.o_rs + w.head * 64 + d,
-                      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-    } else {
-      *reinterpret_cast<float4 *>(mine + r * kPaPartStride + d) = x;
-      if (d == 0) *reinterpret_cast<float2 *>(mine + r * kPaPartStride + 64) = make_float2(M, L);
-    }
-  }
-  if (whole) return;
-  pa_sync();
-  if (tid == 0) {
-    __threadfence();
-    s.last = atomicAdd(&p.count[c0], 1) == c1 - c0;
-    if (s.last) __threadfence();
-  }
-  pa_sync();
-  if (!s.last) return;
-  for (int i = tid; i < nr * 16; i += kPaWarps * 32) {
+WATTN_DEVINL void pa_merge(const PagedAttendParams &p, const PaItem &it, int w0, int w1) {
+  for (int i = threadIdx.x; i < it.nr * 16; i += kPaThreads) {
     const int r = i >> 4, d = (i & 15) * 4;
     float M = -INFINITY, L = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, __ldcg(pa_part(p, c, c0) + r * kPaPartStride + 64));
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float *q = pa_part(p, c, c0) + r * kPaPartStride;
+#pragma unroll 8
+    for (int c = w0; c <= w1; ++c)
+      M = fmaxf(M, __ldcg(pa_part(p, c, c == w0) + r * kPaPartStride + 64));
+#pragma unroll 8
+    for (int c = w0; c <= w1; ++c) {
+      const float *q = pa_part(p, c, c == w0) + r * kPaPartStride;
       const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q + 64));
       const float4 y = __ldcg(reinterpret_cast<const float4 *>(q + d));
       const float wt = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
@@ -523,13 +648,46 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, const PaWalk 
       x.z = fmaf(wt, y.z, x.z); x.w = fmaf(wt, y.w, x.w);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    pa_store4<OutT>(p.o, (int64_t)(row0 + r) * p.o_rs + w.head * 64 + d,
+    pa_store4<OutT>(p.o, (int64_t)(it.row0 + r) * p.o_rs + it.head * 64 + d,
                     make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
   }
-  if (tid == 0) p.count[c0] = 0;  // zeroed for the next call
 }
 
-// `map` has boxes of p.box_rows rows (64, 32 or 16: they lie in one page),
+// The items cut by the shares of this CTA's warps, after all of them are done.
+template <typename OutT>
+WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  long long last_at = -1;
+#pragma unroll 1
+  for (int i = 0; i < 2 * kPaWarps; ++i) {
+    const PaItem &it = s.cut[i >> 1][i & 1];
+    if (it.stages == 0 || it.at == last_at) continue;
+    last_at = it.at;
+    const int w0 = pa_owner(it.at, s.total, s.parts);
+    const int w1 = pa_owner(it.at + it.stages - 1, s.total, s.parts);
+    const int c0 = w0 / kPaWarps, c1 = w1 / kPaWarps;
+    if (c0 != c1) {
+      // Release: the barrier orders the CTA's partials before thread 0's
+      // fence, and the fence orders them before the count.
+      if (tid == 0) {
+        __threadfence();
+        s.last = atomicAdd(&p.count[c0], 1) == c1 - c0;
+        if (s.last) {
+          __threadfence();
+          p.count[c0] = 0;  // zeroed for the next call
+        }
+      }
+      __syncthreads();
+      const bool last = s.last;
+      __syncthreads();
+      if (!last) continue;
+    }
+    pa_merge<OutT>(p, it, w0, w1);
+  }
+}
+
+// `map` has boxes of p.box_rows rows (32 or 16: they lie in one page),
 // `map_tail` boxes of 16.
 template <typename T, typename OutT>
 __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
@@ -540,157 +698,37 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   PaSmem &s = *reinterpret_cast<PaSmem *>(
       (reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    for (int st = 0; st < kPaStages; ++st) {
-      mbar_init(&s.kfull[st], 1);
-      mbar_init(&s.vfull[st], 1);
-      mbar_init(&s.empty[st], kPaWarps);
-    }
+  if (lane == 0) {
+    for (int st = 0; st < kPaStages; ++st) mbar_init(&s.full[warp][st], 1);
+    s.cut[warp][0].stages = s.cut[warp][1].stages = 0;
     s.abort = 0;
     fence_barrier_init();
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  PaWalk w;
-  PaShare share;
-  pa_find_share(p, w, share, s.warp_sums, &s.walk);
-  volatile int *abort = &s.abort;
-  uint32_t pos = 0;  // position in the ring
-
-  if (warp == kPaWarps) {
-    // ---- producer. Lane i holds table entry base + i of the request; a
-    // request's heads follow each other, so the entries are mostly there.
-    int have_s = -1, base = 0, entry = 0;
-    for (; pa_more(w); pa_next(p, w)) {
-      const int end = pa_end(p, w.q, w.rt);
-      for (int t = pa_from(w); t < pa_to(w); ++t, ++pos) {
-        const int stage = pos % kPaStages;
-        const bool ok = mbar_wait(&s.empty[stage], ((pos / kPaStages) & 1) ^ 1, abort, p.status,
-                                  (4 << 24) | (3 << 16) | ((pos & 0xff) << 8));
-        if (!__all_sync(0xffffffffu, ok)) return;
-        const int key = t * kPaSub, rows = min(kPaSub, end - key);
-        const bool tail = rows < kPaSub;
-        const int step = tail ? kPaTail : p.box_rows;
-        const int boxes = (rows + step - 1) / step;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&s.kfull[stage], boxes * step * 128);
-          mbar_arrive_expect_tx(&s.vfull[stage], boxes * step * 128);
-        }
-        for (int b = 0; b < boxes; ++b) {
-          const int at = key + b * step;
-          const int pi = at / p.page_rows;
-          if (have_s != w.s || pi < base || pi >= base + 32) {
-            have_s = w.s;
-            base = pi;
-            entry = base + lane < p.max_pages ? p.table[w.s * p.table_stride + base + lane] : 0;
-          }
-          int page = __shfl_sync(0xffffffffu, entry, pi - base);
-          if (page < 0 || page >= p.n_pages) {
-            if (lane == 0) report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
-            page = 0;
-          }
-          if (lane == 0) {
-            const int rk = (((page * p.n_layers + p.layer) * 2) * p.n_heads + w.head) * p.page_rows +
-                           at - pi * p.page_rows;
-            const int rv = rk + p.n_heads * p.page_rows;
-            const CUtensorMap *m = tail ? &map_tail : &map;
-            tma_load_2d(s.k[stage] + b * step * 128, m, &s.kfull[stage], 0, rk);
-            tma_load_2d(s.v[stage] + b * step * 128, m, &s.vfull[stage], 0, rv);
-          }
-        }
-        __syncwarp();
-      }
+  pa_find_shares(p, s);
+  PaLoads ld;
+  ld.w = s.start[warp];
+  ld.issued = ld.announced = 0;
+  ld.have_s = -1;
+  ld.base = ld.entry = 0;
+  ld.more = ld.w.lo < ld.w.hi;
+  if (ld.more) {
+    pa_announce<T>(p, s, ld, warp, lane, true);
+    __syncwarp();
+    for (int st = 0; st < kPaStages; ++st) pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
+    uint32_t pos = 0;
+    for (uint32_t i = 0; i < ld.announced; ++i) {
+      const PaItem it = s.queue[warp][i % kPaQueue];
+      if (it.nr <= 8)
+        pa_item<T, OutT, 1, true>(p, s, ld, map, map_tail, it, pos, warp, lane);
+      else if (it.nr <= 16)
+        pa_item<T, OutT, 1, false>(p, s, ld, map, map_tail, it, pos, warp, lane);
+      else
+        pa_item<T, OutT, 2, false>(p, s, ld, map, map_tail, it, pos, warp, lane);
     }
-    return;
   }
-
-  // ---- compute warps
-  const int g = lane >> 2, t4 = lane & 3;
-  for (; pa_more(w); pa_next(p, w)) {
-    const int from = pa_from(w), to = pa_to(w);
-    if (from >= to) continue;
-    const int nr = min(kPaRows, w.q.n - w.rt * kPaRows);
-    // Warps to a tile of 16 rows: 4 up to 16 rows, 2 up to 32, else one.
-    const int KG = nr <= 16 ? 4 : nr <= 32 ? 2 : 1;
-    const int rg = warp / KG, kg = warp % KG;
-    const int row = w.rt * kPaRows + rg * 16 + g, packed = w.q.first + row;
-    const int here = nr - rg * 16;  // rows of this warp's tile (may be <= 0)
-    const bool few = here <= 8;
-    uint32_t qa[4][4];
-    {
-      const uint32_t *q0 = reinterpret_cast<const uint32_t *>(
-          reinterpret_cast<const T *>(p.q) + (int64_t)packed * p.q_rs + w.head * 64);
-      const uint32_t *q1 = reinterpret_cast<const uint32_t *>(
-          reinterpret_cast<const T *>(p.q) + (int64_t)(packed + 8) * p.q_rs + w.head * 64);
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        qa[ks][0] = g < here ? q0[ks * 8 + t4] : 0u;
-        qa[ks][2] = g < here ? q0[ks * 8 + 4 + t4] : 0u;
-        qa[ks][1] = g + 8 < here ? q1[ks * 8 + t4] : 0u;
-        qa[ks][3] = g + 8 < here ? q1[ks * 8 + 4 + t4] : 0u;
-      }
-    }
-    PaAcc a;
-#pragma unroll
-    for (int db = 0; db < 8; ++db) a.o[db][0] = a.o[db][1] = a.o[db][2] = a.o[db][3] = 0.f;
-    a.m[0] = a.m[1] = -INFINITY;
-    a.l[0] = a.l[1] = 0.f;
-    const int end = pa_end(p, w.q, w.rt);
-    for (int t = from; t < to; ++t, ++pos) {
-      const int stage = pos % kPaStages;
-      const uint32_t ph = (pos / kPaStages) & 1;
-      // (a warp without rows waits too: it may not hand a stage back early)
-      mbar_wait(&s.kfull[stage], ph, abort, p.status, (4 << 24) | (1 << 16) | ((pos & 0xff) << 8));
-      if (here > 0) {
-        const uint32_t kt = smem_u32(s.k[stage]), vt = smem_u32(s.v[stage]);
-        const int off = t * kPaSub - w.q.len, left = end - t * kPaSub;
-        if (KG == 4)
-          pa_sub_tile<T, 1>(p, qa, a, kt, vt, &s.vfull[stage], ph, abort, kg, few, packed, row,
-                            w.q.n, off, left, lane);
-        else if (KG == 2)
-          pa_sub_tile<T, 2>(p, qa, a, kt, vt, &s.vfull[stage], ph, abort, kg, few, packed, row,
-                            w.q.n, off, left, lane);
-        else
-          pa_sub_tile<T, 4>(p, qa, a, kt, vt, &s.vfull[stage], ph, abort, kg, few, packed, row,
-                            w.q.n, off, left, lane);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.empty[stage]);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      a.l[h] += __shfl_xor_sync(0xffffffffu, a.l[h], 1);
-      a.l[h] += __shfl_xor_sync(0xffffffffu, a.l[h], 2);
-    }
-    if (few) {
-#pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        a.o[db][0] += a.o[db][2];
-        a.o[db][1] += a.o[db][3];
-      }
-    }
-    // ---- the KG warps of a tile of 16 rows merge (log-sum-exp)
-    pa_sync();  // the previous item's sums have been read
-    if (t4 == 0) {
-      s.wm[warp][g] = a.m[0];
-      s.wm[warp][g + 8] = a.m[1];
-    }
-    pa_sync();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (g + 8 * h >= here) continue;
-      float M = -INFINITY;
-      for (int k = 0; k < KG; ++k) M = fmaxf(M, s.wm[rg * KG + k][g + 8 * h]);
-      const float wt = a.m[h] == -INFINITY ? 0.f : ex2(a.m[h] - M);
-#pragma unroll
-      for (int db = 0; db < 8; ++db)
-        *reinterpret_cast<float2 *>(&s.red[warp][g + 8 * h][db * 8 + 2 * t4]) =
-            make_float2(a.o[db][2 * h] * wt, a.o[db][2 * h + 1] * wt);
-      if (t4 == 0) s.wl[warp][g + 8 * h] = a.l[h] * wt;
-    }
-    pa_sync();
-    pa_finish<OutT>(p, s, w, share, KG, nr);
-  }
+  pa_finish<OutT>(p, s);
 }
 
 int pa_grid() {
@@ -702,13 +740,13 @@ int pa_grid() {
 }
 
 size_t pa_workspace(int grid) {
-  return kCounterBytes + (size_t)grid * 2 * kPaRows * kPaPartStride * sizeof(float);
+  return kCounterBytes + (size_t)grid * kPaWarps * 2 * kPaRows * kPaPartStride * sizeof(float);
 }
 
 template <typename T, typename OutT>
 int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
   const uint64_t rows = (uint64_t)p.n_pages * p.n_layers * 2 * p.n_heads * p.page_rows;
-  p.box_rows = p.page_rows % 64 == 0 ? 64 : p.page_rows % 32 == 0 ? 32 : 16;
+  p.box_rows = p.page_rows % kPaKeys == 0 ? kPaKeys : kPaTail;
   const uint64_t dims[2] = {64, rows}, strides[1] = {128};
   const uint32_t box[2] = {64, (uint32_t)p.box_rows}, box_tail[2] = {64, kPaTail};
   CUtensorMap map, map_tail;
@@ -863,7 +901,7 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.o_rs = o_row_stride;
   p.max_rows = max_rows;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 2 * kPaSub);
+  p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 2 * kPaKeys);
   p.status = device_status_ptr();
   if (p.status == nullptr) return WATTN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
