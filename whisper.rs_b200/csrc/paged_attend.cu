@@ -13,6 +13,8 @@
 // share of them, in order, wherever that cuts an item's keys. The parts of a
 // cut item are merged by log-sum-exp in the order of the keys, by its CTA or,
 // where it spans several, by the last of them: same inputs, same bits.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "wattn_common.cuh"
@@ -38,7 +40,8 @@ struct PagedAttendParams {
   int max_rows;
   float scale_log2;
   int cap;       // positions that the table can hold
-  int box_rows;  // rows of a TMA box of whole sub-tiles
+  int box_rows;  // rows of a TMA box of whole stages
+  int page_stride, kv_stride;  // head rows from page to page, from K to V
   float *part;   // partials of cut items, two per warp
   int *count;    // finished CTAs of the item that each CTA starts and another ends
   int *status;
@@ -49,12 +52,12 @@ struct PagedAttendParams {
 constexpr int kPaKeys = 32;       // keys of a stage
 constexpr int kPaTail = 16;       // rows of a tail box: the pool's unit of page rows
 constexpr int kPaRows = 32;       // rows of a row tile
-constexpr int kPaStages = 2;      // stages of a warp's ring
+constexpr int kPaStages = 3;      // stages of a warp's ring
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = kPaWarps * 32;
-constexpr int kPaCtasPerSm = 3;
+constexpr int kPaCtasPerSm = 2;
 constexpr int kPaMinUnits = 4;    // units of a share below which fewer warps work
-constexpr int kPaQueue = 4;       // items a warp may have loads for, and one more
+constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaPartStride = 68; // floats per row of a partial: acc[64], m, l
 
 // One request as the kernel sees it, its arrays' values forced into range.
@@ -97,10 +100,31 @@ WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q)
   return u;
 }
 
-// The share that unit u belongs to, of `parts` shares of `total` units:
-// share c is [c * total / parts, (c + 1) * total / parts).
-WATTN_DEVINL int pa_owner(long long u, long long total, int parts) {
-  return (int)(((u + 1) * parts - 1) / total);
+// (a 64-bit division costs hundreds of cycles: the counts mostly fit 32 bits)
+WATTN_DEVINL long long pa_div(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// `total` units in `parts` shares, in order: the first `more` of them have
+// size + 1 units, the others size.
+struct PaShares {
+  long long size;
+  int parts, more;
+};
+WATTN_DEVINL PaShares pa_shares(long long total, int max_parts) {
+  PaShares s;
+  s.parts = (int)max(1ll, min((long long)max_parts, total / kPaMinUnits));
+  s.size = pa_div(total, s.parts);
+  s.more = (int)(total - s.size * s.parts);
+  return s;
+}
+WATTN_DEVINL long long pa_share_begin(const PaShares &s, int c) {
+  return c * s.size + min(c, s.more);
+}
+// The share that unit u belongs to.
+WATTN_DEVINL int pa_owner(const PaShares &s, long long u) {
+  const long long big = s.more * (s.size + 1);
+  return u < big ? (int)pa_div(u, s.size + 1) : s.more + (int)pa_div(u - big, s.size);
 }
 
 // Where a warp's share [lo, hi) begins: in units `at` .. `at` + units of the
@@ -129,8 +153,7 @@ struct PaSmem {
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
   PaStart start[kPaWarps];
   long long warp_sums[kPaWarps];
-  long long total;
-  int parts;
+  PaShares shares;
   int abort, last;
 };
 
@@ -162,16 +185,13 @@ WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
     if (w < warp) before += s.warp_sums[w];
     total += s.warp_sums[w];
   }
-  const int parts = (int)max(1ll, min((long long)gridDim.x * kPaWarps, total / kPaMinUnits));
-  if (tid == 0) {
-    s.total = total;
-    s.parts = parts;
-  }
+  const PaShares shares = pa_shares(total, gridDim.x * kPaWarps);
+  if (tid == 0) s.shares = shares;
 #pragma unroll 1
   for (int k = 0; k < kPaWarps; ++k) {
     const int c = blockIdx.x * kPaWarps + k;
-    const long long lo = c < parts ? c * total / parts : 0;
-    const long long hi = c < parts ? (c + 1) * total / parts : 0;
+    const long long lo = c < shares.parts ? pa_share_begin(shares, c) : 0;
+    const long long hi = c < shares.parts ? pa_share_begin(shares, c + 1) : 0;
     if (lo >= hi) {
       if (tid == 0) s.start[k].lo = s.start[k].hi = 0;
     } else if (before <= lo && lo < before + mine) {
@@ -183,7 +203,7 @@ WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
         w.q = pa_seq(p, w.s, nullptr);
         const long long u = pa_head_units(p, w.q);
         if (lo < w.at + u * p.n_heads) {
-          w.head = (int)((lo - w.at) / u);
+          w.head = (int)pa_div(lo - w.at, u);
           w.at += w.head * u;
           break;
         }
@@ -215,14 +235,12 @@ template <> struct PaType<__nv_bfloat16> {
 template <typename T>
 WATTN_DEVINL void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (__is_same(T, __nv_bfloat16))
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -264,6 +282,16 @@ template <typename T> WATTN_DEVINL uint32_t pa_not_finite(uint32_t w) {
   return __vcmpeq2(w & kInf2, kInf2);
 }
 
+// x, or NaN where a half of w is infinite or NaN.
+template <typename T> WATTN_DEVINL float pa_nil(uint32_t w, float x) {
+  const float2 v = unpack2<T>(w);
+  return fmaf(v.x, 0.f, fmaf(v.y, 0.f, x));
+}
+// The halves of a word holding keys k and k + 1 that lie before `left`.
+WATTN_DEVINL uint32_t pa_keep(int k, int left) {
+  return k + 1 < left ? 0xffffffffu : k < left ? 0xffffu : 0u;
+}
+
 template <typename OutT> WATTN_DEVINL void pa_store2(void *o, int64_t at, float x, float y) {
   if constexpr (sizeof(OutT) == 4)
     *reinterpret_cast<float2 *>(reinterpret_cast<float *>(o) + at) = make_float2(x, y);
@@ -286,10 +314,12 @@ WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, bool starts) {
 // The loads of a warp's share, running ahead of its products.
 struct PaLoads {
   PaStart w;
-  int t, to;             // next stage and end within the current item
+  int t, to, end;        // next stage, the share's last and the positions of the item
+  int page, in_page;     // table index and row of the next box
+  int head_row;          // first row of the head's keys in a page
   uint32_t issued;       // stages issued
   uint32_t announced;    // items announced
-  int have_s, base, entry;  // lane i holds table entry base + i of request have_s
+  int base, entry;       // lane i holds table entry base + i of the request
   bool more;
 };
 
@@ -310,6 +340,7 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
         if (++w.head == p.n_heads) {
           w.head = 0;
           do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
+          ld.base = INT_MIN / 2;  // another request's table
         }
       }
       w.units = pa_units(p, w.q, w.rt);
@@ -319,6 +350,10 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
     ld.to = (int)min((long long)w.units - 1, w.hi - w.at);
     if (ld.t < ld.to) break;
   }
+  ld.end = pa_end(p, w.q, w.rt);
+  ld.page = ld.t * kPaKeys / p.page_rows;
+  ld.in_page = ld.t * kPaKeys - ld.page * p.page_rows;
+  ld.head_row = (p.layer * 2 * p.n_heads + w.head) * p.page_rows;
   const int row = w.rt * kPaRows, row0 = w.q.first + row, nr = min(kPaRows, w.q.n - row);
   if (lane == 0) {
     PaItem &it = s.queue[warp][ld.announced % kPaQueue];
@@ -327,7 +362,7 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
     it.row = row;
     it.n = w.q.n;
     it.len = w.q.len;
-    it.end = pa_end(p, w.q, w.rt);
+    it.end = ld.end;
     it.head = w.head;
     it.from = ld.t;
     it.to = ld.to;
@@ -346,34 +381,32 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
                            const CUtensorMap &map_tail, int warp, int lane) {
   if (!ld.more) return;
   const int slot = ld.issued % kPaStages;
-  const int key = ld.t * kPaKeys;
-  const int rows = min(kPaKeys, pa_end(p, ld.w.q, ld.w.rt) - key);
+  const int rows = min(kPaKeys, ld.end - ld.t * kPaKeys);
   const bool tail = rows < kPaKeys;
   const int step = tail ? kPaTail : p.box_rows;
-  const int boxes = (rows + step - 1) / step;
+  const int boxes = rows > step ? 2 : 1;  // a step is a stage, or half of one
   uint64_t *bar = &s.full[warp][slot];
   if (lane == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);
-#pragma unroll 1
   for (int b = 0; b < boxes; ++b) {
-    const int at = key + b * step;
-    const int pi = at / p.page_rows;
-    if (ld.have_s != ld.w.s || pi < ld.base || pi >= ld.base + 32) {
-      ld.have_s = ld.w.s;
-      ld.base = pi;
-      ld.entry = pi + lane < p.max_pages ? p.table[ld.w.s * p.table_stride + pi + lane] : 0;
+    if (ld.page < ld.base || ld.page >= ld.base + 32) {
+      ld.base = ld.page;
+      ld.entry = ld.base + lane < p.max_pages ? p.table[ld.w.s * p.table_stride + ld.base + lane] : 0;
     }
-    int page = __shfl_sync(0xffffffffu, ld.entry, pi - ld.base);
-    if (page < 0 || page >= p.n_pages) {
-      if (lane == 0) report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
-      page = 0;
-    }
+    int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
     if (lane == 0) {
-      const int rk = ((page * p.n_layers + p.layer) * 2 * p.n_heads + ld.w.head) * p.page_rows + at -
-                     pi * p.page_rows;
-      const int rv = rk + p.n_heads * p.page_rows;
+      if ((unsigned)page >= (unsigned)p.n_pages) {
+        report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
+        page = 0;
+      }
+      const int rk = page * p.page_stride + ld.head_row + ld.in_page;
       const CUtensorMap *m = tail ? &map_tail : &map;
       tma_load_2d(s.k[warp][slot] + b * step * 128, m, bar, 0, rk);
-      tma_load_2d(s.v[warp][slot] + b * step * 128, m, bar, 0, rv);
+      tma_load_2d(s.v[warp][slot] + b * step * 128, m, bar, 0, rk + p.kv_stride);
+    }
+    ld.in_page += step;
+    if (ld.in_page >= p.page_rows) {
+      ld.in_page = 0;
+      ++ld.page;
     }
   }
   ++ld.issued;
@@ -419,20 +452,24 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
     const uint32_t ktile = smem_u32(s.k[warp][slot]), vtile = smem_u32(s.v[warp][slot]);
     float sc[MT][4][4];
 #pragma unroll
-    for (int nb = 0; nb < 4; ++nb) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sc[mt][nb][0] = sc[mt][nb][1] = sc[mt][nb][2] = sc[mt][nb][3] = 0.f;
-      const int key = nb * 8 + (lane & 7);
+      for (int nb = 0; nb < 4; ++nb) sc[mt][nb][0] = sc[mt][nb][1] = sc[mt][nb][2] = sc[mt][nb][3] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        uint32_t r[4];
-        pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r);
+    for (int ks = 0; ks < 2; ++ks) {
+      uint32_t r[4][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          pa_mma<T>(sc[mt][nb], qa[mt][2 * ks], r[0], r[1]);
-          pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + 1], r[2], r[3]);
-        }
+      for (int nb = 0; nb < 4; ++nb) {
+        const int key = nb * 8 + (lane & 7);
+        pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r[nb]);
       }
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int nb = 0; nb < 4; ++nb)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
     }
     const int off = t * kPaKeys - it.len, left = it.end - t * kPaKeys;
     const bool drafts = off + kPaKeys > 0;       // the stage reaches past the cached positions
@@ -481,25 +518,28 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
     // Value rows behind the last position hold anything: zero for the
     // product. A draft's value that is infinite or NaN belongs to the rows
     // that see it and would, as 0 times it, spoil those that do not.
-    uint32_t odd = 0;
+    bool odd = false;
     if (drafts) {
+      float nil = 0.f;  // stays 0 while all is finite
 #pragma unroll
-      for (int sl = 0; sl < 2; ++sl)
+      for (int sl = 0; sl < 2; ++sl) {
+        if (off + 16 * (sl + 1) <= 0 || left <= 16 * sl) continue;
+        const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+        uint32_t vr[4][4];
 #pragma unroll
-        for (int d2 = 0; d2 < 4; ++d2) {
-          const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-          uint32_t vr[4];
-          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+        for (int d2 = 0; d2 < 4; ++d2)
+          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr[d2]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k0 = sl * 16 + (e & 1) * 8 + 2 * t4;
-            odd |= pa_not_finite<T>(vr[e]) &
-                   ((k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u));
-          }
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t keep = pa_keep(sl * 16 + e * 8 + 2 * t4, left);
+#pragma unroll
+          for (int d2 = 0; d2 < 4; ++d2)
+            nil = pa_nil<T>(vr[d2][e] & keep, pa_nil<T>(vr[d2][2 + e] & keep, nil));
         }
-      odd = __any_sync(0xffffffffu, odd != 0);
+      }
+      odd = __any_sync(0xffffffffu, nil != nil);
     }
-    if (__builtin_expect(odd != 0, 0)) {
+    if (__builtin_expect(odd, 0)) {
       constexpr uint32_t one2 = PaType<T>::kOne * 0x10001u, inf2 = PaType<T>::kInf * 0x10001u;
 #pragma unroll
       for (int sl = 0; sl < 2; ++sl) {
@@ -520,8 +560,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int k0 = sl * 16 + (e & 1) * 8 + 2 * t4;
-            vr[e] &= (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
+            vr[e] &= pa_keep(sl * 16 + (e & 1) * 8 + 2 * t4, left);
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half)
@@ -548,6 +587,26 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
     }
 #pragma unroll
     for (int sl = 0; sl < 2; ++sl) {
+      const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+      uint32_t vr[4][4];
+#pragma unroll
+      for (int d2 = 0; d2 < 4; ++d2)
+        pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr[d2]);
+      if (special) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t keep = pa_keep(sl * 16 + e * 8 + 2 * t4, left);
+#pragma unroll
+          for (int d2 = 0; d2 < 4; ++d2) {
+            vr[d2][e] &= keep;
+            vr[d2][2 + e] &= keep;
+            if (odd) {
+              vr[d2][e] &= ~pa_not_finite<T>(vr[d2][e]);
+              vr[d2][2 + e] &= ~pa_not_finite<T>(vr[d2][2 + e]);
+            }
+          }
+        }
+      }
       uint32_t pa[MT][4], pr[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -568,28 +627,16 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
             }
           }
         }
-      const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2) {
-        uint32_t vr[4];
-        pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
-        if (special) {
+      for (int d2 = 0; d2 < 4; ++d2)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k0 = sl * 16 + (e & 1) * 8 + 2 * t4;
-            vr[e] &= (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
-            if (odd) vr[e] &= ~pa_not_finite<T>(vr[e]);
-          }
-        }
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            pa_mma<T>(o[mt][2 * d2 + half], pa[mt], vr[2 * half], vr[2 * half + 1]);
+          for (int mt = 0; mt < MT; ++mt) {
+            pa_mma<T>(o[mt][2 * d2 + half], pa[mt], vr[d2][2 * half], vr[d2][2 * half + 1]);
             if constexpr (!FEW && PaType<T>::kResidual)
-              pa_mma<T>(o[mt][2 * d2 + half], pr[mt], vr[2 * half], vr[2 * half + 1]);
+              pa_mma<T>(o[mt][2 * d2 + half], pr[mt], vr[d2][2 * half], vr[d2][2 * half + 1]);
           }
-      }
     }
     __syncwarp();  // every lane has read the stage
     pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
@@ -664,8 +711,8 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s) {
     const PaItem &it = s.cut[i >> 1][i & 1];
     if (it.stages == 0 || it.at == last_at) continue;
     last_at = it.at;
-    const int w0 = pa_owner(it.at, s.total, s.parts);
-    const int w1 = pa_owner(it.at + it.stages - 1, s.total, s.parts);
+    const int w0 = pa_owner(s.shares, it.at);
+    const int w1 = pa_owner(s.shares, it.at + it.stages - 1);
     const int c0 = w0 / kPaWarps, c1 = w1 / kPaWarps;
     if (c0 != c1) {
       // Release: the barrier orders the CTA's partials before thread 0's
@@ -710,8 +757,8 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   PaLoads ld;
   ld.w = s.start[warp];
   ld.issued = ld.announced = 0;
-  ld.have_s = -1;
-  ld.base = ld.entry = 0;
+  ld.base = INT_MIN / 2;
+  ld.entry = 0;
   ld.more = ld.w.lo < ld.w.hi;
   if (ld.more) {
     pa_announce<T>(p, s, ld, warp, lane, true);
@@ -746,6 +793,8 @@ size_t pa_workspace(int grid) {
 template <typename T, typename OutT>
 int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
   const uint64_t rows = (uint64_t)p.n_pages * p.n_layers * 2 * p.n_heads * p.page_rows;
+  p.kv_stride = p.n_heads * p.page_rows;
+  p.page_stride = p.n_layers * 2 * p.kv_stride;
   p.box_rows = p.page_rows % kPaKeys == 0 ? kPaKeys : kPaTail;
   const uint64_t dims[2] = {64, rows}, strides[1] = {128};
   const uint32_t box[2] = {64, (uint32_t)p.box_rows}, box_tail[2] = {64, kPaTail};
