@@ -42,7 +42,7 @@ struct PagedAttendParams {
   int cap;       // positions that the table can hold
   int box_rows;  // rows of a TMA box of whole stages
   int page_stride, kv_stride;  // head rows from page to page, from K to V
-  float *part;   // partials of cut items, two per warp
+  float *part;   // partials of cut items, two per warp and two per CTA
   int *count;    // finished CTAs of the item that each CTA starts and another ends
   int *status;
 };
@@ -56,7 +56,8 @@ constexpr int kPaStages = 3;      // stages of a warp's ring
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = kPaWarps * 32;
 constexpr int kPaCtasPerSm = 2;
-constexpr int kPaMinUnits = 4;    // units of a share below which fewer warps work
+constexpr int kPaStageUnits = 2, kPaWideUnits = 3, kPaItemUnits = 2;
+constexpr int kPaMinUnits = 8;    // units of a share below which fewer warps work
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaPartStride = 68; // floats per row of a partial: acc[64], m, l
 
@@ -88,13 +89,19 @@ WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
              ? q.end
              : (int)min((int64_t)q.len + min(q.n, kPaRows * (rt + 1)), (int64_t)q.end);
 }
-// Units of one row tile: its stages, and one for what an item costs besides.
-WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return (pa_end(p, q, rt) + kPaKeys - 1) / kPaKeys + 1;
+WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return (pa_end(p, q, rt) + kPaKeys - 1) / kPaKeys;
+}
+// Units that a stage of row tile rt costs: two tiles of 16 rows cost more
+// than one; kPaItemUnits are what an item costs besides its stages.
+WATTN_DEVINL int pa_weight(const PaSeq &q, int rt) {
+  return q.n - rt * kPaRows > 16 ? kPaWideUnits : kPaStageUnits;
+}
+WATTN_DEVINL long long pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return (long long)pa_stages(p, q, rt) * pa_weight(q, rt) + kPaItemUnits;
 }
 // Units of one head of a request.
 WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
-  if (p.row_mask != nullptr) return (long long)q.row_tiles * pa_units(p, q, 0);
   long long u = 0;
   for (int rt = 0; rt < q.row_tiles; ++rt) u += pa_units(p, q, rt);
   return u;
@@ -131,7 +138,7 @@ WATTN_DEVINL int pa_owner(const PaShares &s, long long u) {
 // item (s, head, rt).
 struct PaStart {
   PaSeq q;
-  int s, head, rt, units;
+  int s, head, rt;
   long long at, lo, hi;
 };
 
@@ -141,7 +148,7 @@ struct PaItem {
   int row, n;        // the tile's first row in the request, the request's rows
   int len, end;      // cached positions, positions that some row may see
   int head;
-  int from, to, stages;  // stages of this share, of the item
+  int from, to, stages, weight;  // stages of this share, of the item; units of one
   long long at;      // the item's first unit
 };
 
@@ -151,20 +158,22 @@ struct PaSmem {
   uint64_t full[kPaWarps][kPaStages];
   PaItem queue[kPaWarps][kPaQueue];
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
-  PaStart start[kPaWarps];
-  long long warp_sums[kPaWarps];
+  int run_first[kPaWarps];
+  long long run_at[kPaWarps], warp_sums[kPaWarps];
   PaShares shares;
-  int abort, last;
+  int merge_first[2 * kPaWarps], merge_last[2 * kPaWarps];  // shares to merge, per cut item
+  int abort;
 };
 
-// The warps' shares, found by all threads of the CTA: each adds up the units
-// of a run of requests, the sums are scanned, and the thread whose run holds
-// a share's first unit walks to the item that holds it.
-WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
+// The warps' shares. All threads of the CTA add up the units of a run of
+// requests each; the sums are scanned; then each warp walks, from the first
+// request of the run that holds its share's first unit, to the item there.
+WATTN_DEVINL PaStart pa_find_share(const PagedAttendParams &p, PaSmem &s) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.n_seqs + kPaThreads - 1) / kPaThreads;
   const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
   long long mine = 0;
+#pragma unroll 4
   for (int i = s0; i < s1; ++i) {
     bool bad;
     const PaSeq q = pa_seq(p, i, &bad);
@@ -187,37 +196,39 @@ WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
   }
   const PaShares shares = pa_shares(total, gridDim.x * kPaWarps);
   if (tid == 0) s.shares = shares;
-#pragma unroll 1
+  const int c0 = blockIdx.x * kPaWarps;
+#pragma unroll
   for (int k = 0; k < kPaWarps; ++k) {
-    const int c = blockIdx.x * kPaWarps + k;
-    const long long lo = c < shares.parts ? pa_share_begin(shares, c) : 0;
-    const long long hi = c < shares.parts ? pa_share_begin(shares, c + 1) : 0;
-    if (lo >= hi) {
-      if (tid == 0) s.start[k].lo = s.start[k].hi = 0;
-    } else if (before <= lo && lo < before + mine) {
-      PaStart w;
-      w.lo = lo;
-      w.hi = hi;
-      w.at = before;
-      for (w.s = s0;; ++w.s) {
-        w.q = pa_seq(p, w.s, nullptr);
-        const long long u = pa_head_units(p, w.q);
-        if (lo < w.at + u * p.n_heads) {
-          w.head = (int)pa_div(lo - w.at, u);
-          w.at += w.head * u;
-          break;
-        }
-        w.at += u * p.n_heads;
-      }
-      for (w.rt = 0;; ++w.rt) {
-        w.units = pa_units(p, w.q, w.rt);
-        if (lo < w.at + w.units) break;
-        w.at += w.units;
-      }
-      s.start[k] = w;
+    const long long lo = pa_share_begin(shares, c0 + k);
+    if (c0 + k < shares.parts && before <= lo && lo < before + mine) {
+      s.run_first[k] = s0;
+      s.run_at[k] = before;
     }
   }
   __syncthreads();
+  PaStart w;
+  w.lo = w.hi = 0;
+  const int c = c0 + warp;
+  if (c >= shares.parts || total == 0) return w;
+  w.lo = pa_share_begin(shares, c);
+  w.hi = pa_share_begin(shares, c + 1);
+  w.at = s.run_at[warp];
+  for (w.s = s.run_first[warp];; ++w.s) {
+    w.q = pa_seq(p, w.s, nullptr);
+    const long long u = pa_head_units(p, w.q);
+    if (w.lo < w.at + u * p.n_heads) {
+      w.head = (int)pa_div(w.lo - w.at, u);
+      w.at += w.head * u;
+      break;
+    }
+    w.at += u * p.n_heads;
+  }
+  for (w.rt = 0;; ++w.rt) {
+    const long long u = pa_units(p, w.q, w.rt);
+    if (w.lo < w.at + u) break;
+    w.at += u;
+  }
+  return w;
 }
 
 // ---------------------------------------------------------------- 16-bit pools
@@ -306,7 +317,8 @@ template <typename OutT> WATTN_DEVINL void pa_store4(void *o, int64_t at, float4
         make_uint2(pack2<OutT>(x.x, x.y), pack2<OutT>(x.z, x.w));
 }
 
-// The partial of share c for a cut item that share c0 starts.
+// The partial of share c for a cut item: `starts`, the one that it starts.
+// Behind those of the warps come those of the CTAs.
 WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, bool starts) {
   return p.part + ((int64_t)c * 2 + (starts ? 1 : 0)) * kPaRows * kPaPartStride;
 }
@@ -314,6 +326,7 @@ WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, bool starts) {
 // The loads of a warp's share, running ahead of its products.
 struct PaLoads {
   PaStart w;
+  long long units;       // of the current item
   int t, to, end;        // next stage, the share's last and the positions of the item
   int page, in_page;     // table index and row of the next box
   int head_row;          // first row of the head's keys in a page
@@ -328,9 +341,10 @@ template <typename T>
 WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, int warp, int lane,
                               bool first) {
   PaStart &w = ld.w;
+  int stages, weight;
   for (;;) {
     if (!first) {
-      w.at += w.units;
+      w.at += ld.units;
       if (w.at >= w.hi) {
         ld.more = false;
         return;
@@ -343,11 +357,15 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
           ld.base = INT_MIN / 2;  // another request's table
         }
       }
-      w.units = pa_units(p, w.q, w.rt);
     }
     first = false;
-    ld.t = (int)max(0ll, w.lo - w.at);
-    ld.to = (int)min((long long)w.units - 1, w.hi - w.at);
+    ld.units = pa_units(p, w.q, w.rt);
+    stages = pa_stages(p, w.q, w.rt);
+    weight = pa_weight(w.q, w.rt);
+    // a stage belongs to the share that holds its first unit
+    ld.t = w.lo <= w.at ? 0 : (int)pa_div(w.lo - w.at + weight - 1, weight);
+    ld.to = w.hi - w.at >= (long long)stages * weight ? stages
+                                                      : (int)pa_div(w.hi - w.at + weight - 1, weight);
     if (ld.t < ld.to) break;
   }
   ld.end = pa_end(p, w.q, w.rt);
@@ -366,12 +384,17 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
     it.head = w.head;
     it.from = ld.t;
     it.to = ld.to;
-    it.stages = w.units - 1;
+    it.stages = stages;
+    it.weight = weight;
     it.at = w.at;
   }
-  if (lane < nr)  // the products will want the query rows soon
+  if (lane < nr) {  // the products will want the query rows and masks soon
     asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const T *>(p.q) +
                                                   (int64_t)(row0 + lane) * p.q_rs + w.head * 64));
+    if (p.row_mask != nullptr)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.row_mask +
+                                                    (int64_t)(row0 + lane) * p.mask_words));
+  }
   ++ld.announced;
 }
 
@@ -471,16 +494,20 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           for (int mt = 0; mt < MT; ++mt)
             pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
     }
+    // The slot of the stage before this one is free (3 slots, 2 in flight).
+    pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
     const int off = t * kPaKeys - it.len, left = it.end - t * kPaKeys;
     const bool drafts = off + kPaKeys > 0;       // the stage reaches past the cached positions
     const bool special = drafts || left < kPaKeys;
     if (special) {
+      // lane r finds what row r sees
+      const uint32_t sees =
+          lane < it.nr ? pa_visible(p, it.row0 + lane, it.row + lane, off, left) : 0u;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int h = 0; h < (FEW ? 1 : 2); ++h) {
-          const int r = mt * 16 + h * 8 + g;
-          const uint32_t vis = r < it.nr ? pa_visible(p, it.row0 + r, it.row + r, off, left) : 0u;
+          const uint32_t vis = __shfl_sync(0xffffffffu, sees, mt * 16 + h * 8 + g);
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb)
 #pragma unroll
@@ -639,7 +666,6 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           }
     }
     __syncwarp();  // every lane has read the stage
-    pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
   }
   const bool whole = it.from == 0 && it.to == it.stages;
   const bool starts = it.from == 0;
@@ -674,63 +700,99 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
     }
 }
 
-// Merges the partials of shares w0 .. w1 of a cut item, all threads of a CTA.
+// Merges partials c0 .. c1 (of which c0's is the one that starts the item)
+// of nr rows by log-sum-exp, in order, by all threads of the CTA: into
+// another partial, or as the item's output.
 template <typename OutT>
-WATTN_DEVINL void pa_merge(const PagedAttendParams &p, const PaItem &it, int w0, int w1) {
-  for (int i = threadIdx.x; i < it.nr * 16; i += kPaThreads) {
+WATTN_DEVINL void pa_merge(const PagedAttendParams &p, int c0, int c1, bool starts, int nr, float *part,
+                           int row0, int head) {
+  for (int i = threadIdx.x; i < nr * 16; i += kPaThreads) {
     const int r = i >> 4, d = (i & 15) * 4;
     float M = -INFINITY, L = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int c = w0; c <= w1; ++c)
-      M = fmaxf(M, __ldcg(pa_part(p, c, c == w0) + r * kPaPartStride + 64));
-#pragma unroll 8
-    for (int c = w0; c <= w1; ++c) {
-      const float *q = pa_part(p, c, c == w0) + r * kPaPartStride;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float *q = pa_part(p, c, starts && c == c0) + r * kPaPartStride;
       const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q + 64));
       const float4 y = __ldcg(reinterpret_cast<const float4 *>(q + d));
-      const float wt = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      L = fmaf(wt, ml.y, L);
-      x.x = fmaf(wt, y.x, x.x); x.y = fmaf(wt, y.y, x.y);
-      x.z = fmaf(wt, y.z, x.z); x.w = fmaf(wt, y.w, x.w);
+      const float m = fmaxf(M, ml.x);
+      const float wa = M == -INFINITY ? 0.f : ex2(M - m), wb = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+      M = m;
+      L = fmaf(L, wa, wb * ml.y);
+      x.x = fmaf(x.x, wa, wb * y.x); x.y = fmaf(x.y, wa, wb * y.y);
+      x.z = fmaf(x.z, wa, wb * y.z); x.w = fmaf(x.w, wa, wb * y.w);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    pa_store4<OutT>(p.o, (int64_t)(it.row0 + r) * p.o_rs + it.head * 64 + d,
-                    make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    if (part != nullptr) {
+      *reinterpret_cast<float4 *>(part + r * kPaPartStride + d) = x;
+      if (d == 0) *reinterpret_cast<float2 *>(part + r * kPaPartStride + 64) = make_float2(M, L);
+    } else {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      pa_store4<OutT>(p.o, (int64_t)(row0 + r) * p.o_rs + head * 64 + d,
+                      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    }
   }
 }
 
-// The items cut by the shares of this CTA's warps, after all of them are done.
+// The items cut by the shares of this CTA's warps, after all of them are
+// done: the CTA's parts of an item are merged, and where several CTAs have
+// parts the last of them to arrive merges theirs.
 template <typename OutT>
 WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s) {
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps;
   __syncthreads();
-  long long last_at = -1;
-#pragma unroll 1
-  for (int i = 0; i < 2 * kPaWarps; ++i) {
-    const PaItem &it = s.cut[i >> 1][i & 1];
-    if (it.stages == 0 || it.at == last_at) continue;
-    last_at = it.at;
-    const int w0 = pa_owner(s.shares, it.at);
-    const int w1 = pa_owner(s.shares, it.at + it.stages - 1);
-    const int c0 = w0 / kPaWarps, c1 = w1 / kPaWarps;
-    if (c0 != c1) {
-      // Release: the barrier orders the CTA's partials before thread 0's
-      // fence, and the fence orders them before the count.
-      if (tid == 0) {
-        __threadfence();
-        s.last = atomicAdd(&p.count[c0], 1) == c1 - c0;
-        if (s.last) {
-          __threadfence();
-          p.count[c0] = 0;  // zeroed for the next call
-        }
-      }
-      __syncthreads();
-      const bool last = s.last;
-      __syncthreads();
-      if (!last) continue;
+  if (tid < 2 * kPaWarps) {
+    const PaItem &it = s.cut[tid >> 1][tid & 1];
+    int w0 = 0, w1 = -1;
+    bool fresh = it.stages > 0;  // (the same item may be listed by several warps)
+    for (int i = 0; i < tid; ++i)
+      if (s.cut[i >> 1][i & 1].stages > 0 && s.cut[i >> 1][i & 1].at == it.at) fresh = false;
+    if (fresh) {
+      w0 = pa_owner(s.shares, it.at);
+      w1 = pa_owner(s.shares, it.at + (long long)(it.stages - 1) * it.weight);
     }
-    pa_merge<OutT>(p, it, w0, w1);
+    s.merge_first[tid] = w0;
+    s.merge_last[tid] = w1;
+  }
+  __syncthreads();
+  bool spans = false;
+#pragma unroll 1
+  for (int e = 0; e < 2 * kPaWarps; ++e) {
+    const int w0 = s.merge_first[e], w1 = s.merge_last[e];
+    if (w1 < w0) continue;
+    const PaItem &it = s.cut[e >> 1][e & 1];
+    const int first = max(w0, cta0), last = min(w1, cta0 + kPaWarps - 1);
+    const bool alone = first == w0 && last == w1;
+    spans |= !alone;
+    pa_merge<OutT>(p, first, last, first == w0, it.nr,
+                   alone ? nullptr : pa_part(p, gridDim.x * kPaWarps + blockIdx.x, first == w0), it.row0,
+                   it.head);
+  }
+  if (!spans) return;
+  __syncthreads();
+  if (tid < 2 * kPaWarps) {
+    const int c0 = s.merge_first[tid] / kPaWarps, c1 = s.merge_last[tid] / kPaWarps;
+    bool mine = false;
+    if (s.merge_last[tid] >= s.merge_first[tid] && c0 != c1) {
+      // Release: the barrier orders the CTA's partials before this thread's
+      // fence, and the fence orders them before the count.
+      __threadfence();
+      mine = atomicAdd(&p.count[c0], 1) == c1 - c0;
+      if (mine) {
+        __threadfence();
+        p.count[c0] = 0;  // zeroed for the next call
+      }
+    }
+    s.merge_first[tid] = c0;
+    s.merge_last[tid] = mine ? c1 : -1;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int e = 0; e < 2 * kPaWarps; ++e) {
+    const int c0 = s.merge_first[e], c1 = s.merge_last[e];
+    if (c1 < 0) continue;
+    const PaItem &it = s.cut[e >> 1][e & 1];
+    const int base = gridDim.x * kPaWarps;
+    pa_merge<OutT>(p, base + c0, base + c1, true, it.nr, nullptr, it.row0, it.head);
   }
 }
 
@@ -753,9 +815,8 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  pa_find_shares(p, s);
   PaLoads ld;
-  ld.w = s.start[warp];
+  ld.w = pa_find_share(p, s);
   ld.issued = ld.announced = 0;
   ld.base = INT_MIN / 2;
   ld.entry = 0;
@@ -763,7 +824,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   if (ld.more) {
     pa_announce<T>(p, s, ld, warp, lane, true);
     __syncwarp();
-    for (int st = 0; st < kPaStages; ++st) pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
+    for (int st = 0; st < kPaStages - 1; ++st) pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
     uint32_t pos = 0;
     for (uint32_t i = 0; i < ld.announced; ++i) {
       const PaItem it = s.queue[warp][i % kPaQueue];
@@ -787,7 +848,7 @@ int pa_grid() {
 }
 
 size_t pa_workspace(int grid) {
-  return kCounterBytes + (size_t)grid * kPaWarps * 2 * kPaRows * kPaPartStride * sizeof(float);
+  return kCounterBytes + (size_t)grid * (kPaWarps + 1) * 2 * kPaRows * kPaPartStride * sizeof(float);
 }
 
 template <typename T, typename OutT>
