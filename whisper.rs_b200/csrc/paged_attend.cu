@@ -33,7 +33,7 @@ struct PagedAttendParams {
   const int *seq_lens, *row_start;
   int n_seqs;
   const int *row_mask;
-  int mask_words;
+  int mask_words, mask_bits;
   const void *q;
   void *o;
   int64_t q_rs, o_rs;
@@ -61,33 +61,22 @@ constexpr int kPaMinUnits = 8;    // units of a share below which fewer warps wo
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaPartStride = 68; // floats per row of a partial: acc[64], m, l
 
-// One request as the kernel sees it, its arrays' values forced into range.
+// One request as the kernel sees it. One whose arrays are out of range has
+// no rows here (and is reported).
 struct PaSeq {
   int first, n;   // packed rows
   int len;        // cached positions, all seen
-  int end;        // positions that some row may see (without masks: of the last row tile)
-  int row_tiles;
 };
 
 WATTN_DEVINL PaSeq pa_seq(const PagedAttendParams &p, int s, bool *bad) {
-  PaSeq q;
   const int a = p.row_start[s], b = p.row_start[s + 1], len = p.seq_lens[s];
-  q.first = min(max(a, 0), p.max_rows);
-  q.n = min(max(b, q.first), p.max_rows) - q.first;
-  q.len = min(max(len, 0), p.cap);
-  const int vis = p.row_mask != nullptr ? (int)min((int64_t)q.n, (int64_t)p.mask_words * 32) : q.n;
-  q.end = (int)min((int64_t)q.len + vis, (int64_t)p.cap);
-  q.row_tiles = (q.n + kPaRows - 1) / kPaRows;
-  if (bad != nullptr)
-    *bad = a < 0 || b < a || b > p.max_rows || len < 0 || (int64_t)len + q.n > p.cap;
-  return q;
+  const bool ok = a >= 0 && b >= a && b <= p.max_rows && len >= 0 && len <= p.cap && b - a <= p.cap - len;
+  if (bad != nullptr) *bad = !ok;
+  return {a, ok ? b - a : 0, len};
 }
-
 // Positions that rows of tile rt may see.
 WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return p.row_mask != nullptr
-             ? q.end
-             : (int)min((int64_t)q.len + min(q.n, kPaRows * (rt + 1)), (int64_t)q.end);
+  return q.len + min(q.n, p.row_mask != nullptr ? p.mask_bits : kPaRows * (rt + 1));
 }
 WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
   return (pa_end(p, q, rt) + kPaKeys - 1) / kPaKeys;
@@ -97,19 +86,22 @@ WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
 WATTN_DEVINL int pa_weight(const PaSeq &q, int rt) {
   return q.n - rt * kPaRows > 16 ? kPaWideUnits : kPaStageUnits;
 }
-WATTN_DEVINL long long pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return (long long)pa_stages(p, q, rt) * pa_weight(q, rt) + kPaItemUnits;
+WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return pa_stages(p, q, rt) * pa_weight(q, rt) + kPaItemUnits;
 }
-// Units of one head of a request.
+// Units of one head of a request: its full row tiles, then the last.
 WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
-  long long u = 0;
-  for (int rt = 0; rt < q.row_tiles; ++rt) u += pa_units(p, q, rt);
-  return u;
+  if (q.n <= kPaRows) return q.n > 0 ? pa_units(p, q, 0) : 0;
+  const long long full = (q.n - 1) / kPaRows;
+  long long stages = full * pa_stages(p, q, 0);
+  if (p.row_mask == nullptr) stages += full * (full - 1) / 2;  // one more from tile to tile
+  return stages * kPaWideUnits + full * kPaItemUnits + pa_units(p, q, (int)full);
 }
 
 // (a 64-bit division costs hundreds of cycles: the counts mostly fit 32 bits)
+__device__ __noinline__ long long pa_div64(long long a, long long b) { return a / b; }
 WATTN_DEVINL long long pa_div(long long a, long long b) {
-  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : pa_div64(a, b);
 }
 
 // `total` units in `parts` shares, in order: the first `more` of them have
@@ -145,7 +137,7 @@ struct PaStart {
 // An item of a warp's share, as the loads announce it to the products.
 struct PaItem {
   int row0, nr;      // packed rows of the tile
-  int row, n;        // the tile's first row in the request, the request's rows
+  int row;           // the tile's first row in the request
   int len, end;      // cached positions, positions that some row may see
   int head;
   int from, to, stages, weight;  // stages of this share, of the item; units of one
@@ -224,7 +216,7 @@ WATTN_DEVINL PaStart pa_find_share(const PagedAttendParams &p, PaSmem &s) {
     w.at += u * p.n_heads;
   }
   for (w.rt = 0;; ++w.rt) {
-    const long long u = pa_units(p, w.q, w.rt);
+    const int u = pa_units(p, w.q, w.rt);
     if (w.lo < w.at + u) break;
     w.at += u;
   }
@@ -293,10 +285,13 @@ template <typename T> WATTN_DEVINL uint32_t pa_not_finite(uint32_t w) {
   return __vcmpeq2(w & kInf2, kInf2);
 }
 
-// x, or NaN where a half of w is infinite or NaN.
-template <typename T> WATTN_DEVINL float pa_nil(uint32_t w, float x) {
-  const float2 v = unpack2<T>(w);
-  return fmaf(v.x, 0.f, fmaf(v.y, 0.f, x));
+// x, or NaN in a half where that of w is infinite or NaN (x: two zeros of T).
+template <typename T> WATTN_DEVINL uint32_t pa_nil(uint32_t w, uint32_t x) {
+  if constexpr (__is_same(T, __nv_bfloat16))
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(x) : "r"(w), "r"(0u));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(x) : "r"(w), "r"(0u));
+  return x;
 }
 // The halves of a word holding keys k and k + 1 that lie before `left`.
 WATTN_DEVINL uint32_t pa_keep(int k, int left) {
@@ -326,66 +321,50 @@ WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, bool starts) {
 // The loads of a warp's share, running ahead of its products.
 struct PaLoads {
   PaStart w;
-  long long units;       // of the current item
-  int t, to, end;        // next stage, the share's last and the positions of the item
+  int units, stages, weight;  // of the current item
+  int t, to, end;        // its next stage, the share's last, its positions
   int page, in_page;     // table index and row of the next box
   int head_row;          // first row of the head's keys in a page
   uint32_t issued;       // stages issued
   uint32_t announced;    // items announced
   int base, entry;       // lane i holds table entry base + i of the request
-  bool more;
 };
 
-// Announces the next item of the share that has stages in it.
-template <typename T>
-WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, int warp, int lane,
-                              bool first) {
-  PaStart &w = ld.w;
-  int stages, weight;
-  for (;;) {
-    if (!first) {
-      w.at += ld.units;
-      if (w.at >= w.hi) {
-        ld.more = false;
-        return;
-      }
-      if (++w.rt == w.q.row_tiles) {
-        w.rt = 0;
-        if (++w.head == p.n_heads) {
-          w.head = 0;
-          do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
-          ld.base = INT_MIN / 2;  // another request's table
-        }
-      }
-    }
-    first = false;
-    ld.units = pa_units(p, w.q, w.rt);
-    stages = pa_stages(p, w.q, w.rt);
-    weight = pa_weight(w.q, w.rt);
-    // a stage belongs to the share that holds its first unit
-    ld.t = w.lo <= w.at ? 0 : (int)pa_div(w.lo - w.at + weight - 1, weight);
-    ld.to = w.hi - w.at >= (long long)stages * weight ? stages
-                                                      : (int)pa_div(w.hi - w.at + weight - 1, weight);
-    if (ld.t < ld.to) break;
-  }
+// The current item's stages that this share holds (a stage belongs to the
+// share that holds its first unit), and where their keys are. False if none.
+WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
+  const PaStart &w = ld.w;
+  ld.units = pa_units(p, w.q, w.rt);
+  ld.stages = pa_stages(p, w.q, w.rt);
+  ld.weight = pa_weight(w.q, w.rt);
+  // (both differences are below an item's units where they are divided)
+  const long long d = w.lo - w.at, e = w.hi - w.at;
+  ld.t = d <= 0 ? 0 : ((int)d + ld.weight - 1) / ld.weight;
+  ld.to = e >= ld.units ? ld.stages : min(ld.stages, ((int)e + ld.weight - 1) / ld.weight);
   ld.end = pa_end(p, w.q, w.rt);
   ld.page = ld.t * kPaKeys / p.page_rows;
   ld.in_page = ld.t * kPaKeys - ld.page * p.page_rows;
   ld.head_row = (p.layer * 2 * p.n_heads + w.head) * p.page_rows;
+  return ld.t < ld.to;
+}
+
+// Announces the current item to the products.
+template <typename T>
+WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, int warp, int lane) {
+  const PaStart &w = ld.w;
   const int row = w.rt * kPaRows, row0 = w.q.first + row, nr = min(kPaRows, w.q.n - row);
   if (lane == 0) {
     PaItem &it = s.queue[warp][ld.announced % kPaQueue];
     it.row0 = row0;
     it.nr = nr;
     it.row = row;
-    it.n = w.q.n;
     it.len = w.q.len;
     it.end = ld.end;
     it.head = w.head;
     it.from = ld.t;
     it.to = ld.to;
-    it.stages = stages;
-    it.weight = weight;
+    it.stages = ld.stages;
+    it.weight = ld.weight;
     it.at = w.at;
   }
   if (lane < nr) {  // the products will want the query rows and masks soon
@@ -398,11 +377,25 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
   ++ld.announced;
 }
 
-// Issues the next stage's loads into the ring slot that the products have left.
+// Issues the next stage's loads into the ring slot that the products have
+// left, announcing its item if it is the first of it.
 template <typename T>
 WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
                            const CUtensorMap &map_tail, int warp, int lane) {
-  if (!ld.more) return;
+  PaStart &w = ld.w;
+  while (ld.t >= ld.to) {  // on to the next item of the share
+    w.at += ld.units;
+    if (w.at >= w.hi) return;
+    if (++w.rt * kPaRows >= w.q.n) {
+      w.rt = 0;
+      if (++w.head == p.n_heads) {
+        w.head = 0;
+        do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
+        ld.base = INT_MIN / 2;  // another request's table
+      }
+    }
+    if (pa_enter(p, ld)) pa_announce<T>(p, s, ld, warp, lane);
+  }
   const int slot = ld.issued % kPaStages;
   const int rows = min(kPaKeys, ld.end - ld.t * kPaKeys);
   const bool tail = rows < kPaKeys;
@@ -410,10 +403,11 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
   const int boxes = rows > step ? 2 : 1;  // a step is a stage, or half of one
   uint64_t *bar = &s.full[warp][slot];
   if (lane == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);
+#pragma unroll 1
   for (int b = 0; b < boxes; ++b) {
     if (ld.page < ld.base || ld.page >= ld.base + 32) {
       ld.base = ld.page;
-      ld.entry = ld.base + lane < p.max_pages ? p.table[ld.w.s * p.table_stride + ld.base + lane] : 0;
+      ld.entry = ld.base + lane < p.max_pages ? p.table[w.s * p.table_stride + ld.base + lane] : 0;
     }
     int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
     if (lane == 0) {
@@ -433,21 +427,24 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
     }
   }
   ++ld.issued;
-  if (++ld.t == ld.to) pa_announce<T>(p, s, ld, warp, lane, false);
+  ++ld.t;
   __syncwarp();
 }
 
-// The products of one item's stages: MT tiles of 16 query rows against 32
-// keys a stage. FEW (at most 8 rows): rows 8..15 of the tile carry the
-// weights' rounding residuals and cost no further products.
-template <typename T, typename OutT, int MT, bool FEW>
+// The products of one item's stages: one or (wide) two tiles of 16 query
+// rows against 32 keys a stage. One body serves all: three specialised ones
+// cost more in instruction fetches than they saved. few (at most 8 rows):
+// rows 8..15 of the tile carry the weights' rounding residuals and cost no
+// further products.
+template <typename T, typename OutT>
 WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
                           const CUtensorMap &map_tail, const PaItem &it, uint32_t &pos, int warp,
                           int lane) {
   const int g = lane >> 2, t4 = lane & 3;
-  uint32_t qa[MT][4][4];
+  const bool few = it.nr <= 8, wide = it.nr > 16;
+  uint32_t qa[2][4][4];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = mt * 16 + h * 8 + g;
@@ -455,27 +452,28 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           reinterpret_cast<const T *>(p.q) + (int64_t)(it.row0 + r) * p.q_rs + it.head * 64);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        qa[mt][ks][h] = !(FEW && h) && r < it.nr ? q[ks * 8 + t4] : 0u;
-        qa[mt][ks][2 + h] = !(FEW && h) && r < it.nr ? q[ks * 8 + 4 + t4] : 0u;
+        qa[mt][ks][h] = r < it.nr ? q[ks * 8 + t4] : 0u;
+        qa[mt][ks][2 + h] = r < it.nr ? q[ks * 8 + 4 + t4] : 0u;
       }
     }
-  float o[MT][8][4], m[MT][2], l[MT][2];
+  float o[2][8][4], m[2][2], l[2][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
     for (int db = 0; db < 8; ++db) o[mt][db][0] = o[mt][db][1] = o[mt][db][2] = o[mt][db][3] = 0.f;
     m[mt][0] = m[mt][1] = -INFINITY;
     l[mt][0] = l[mt][1] = 0.f;
   }
 #pragma unroll 1
-  for (int t = it.from; t < it.to; ++t, ++pos) {
+  for (int t = it.from; t < it.to; ++t) {
     const int slot = pos % kPaStages;
     mbar_wait(&s.full[warp][slot], (pos / kPaStages) & 1, &s.abort, p.status,
               (4 << 24) | (1 << 16) | ((pos & 0xff) << 8));
+    ++pos;
     const uint32_t ktile = smem_u32(s.k[warp][slot]), vtile = smem_u32(s.v[warp][slot]);
-    float sc[MT][4][4];
+    float sc[2][4][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int nb = 0; nb < 4; ++nb) sc[mt][nb][0] = sc[mt][nb][1] = sc[mt][nb][2] = sc[mt][nb][3] = 0.f;
 #pragma unroll
@@ -487,12 +485,14 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r[nb]);
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int mt = 0; mt < 2; ++mt) {
+        if (mt == 1 && !wide) break;
 #pragma unroll
-        for (int nb = 0; nb < 4; ++nb)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int nb = 0; nb < 4; ++nb)
             pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
+      }
     }
     // The slot of the stage before this one is free (3 slots, 2 in flight).
     pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
@@ -504,22 +504,26 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
       const uint32_t sees =
           lane < it.nr ? pa_visible(p, it.row0 + lane, it.row + lane, off, left) : 0u;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < 2; ++mt) {
+        if (mt == 1 && !wide) break;
 #pragma unroll
-        for (int h = 0; h < (FEW ? 1 : 2); ++h) {
-          const uint32_t vis = __shfl_sync(0xffffffffu, sees, mt * 16 + h * 8 + g);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t vis = __shfl_sync(0xffffffffu, sees, mt * 16 + h * 8 + g) >> (2 * t4);
 #pragma unroll
           for (int nb = 0; nb < 4; ++nb)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (!(vis >> (nb * 8 + 2 * t4 + e) & 1u)) sc[mt][nb][2 * h + e] = -INFINITY;
+              if (!(vis >> (nb * 8 + e) & 1u)) sc[mt][nb][2 * h + e] = -INFINITY;
         }
+      }
     }
-    float mu[MT][2];
+    float mu[2][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < 2; ++mt) {
+      if (mt == 1 && !wide) break;
 #pragma unroll
-      for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && few) break;
         float mx = -INFINITY;
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) mx = fmax3(mx, sc[mt][nb][2 * h], sc[mt][nb][2 * h + 1]);
@@ -533,52 +537,52 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           for (int db = 0; db < 8; ++db) {
             o[mt][db][2 * h] *= alpha;
             o[mt][db][2 * h + 1] *= alpha;
-            if (FEW) {
-              o[mt][db][2] *= alpha;
-              o[mt][db][3] *= alpha;
+            if (mt == 0 && h == 0 && few) {  // rows 8..15 hold the residuals of rows 0..7
+              o[0][db][2] *= alpha;
+              o[0][db][3] *= alpha;
             }
           }
           m[mt][h] = mc;
         }
         mu[mt][h] = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
       }
+    }
     // Value rows behind the last position hold anything: zero for the
     // product. A draft's value that is infinite or NaN belongs to the rows
     // that see it and would, as 0 times it, spoil those that do not.
     bool odd = false;
     if (drafts) {
-      float nil = 0.f;  // stays 0 while all is finite
+      uint32_t nil = 0;  // stays 0 while all is finite
 #pragma unroll
       for (int sl = 0; sl < 2; ++sl) {
-        if (off + 16 * (sl + 1) <= 0 || left <= 16 * sl) continue;
         const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-        uint32_t vr[4][4];
+        const uint32_t keep0 = pa_keep(sl * 16 + 2 * t4, left), keep1 = pa_keep(sl * 16 + 8 + 2 * t4, left);
 #pragma unroll
-        for (int d2 = 0; d2 < 4; ++d2)
-          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr[d2]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t keep = pa_keep(sl * 16 + e * 8 + 2 * t4, left);
-#pragma unroll
-          for (int d2 = 0; d2 < 4; ++d2)
-            nil = pa_nil<T>(vr[d2][e] & keep, pa_nil<T>(vr[d2][2 + e] & keep, nil));
+        for (int d2 = 0; d2 < 4; ++d2) {
+          uint32_t vr[4];
+          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+          nil = pa_nil<T>(vr[0] & keep0, nil);
+          nil = pa_nil<T>(vr[1] & keep1, nil);
+          nil = pa_nil<T>(vr[2] & keep0, nil);
+          nil = pa_nil<T>(vr[3] & keep1, nil);
         }
       }
-      odd = __any_sync(0xffffffffu, nil != nil);
+      odd = __any_sync(0xffffffffu, pa_not_finite<T>(nil) != 0);
     }
     if (__builtin_expect(odd, 0)) {
       constexpr uint32_t one2 = PaType<T>::kOne * 0x10001u, inf2 = PaType<T>::kInf * 0x10001u;
 #pragma unroll
       for (int sl = 0; sl < 2; ++sl) {
-        uint32_t sees[MT][4];
+        uint32_t sees[2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int nb = sl * 2 + (e >> 1), h = e & 1;
-            sees[mt][e] = FEW && h ? 0u
-                                   : ((sc[mt][nb][2 * h] != -INFINITY ? 0xffffu : 0u) |
-                                      (sc[mt][nb][2 * h + 1] != -INFINITY ? 0xffff0000u : 0u)) & one2;
+            sees[mt][e] = (h && few) || (mt && !wide)
+                              ? 0u
+                              : ((sc[mt][nb][2 * h] != -INFINITY ? 0xffffu : 0u) |
+                                 (sc[mt][nb][2 * h + 1] != -INFINITY ? 0xffff0000u : 0u)) & one2;
           }
 #pragma unroll
         for (int d2 = 0; d2 < 4; ++d2) {
@@ -586,13 +590,11 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           uint32_t vr[4];
           pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            vr[e] &= pa_keep(sl * 16 + (e & 1) * 8 + 2 * t4, left);
-          }
+          for (int e = 0; e < 4; ++e) vr[e] &= pa_keep(sl * 16 + (e & 1) * 8 + 2 * t4, left);
 #pragma unroll
           for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int mt = 0; mt < 2; ++mt) {
               // how many +inf, -inf and NaN values each row sees
               float np[4] = {0, 0, 0, 0}, nm[4] = {0, 0, 0, 0}, nn[4] = {0, 0, 0, 0};
               const uint32_t v0 = vr[2 * half], v1 = vr[2 * half + 1];
@@ -627,43 +629,51 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           for (int d2 = 0; d2 < 4; ++d2) {
             vr[d2][e] &= keep;
             vr[d2][2 + e] &= keep;
-            if (odd) {
-              vr[d2][e] &= ~pa_not_finite<T>(vr[d2][e]);
-              vr[d2][2 + e] &= ~pa_not_finite<T>(vr[d2][2 + e]);
-            }
           }
         }
-      }
-      uint32_t pa[MT][4], pr[MT][4];
+        if (__builtin_expect(odd, 0)) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+          for (int d2 = 0; d2 < 4; ++d2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[d2][e] &= ~pa_not_finite<T>(vr[d2][e]);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        if (mt == 1 && !wide) break;
+        uint32_t pa[4], pr[4];
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2) {
           const float *x = sc[mt][sl * 2 + n2];
-#pragma unroll
-          for (int h = 0; h < (FEW ? 1 : 2); ++h) {
-            const float e0 = ex2(fmaf(x[2 * h], p.scale_log2, -mu[mt][h]));
-            const float e1 = ex2(fmaf(x[2 * h + 1], p.scale_log2, -mu[mt][h]));
-            l[mt][h] += e0 + e1;
-            const uint32_t hi = pack2<T>(e0, e1);
-            pa[mt][2 * n2 + h] = hi;
-            if (FEW || PaType<T>::kResidual) {
-              const float2 r = unpack2<T>(hi);
-              const uint32_t lo = pack2<T>(e0 - r.x, e1 - r.y);
-              if (FEW) pa[mt][2 * n2 + 1] = lo; else pr[mt][2 * n2 + h] = lo;
+          const float e0 = ex2(fmaf(x[0], p.scale_log2, -mu[mt][0]));
+          const float e1 = ex2(fmaf(x[1], p.scale_log2, -mu[mt][0]));
+          l[mt][0] += e0 + e1;
+          pa[2 * n2] = pack2<T>(e0, e1);
+          if (PaType<T>::kResidual || mt == 0) {
+            const float2 r = unpack2<T>(pa[2 * n2]);
+            pr[2 * n2] = pack2<T>(e0 - r.x, e1 - r.y);
+          }
+          if (mt == 0 && few) {
+            pa[2 * n2 + 1] = pr[2 * n2];
+          } else {
+            const float f0 = ex2(fmaf(x[2], p.scale_log2, -mu[mt][1]));
+            const float f1 = ex2(fmaf(x[3], p.scale_log2, -mu[mt][1]));
+            l[mt][1] += f0 + f1;
+            pa[2 * n2 + 1] = pack2<T>(f0, f1);
+            if (PaType<T>::kResidual) {
+              const float2 r = unpack2<T>(pa[2 * n2 + 1]);
+              pr[2 * n2 + 1] = pack2<T>(f0 - r.x, f1 - r.y);
             }
           }
         }
 #pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2)
+        for (int db = 0; db < 8; ++db)
+          pa_mma<T>(o[mt][db], pa, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
+        if (PaType<T>::kResidual && !(mt == 0 && few))
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            pa_mma<T>(o[mt][2 * d2 + half], pa[mt], vr[d2][2 * half], vr[d2][2 * half + 1]);
-            if constexpr (!FEW && PaType<T>::kResidual)
-              pa_mma<T>(o[mt][2 * d2 + half], pr[mt], vr[d2][2 * half], vr[d2][2 * half + 1]);
-          }
+          for (int db = 0; db < 8; ++db)
+            pa_mma<T>(o[mt][db], pr, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
+      }
     }
     __syncwarp();  // every lane has read the stage
   }
@@ -671,33 +681,39 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
   const bool starts = it.from == 0;
   if (!whole && lane == 0) s.cut[warp][starts ? 1 : 0] = it;
   float *part = whole ? nullptr : pa_part(p, blockIdx.x * kPaWarps + warp, starts);
+  if (few) {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+    for (int db = 0; db < 8; ++db) {
+      o[0][db][0] += o[0][db][2];
+      o[0][db][1] += o[0][db][3];
+    }
+  }
 #pragma unroll
-    for (int h = 0; h < (FEW ? 1 : 2); ++h) {
+  for (int mt = 0; mt < 2; ++mt) {
+    if (mt == 1 && !wide) break;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h == 1 && few) break;
       float sum = l[mt][h];
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       const int r = mt * 16 + h * 8 + g;
       if (r >= it.nr) continue;
-      const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      if (whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t at = (int64_t)(it.row0 + r) * p.o_rs + it.head * 64 + 2 * t4;
 #pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        float x = o[mt][db][2 * h], y = o[mt][db][2 * h + 1];
-        if (FEW) {
-          x += o[mt][db][2];
-          y += o[mt][db][3];
-        }
-        x *= inv;
-        y *= inv;
-        if (whole)
-          pa_store2<OutT>(p.o, (int64_t)(it.row0 + r) * p.o_rs + it.head * 64 + db * 8 + 2 * t4, x, y);
-        else
-          *reinterpret_cast<float2 *>(part + r * kPaPartStride + db * 8 + 2 * t4) = make_float2(x, y);
+        for (int db = 0; db < 8; ++db)
+          pa_store2<OutT>(p.o, at + db * 8, o[mt][db][2 * h] * inv, o[mt][db][2 * h + 1] * inv);
+      } else {
+        float *to = part + r * kPaPartStride + 2 * t4;
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+          *reinterpret_cast<float2 *>(to + db * 8) = make_float2(o[mt][db][2 * h], o[mt][db][2 * h + 1]);
+        if (t4 == 0) *reinterpret_cast<float2 *>(to + 64) = make_float2(m[mt][h], sum);
       }
-      if (!whole && t4 == 0)
-        *reinterpret_cast<float2 *>(part + r * kPaPartStride + 64) = make_float2(m[mt][h], sum);
     }
+  }
 }
 
 // Merges partials c0 .. c1 (of which c0's is the one that starts the item)
@@ -820,20 +836,16 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   ld.issued = ld.announced = 0;
   ld.base = INT_MIN / 2;
   ld.entry = 0;
-  ld.more = ld.w.lo < ld.w.hi;
-  if (ld.more) {
-    pa_announce<T>(p, s, ld, warp, lane, true);
-    __syncwarp();
+  if (ld.w.lo < ld.w.hi) {
+    if (pa_enter(p, ld)) pa_announce<T>(p, s, ld, warp, lane);
+#pragma unroll 1
     for (int st = 0; st < kPaStages - 1; ++st) pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
+    __syncwarp();
     uint32_t pos = 0;
+#pragma unroll 1
     for (uint32_t i = 0; i < ld.announced; ++i) {
       const PaItem it = s.queue[warp][i % kPaQueue];
-      if (it.nr <= 8)
-        pa_item<T, OutT, 1, true>(p, s, ld, map, map_tail, it, pos, warp, lane);
-      else if (it.nr <= 16)
-        pa_item<T, OutT, 1, false>(p, s, ld, map, map_tail, it, pos, warp, lane);
-      else
-        pa_item<T, OutT, 2, false>(p, s, ld, map, map_tail, it, pos, warp, lane);
+      pa_item<T, OutT>(p, s, ld, map, map_tail, it, pos, warp, lane);
     }
   }
   pa_finish<OutT>(p, s);
@@ -1005,6 +1017,7 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.n_seqs = n_seqs;
   p.row_mask = row_mask;
   p.mask_words = mask_words;
+  p.mask_bits = (int)std::min((int64_t)mask_words * 32, (int64_t)INT32_MAX);
   p.q = q;
   p.o = o;
   p.q_rs = q_row_stride;
