@@ -59,7 +59,7 @@ constexpr int kPaCtasPerSm = 2;
 constexpr int kPaStageUnits = 2, kPaWideUnits = 3, kPaItemUnits = 2;
 constexpr int kPaMinUnits = 8;    // units of a share below which fewer warps work
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
-constexpr int kPaPartStride = 68; // floats per row of a partial: acc[64], m, l
+constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
 
 // One request as the kernel sees it. One whose arrays are out of range has
 // no rows here (and is reported).
@@ -304,18 +304,63 @@ template <typename OutT> WATTN_DEVINL void pa_store2(void *o, int64_t at, float 
   else
     *reinterpret_cast<uint32_t *>(reinterpret_cast<OutT *>(o) + at) = pack2<OutT>(x, y);
 }
-template <typename OutT> WATTN_DEVINL void pa_store4(void *o, int64_t at, float4 x) {
-  if constexpr (sizeof(OutT) == 4)
-    *reinterpret_cast<float4 *>(reinterpret_cast<float *>(o) + at) = x;
-  else
-    *reinterpret_cast<uint2 *>(reinterpret_cast<OutT *>(o) + at) =
-        make_uint2(pack2<OutT>(x.x, x.y), pack2<OutT>(x.z, x.w));
-}
+// A warp's 16 query rows over some keys: this lane's part of rows g and g + 8.
+struct PaTile {
+  float o[8][4];     // dims 8 db + 2 t4 and + 1 of row g, then of row g + 8
+  float m[2], l[2];  // running max; sum of this lane's weights
+};
 
-// The partial of share c for a cut item: `starts`, the one that it starts.
-// Behind those of the warps come those of the CTAs.
-WATTN_DEVINL float *pa_part(const PagedAttendParams &p, int c, bool starts) {
-  return p.part + ((int64_t)c * 2 + (starts ? 1 : 0)) * kPaRows * kPaPartStride;
+// Partials of cut items, in the lanes' layout: two slots per share (`starts`:
+// the item that the share starts), behind them two per CTA.
+WATTN_DEVINL float4 *pa_part(const PagedAttendParams &p, int slot, bool starts, int mt, int lane) {
+  return reinterpret_cast<float4 *>(
+             p.part + (((int64_t)slot * 2 + (starts ? 1 : 0)) * 2 + mt) * kPaTileFloats) + lane;
+}
+WATTN_DEVINL void pa_put(float4 *part, const PaTile &a) {
+#pragma unroll
+  for (int db = 0; db < 8; ++db) part[db * 32] = make_float4(a.o[db][0], a.o[db][1], a.o[db][2], a.o[db][3]);
+  part[8 * 32] = make_float4(a.m[0], a.m[1], a.l[0], a.l[1]);
+}
+// Adds a partial to `a` (log-sum-exp).
+WATTN_DEVINL void pa_add(PaTile &a, const float4 *part) {
+  float4 x[9];
+#pragma unroll
+  for (int i = 0; i < 9; ++i) x[i] = __ldcg(part + i * 32);
+  float wa[2], wb[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float mb = h ? x[8].y : x[8].x, lb = h ? x[8].w : x[8].z;
+    const float m = fmaxf(a.m[h], mb);
+    wa[h] = a.m[h] == -INFINITY ? 0.f : ex2(a.m[h] - m);
+    wb[h] = mb == -INFINITY ? 0.f : ex2(mb - m);
+    a.m[h] = m;
+    a.l[h] = fmaf(a.l[h], wa[h], wb[h] * lb);
+  }
+#pragma unroll
+  for (int db = 0; db < 8; ++db) {
+    a.o[db][0] = fmaf(a.o[db][0], wa[0], wb[0] * x[db].x);
+    a.o[db][1] = fmaf(a.o[db][1], wa[0], wb[0] * x[db].y);
+    a.o[db][2] = fmaf(a.o[db][2], wa[1], wb[1] * x[db].z);
+    a.o[db][3] = fmaf(a.o[db][3], wa[1], wb[1] * x[db].w);
+  }
+}
+// The outputs of packed rows row0 + g and + 8 (nr rows exist), head h.
+template <typename OutT>
+WATTN_DEVINL void pa_output(const PagedAttendParams &p, const PaTile &a, int row0, int nr, int head,
+                            int lane) {
+  const int g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float sum = a.l[h];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (g + 8 * h >= nr) continue;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at = (int64_t)(row0 + g + 8 * h) * p.o_rs + head * 64 + 2 * t4;
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+      pa_store2<OutT>(p.o, at + db * 8, a.o[db][2 * h] * inv, a.o[db][2 * h + 1] * inv);
+  }
 }
 
 // The loads of a warp's share, running ahead of its products.
@@ -456,13 +501,13 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         qa[mt][ks][2 + h] = r < it.nr ? q[ks * 8 + 4 + t4] : 0u;
       }
     }
-  float o[2][8][4], m[2][2], l[2][2];
+  PaTile a[2];
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-    for (int db = 0; db < 8; ++db) o[mt][db][0] = o[mt][db][1] = o[mt][db][2] = o[mt][db][3] = 0.f;
-    m[mt][0] = m[mt][1] = -INFINITY;
-    l[mt][0] = l[mt][1] = 0.f;
+    for (int db = 0; db < 8; ++db) a[mt].o[db][0] = a[mt].o[db][1] = a[mt].o[db][2] = a[mt].o[db][3] = 0.f;
+    a[mt].m[0] = a[mt].m[1] = -INFINITY;
+    a[mt].l[0] = a[mt].l[1] = 0.f;
   }
 #pragma unroll 1
   for (int t = it.from; t < it.to; ++t) {
@@ -530,21 +575,21 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float mc = mx * p.scale_log2;
-        if (mc > m[mt][h] + 8.0f) {  // rescale only when the running max grows by more than 2^8
-          const float alpha = ex2(m[mt][h] - mc);
-          l[mt][h] *= alpha;
+        if (mc > a[mt].m[h] + 8.0f) {  // rescale only when the running max grows by more than 2^8
+          const float alpha = ex2(a[mt].m[h] - mc);
+          a[mt].l[h] *= alpha;
 #pragma unroll
           for (int db = 0; db < 8; ++db) {
-            o[mt][db][2 * h] *= alpha;
-            o[mt][db][2 * h + 1] *= alpha;
+            a[mt].o[db][2 * h] *= alpha;
+            a[mt].o[db][2 * h + 1] *= alpha;
             if (mt == 0 && h == 0 && few) {  // rows 8..15 hold the residuals of rows 0..7
-              o[0][db][2] *= alpha;
-              o[0][db][3] *= alpha;
+              a[0].o[db][2] *= alpha;
+              a[0].o[db][3] *= alpha;
             }
           }
-          m[mt][h] = mc;
+          a[mt].m[h] = mc;
         }
-        mu[mt][h] = m[mt][h] == -INFINITY ? 0.f : m[mt][h];
+        mu[mt][h] = a[mt].m[h] == -INFINITY ? 0.f : a[mt].m[h];
       }
     }
     // Value rows behind the last position hold anything: zero for the
@@ -605,7 +650,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
                         __vcmpgtu2(v1 & 0x7fff7fffu, inf2) & one2);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                float &x = o[mt][2 * d2 + half][e];
+                float &x = a[mt].o[2 * d2 + half][e];
                 if (np[e] > 0.f) x += INFINITY;
                 if (nm[e] > 0.f) x -= INFINITY;
                 if (nn[e] > 0.f) x = NAN;
@@ -647,7 +692,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           const float *x = sc[mt][sl * 2 + n2];
           const float e0 = ex2(fmaf(x[0], p.scale_log2, -mu[mt][0]));
           const float e1 = ex2(fmaf(x[1], p.scale_log2, -mu[mt][0]));
-          l[mt][0] += e0 + e1;
+          a[mt].l[0] += e0 + e1;
           pa[2 * n2] = pack2<T>(e0, e1);
           if (PaType<T>::kResidual || mt == 0) {
             const float2 r = unpack2<T>(pa[2 * n2]);
@@ -658,7 +703,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           } else {
             const float f0 = ex2(fmaf(x[2], p.scale_log2, -mu[mt][1]));
             const float f1 = ex2(fmaf(x[3], p.scale_log2, -mu[mt][1]));
-            l[mt][1] += f0 + f1;
+            a[mt].l[1] += f0 + f1;
             pa[2 * n2 + 1] = pack2<T>(f0, f1);
             if (PaType<T>::kResidual) {
               const float2 r = unpack2<T>(pa[2 * n2 + 1]);
@@ -668,93 +713,53 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         }
 #pragma unroll
         for (int db = 0; db < 8; ++db)
-          pa_mma<T>(o[mt][db], pa, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
+          pa_mma<T>(a[mt].o[db], pa, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
         if (PaType<T>::kResidual && !(mt == 0 && few))
 #pragma unroll
           for (int db = 0; db < 8; ++db)
-            pa_mma<T>(o[mt][db], pr, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
+            pa_mma<T>(a[mt].o[db], pr, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
       }
     }
     __syncwarp();  // every lane has read the stage
   }
-  const bool whole = it.from == 0 && it.to == it.stages;
-  const bool starts = it.from == 0;
-  if (!whole && lane == 0) s.cut[warp][starts ? 1 : 0] = it;
-  float *part = whole ? nullptr : pa_part(p, blockIdx.x * kPaWarps + warp, starts);
   if (few) {
 #pragma unroll
     for (int db = 0; db < 8; ++db) {
-      o[0][db][0] += o[0][db][2];
-      o[0][db][1] += o[0][db][3];
+      a[0].o[db][0] += a[0].o[db][2];
+      a[0].o[db][1] += a[0].o[db][3];
     }
   }
+  const bool whole = it.from == 0 && it.to == it.stages;
+  const bool starts = it.from == 0;
+  if (!whole && lane == 0) s.cut[warp][starts ? 1 : 0] = it;
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt) {
     if (mt == 1 && !wide) break;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h == 1 && few) break;
-      float sum = l[mt][h];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const int r = mt * 16 + h * 8 + g;
-      if (r >= it.nr) continue;
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int64_t at = (int64_t)(it.row0 + r) * p.o_rs + it.head * 64 + 2 * t4;
-#pragma unroll
-        for (int db = 0; db < 8; ++db)
-          pa_store2<OutT>(p.o, at + db * 8, o[mt][db][2 * h] * inv, o[mt][db][2 * h + 1] * inv);
-      } else {
-        float *to = part + r * kPaPartStride + 2 * t4;
-#pragma unroll
-        for (int db = 0; db < 8; ++db)
-          *reinterpret_cast<float2 *>(to + db * 8) = make_float2(o[mt][db][2 * h], o[mt][db][2 * h + 1]);
-        if (t4 == 0) *reinterpret_cast<float2 *>(to + 64) = make_float2(m[mt][h], sum);
-      }
-    }
+    if (whole)
+      pa_output<OutT>(p, a[mt], it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+    else
+      pa_put(pa_part(p, blockIdx.x * kPaWarps + warp, starts, mt, lane), a[mt]);
   }
 }
 
-// Merges partials c0 .. c1 (of which c0's is the one that starts the item)
-// of nr rows by log-sum-exp, in order, by all threads of the CTA: into
-// another partial, or as the item's output.
-template <typename OutT>
-WATTN_DEVINL void pa_merge(const PagedAttendParams &p, int c0, int c1, bool starts, int nr, float *part,
-                           int row0, int head) {
-  for (int i = threadIdx.x; i < nr * 16; i += kPaThreads) {
-    const int r = i >> 4, d = (i & 15) * 4;
-    float M = -INFINITY, L = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const float *q = pa_part(p, c, starts && c == c0) + r * kPaPartStride;
-      const float2 ml = __ldcg(reinterpret_cast<const float2 *>(q + 64));
-      const float4 y = __ldcg(reinterpret_cast<const float4 *>(q + d));
-      const float m = fmaxf(M, ml.x);
-      const float wa = M == -INFINITY ? 0.f : ex2(M - m), wb = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-      M = m;
-      L = fmaf(L, wa, wb * ml.y);
-      x.x = fmaf(x.x, wa, wb * y.x); x.y = fmaf(x.y, wa, wb * y.y);
-      x.z = fmaf(x.z, wa, wb * y.z); x.w = fmaf(x.w, wa, wb * y.w);
-    }
-    if (part != nullptr) {
-      *reinterpret_cast<float4 *>(part + r * kPaPartStride + d) = x;
-      if (d == 0) *reinterpret_cast<float2 *>(part + r * kPaPartStride + 64) = make_float2(M, L);
-    } else {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      pa_store4<OutT>(p.o, (int64_t)(row0 + r) * p.o_rs + head * 64 + d,
-                      make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-    }
-  }
+// Adds shares c0 .. c1's partials of a cut item, in order (`starts`: c0's is
+// the one that starts it).
+WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c1, bool starts, int mt,
+                            int lane) {
+#pragma unroll
+  for (int db = 0; db < 8; ++db) a.o[db][0] = a.o[db][1] = a.o[db][2] = a.o[db][3] = 0.f;
+  a.m[0] = a.m[1] = -INFINITY;
+  a.l[0] = a.l[1] = 0.f;
+#pragma unroll 2
+  for (int c = c0; c <= c1; ++c) pa_add(a, pa_part(p, c, starts && c == c0, mt, lane));
 }
 
 // The items cut by the shares of this CTA's warps, after all of them are
-// done: the CTA's parts of an item are merged, and where several CTAs have
-// parts the last of them to arrive merges theirs.
+// done, an item per warp: the CTA's parts of an item are merged, and where
+// several CTAs have parts the last of them to arrive merges theirs.
 template <typename OutT>
-WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s) {
-  const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps;
+WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int lane) {
+  const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps, ctas = gridDim.x * kPaWarps;
   __syncthreads();
   if (tid < 2 * kPaWarps) {
     const PaItem &it = s.cut[tid >> 1][tid & 1];
@@ -770,27 +775,29 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s) {
     s.merge_last[tid] = w1;
   }
   __syncthreads();
-  bool spans = false;
+  int turn = 0;
 #pragma unroll 1
   for (int e = 0; e < 2 * kPaWarps; ++e) {
     const int w0 = s.merge_first[e], w1 = s.merge_last[e];
-    if (w1 < w0) continue;
+    if (w1 < w0 || (turn++ & (kPaWarps - 1)) != warp) continue;
     const PaItem &it = s.cut[e >> 1][e & 1];
     const int first = max(w0, cta0), last = min(w1, cta0 + kPaWarps - 1);
     const bool alone = first == w0 && last == w1;
-    spans |= !alone;
-    pa_merge<OutT>(p, first, last, first == w0, it.nr,
-                   alone ? nullptr : pa_part(p, gridDim.x * kPaWarps + blockIdx.x, first == w0), it.row0,
-                   it.head);
-  }
-  if (!spans) return;
-  __syncthreads();
-  if (tid < 2 * kPaWarps) {
-    const int c0 = s.merge_first[tid] / kPaWarps, c1 = s.merge_last[tid] / kPaWarps;
-    bool mine = false;
-    if (s.merge_last[tid] >= s.merge_first[tid] && c0 != c1) {
-      // Release: the barrier orders the CTA's partials before this thread's
-      // fence, and the fence orders them before the count.
+    const int tiles = it.nr > 16 ? 2 : 1;
+#pragma unroll 1
+    for (int mt = 0; mt < tiles; ++mt) {
+      PaTile a;
+      pa_gather(p, a, first, last, first == w0, mt, lane);
+      if (alone) pa_output<OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+      else pa_put(pa_part(p, ctas + blockIdx.x, first == w0, mt, lane), a);
+    }
+    if (alone) continue;
+    // Release: the warp's sync orders its lanes' partials before lane 0's
+    // fence, and the fence orders them before the count.
+    const int c0 = w0 / kPaWarps, c1 = w1 / kPaWarps;
+    int mine = 0;
+    __syncwarp();
+    if (lane == 0) {
       __threadfence();
       mine = atomicAdd(&p.count[c0], 1) == c1 - c0;
       if (mine) {
@@ -798,17 +805,13 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s) {
         p.count[c0] = 0;  // zeroed for the next call
       }
     }
-    s.merge_first[tid] = c0;
-    s.merge_last[tid] = mine ? c1 : -1;
-  }
-  __syncthreads();
+    if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
 #pragma unroll 1
-  for (int e = 0; e < 2 * kPaWarps; ++e) {
-    const int c0 = s.merge_first[e], c1 = s.merge_last[e];
-    if (c1 < 0) continue;
-    const PaItem &it = s.cut[e >> 1][e & 1];
-    const int base = gridDim.x * kPaWarps;
-    pa_merge<OutT>(p, base + c0, base + c1, true, it.nr, nullptr, it.row0, it.head);
+    for (int mt = 0; mt < tiles; ++mt) {
+      PaTile a;
+      pa_gather(p, a, ctas + c0, ctas + c1, true, mt, lane);
+      pa_output<OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+    }
   }
 }
 
@@ -848,7 +851,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
       pa_item<T, OutT>(p, s, ld, map, map_tail, it, pos, warp, lane);
     }
   }
-  pa_finish<OutT>(p, s);
+  pa_finish<OutT>(p, s, warp, lane);
 }
 
 int pa_grid() {
@@ -860,7 +863,7 @@ int pa_grid() {
 }
 
 size_t pa_workspace(int grid) {
-  return kCounterBytes + (size_t)grid * (kPaWarps + 1) * 2 * kPaRows * kPaPartStride * sizeof(float);
+  return kCounterBytes + (size_t)grid * (kPaWarps + 1) * 4 * kPaTileFloats * sizeof(float);
 }
 
 template <typename T, typename OutT>

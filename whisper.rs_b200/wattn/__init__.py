@@ -223,7 +223,17 @@ def capture_cross_attention_heads(q, k, n_tokens, n_audio, n_heads, d_model, sel
            "capture_cross_attention_heads")
 
 
+_DT_OF = {}  # dtype objects already named
+
+
 def _dt_of(a) -> int:
+    dt = _DT_OF.get(a.dtype)
+    if dt is None:
+        dt = _DT_OF[a.dtype] = _dt_named(a)
+    return dt
+
+
+def _dt_named(a) -> int:
     name = str(a.dtype).rsplit(".", 1)[-1]  # "torch.bfloat16" / numpy "float32"
     if name == "float32":
         return F32
@@ -509,53 +519,75 @@ class DeviceKvCache:
 # ---------------------------------------------------------------- device-planned paged cache
 # (include/wattn.h, "Device-planned paged cache": the meaning of every array)
 
-def _ints(t, shape, name, device):
-    """Address of an int32 CUDA tensor whose last dimension is dense; None passes."""
-    if t is None:
-        return None
+# (These run once per layer and step: checks are attribute reads, and what a
+# refusal says is put together only then.)
+
+def _refuse(t, name, expected, device, dense):
+    """Raises what is wrong with tensor ``t``."""
     if not getattr(t, "is_cuda", False):
         raise TypeError(f"{name}: device entry points take CUDA tensors")
-    if str(t.dtype) != "torch.int32":
-        raise TypeError(f"{name} must be int32, not {t.dtype}")
-    if t.dim() != len(shape) or any(w is not None and n != w for n, w in zip(t.shape, shape)):
-        raise WattnError(ERR_INVALID, f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if not t.is_contiguous() and (t.dim() != 2 or name != "block_table" or t.stride(1) != 1):
-        raise WattnError(ERR_INVALID, f"{name} must be contiguous")
-    if t.device != device:
-        raise WattnError(ERR_INVALID, f"{name} is on {t.device}, not on {device}")
+    if t.get_device() != device:
+        raise WattnError(ERR_INVALID, f"{name} is on {t.device}, not on device {device}")
+    raise WattnError(ERR_INVALID, f"{name} is {t.dtype} {tuple(t.shape)} with strides "
+                                  f"{tuple(t.stride())}; expected {expected}, {dense}")
+
+
+def _ints(t, shape, name, device):
+    """Address of a contiguous int32 CUDA tensor of ``shape``; None passes."""
+    if t is None:
+        return None
+    import torch
+    if getattr(t, "dtype", None) is not torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor, not {getattr(t, 'dtype', type(t))}")
+    if t.shape != shape or not t.is_contiguous() or t.get_device() != device or not t.is_cuda:
+        _refuse(t, name, shape, device, "contiguous")
     return t.data_ptr()
+
+
+def _table(t, n_seqs, device):
+    """(address, row stride, columns) of a block table, whose rows may be strided."""
+    import torch
+    if getattr(t, "dtype", None) is not torch.int32:
+        raise TypeError(f"block_table must be an int32 tensor, not {getattr(t, 'dtype', type(t))}")
+    if (t.dim() != 2 or t.shape[0] != n_seqs or t.get_device() != device or not t.is_cuda
+            or t.shape[1] > 1 and t.stride(1) != 1):
+        _refuse(t, "block_table", (n_seqs, "max_pages"), device, "dense rows")
+    n = t.shape[1]
+    return t.data_ptr(), t.stride(0) if n_seqs > 1 else n, n
 
 
 def _rows(t, n_rows, width, name, device):
     """(address, row stride) of a 2-D CUDA tensor of dense rows."""
-    if not getattr(t, "is_cuda", False):
-        raise TypeError(f"{name}: device entry points take CUDA tensors")
-    if t.dim() != 2 or t.shape[0] != n_rows or t.shape[1] != width or t.stride(1) != 1:
-        raise WattnError(ERR_INVALID, f"{name} must be [{n_rows}][{width}] with dense rows, not "
-                                      f"{tuple(t.shape)} with strides {tuple(t.stride())}")
-    if t.device != device:
-        raise WattnError(ERR_INVALID, f"{name} is on {t.device}, not on {device}")
+    if t.shape != (n_rows, width) or t.stride(1) != 1 or t.get_device() != device or not t.is_cuda:
+        _refuse(t, name, (n_rows, width), device, "dense rows")
     return t.data_ptr(), t.stride(0) if n_rows > 1 else width
 
 
 def _pool(pool):
     """(address, dtype, n_pages, n_layers, n_heads, page_rows) of a page pool."""
-    if not getattr(pool, "is_cuda", False):
-        raise TypeError("pool: device entry points take CUDA tensors")
-    if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[5] != 64 or not pool.is_contiguous():
-        raise WattnError(ERR_INVALID, "pool must be contiguous [n_pages][n_layers][2][n_heads]"
-                                      f"[page_rows][64], not {tuple(pool.shape)}")
-    n_pages, n_layers, _, n_heads, page_rows, _ = pool.shape
-    return pool.data_ptr(), _dt_of(pool), n_pages, n_layers, n_heads, page_rows
+    shape = pool.shape
+    if len(shape) != 6 or shape[2] != 2 or shape[5] != 64 or not pool.is_contiguous() or not pool.is_cuda:
+        _refuse(pool, "pool", "[n_pages][n_layers][2][n_heads][page_rows][64]", pool.get_device(),
+                "contiguous")
+    return pool.data_ptr(), _dt_of(pool), shape[0], shape[1], shape[3], shape[4]
+
+
+def _device_of(t, name):
+    """The index of a CUDA tensor's device."""
+    if not getattr(t, "is_cuda", False):
+        raise TypeError(f"{name}: device entry points take CUDA tensors")
+    return t.get_device()
 
 
 def _call_on(device, stream, fn, *args):
-    """fn(*args, stream) with `device` current."""
+    """fn(*args, stream) with `device` current; its current stream if none is given."""
     import torch
-    if device.index == torch.cuda.current_device():
-        return fn(*args, _stream_ptr(stream))
-    with torch.cuda.device(device):
-        return fn(*args, _stream_ptr(stream))
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call_on(device, stream, fn, *args)
+    if stream is None:
+        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    return fn(*args, getattr(stream, "cuda_stream", stream))
 
 
 def paged_plan(seq_lens, n_new, block_table, n_held, free_pages, n_free, row_start, row_pos,
@@ -564,18 +596,17 @@ def paged_plan(seq_lens, n_new, block_table, n_held, free_pages, n_free, row_sta
     ``row_mask`` [max_rows][mask_words]) tree masks from the requests'
     lengths. Updates block_table, n_held, free_pages and n_free in place and
     fills row_start, row_pos, row_slot, row_mask and status; all int32."""
-    dev, n, rows = seq_lens.device, seq_lens.shape[0], row_pos.shape[0]
-    table = _ints(block_table, (n, None), "block_table", dev)
-    words = 0 if row_mask is None else row_mask.shape[-1]
+    dev, n, rows = _device_of(seq_lens, "seq_lens"), seq_lens.shape[0], row_pos.shape[0]
+    table, stride, max_pages = _table(block_table, n, dev)
+    words, n_pages = 0 if row_mask is None else row_mask.shape[-1], free_pages.shape[0]
     _check(_call_on(
         dev, stream, lib.wattn_paged_plan, _ints(seq_lens, (n,), "seq_lens", dev),
-        _ints(n_new, (n,), "n_new", dev), n, page_rows, free_pages.shape[0], table,
-        block_table.stride(0) if n > 1 else block_table.shape[1], block_table.shape[1],
-        _ints(n_held, (n,), "n_held", dev), _ints(free_pages, (None,), "free_pages", dev),
+        _ints(n_new, (n,), "n_new", dev), n, page_rows, n_pages, table, stride, max_pages,
+        _ints(n_held, (n,), "n_held", dev), _ints(free_pages, (n_pages,), "free_pages", dev),
         _ints(n_free, (1,), "n_free", dev), _ints(parents, (rows,), "parents", dev),
         _ints(row_start, (n + 1,), "row_start", dev), _ints(row_pos, (rows,), "row_pos", dev),
         _ints(row_slot, (rows,), "row_slot", dev),
-        _ints(row_mask, (rows, None), "row_mask", dev), words, rows,
+        _ints(row_mask, (rows, words), "row_mask", dev), words, rows,
         _ints(status, (1,), "status", dev)), "paged_plan")
 
 
@@ -583,7 +614,7 @@ def paged_write(pool, layer, row_slot, k_rows, v_rows, *, stream=None) -> None:
     """``wattn_paged_write``: the new rows' K/V ([n_rows][n_heads*64], one row
     stride) into their slots of ``layer``."""
     p = _pool(pool)
-    dev, n = pool.device, row_slot.shape[0]
+    dev, n = pool.get_device(), row_slot.shape[0]
     k, k_rs = _rows(k_rows, n, p[4] * 64, "k_rows", dev)
     v, v_rs = _rows(v_rows, n, p[4] * 64, "v_rows", dev)
     if k_rs != v_rs or k_rows.dtype != v_rows.dtype:
@@ -604,20 +635,19 @@ def paged_attend(pool, layer, block_table, seq_lens, row_start, q, o, *, row_mas
     ``workspace``: a zero-filled CUDA tensor of at least
     paged_attend_workspace_bytes() bytes, or None."""
     p = _pool(pool)
-    dev, n, rows = pool.device, seq_lens.shape[0], q.shape[0]
+    dev, n, rows = pool.get_device(), seq_lens.shape[0], q.shape[0]
     if q.dtype != pool.dtype:
         raise WattnError(ERR_INVALID, f"q is {q.dtype}, the pool {pool.dtype}")
     qp, q_rs = _rows(q, rows, p[4] * 64, "q", dev)
     op, o_rs = _rows(o, rows, p[4] * 64, "o", dev)
-    table = _ints(block_table, (n, None), "block_table", dev)
+    table, stride, max_pages = _table(block_table, n, dev)
+    words = 0 if row_mask is None else row_mask.shape[-1]
     ws_ptr = _dev(workspace) if workspace is not None else None
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
     _check(_call_on(
-        dev, stream, lib.wattn_paged_attend, *p, layer, table,
-        block_table.stride(0) if n > 1 else block_table.shape[1], block_table.shape[1],
+        dev, stream, lib.wattn_paged_attend, *p, layer, table, stride, max_pages,
         _ints(seq_lens, (n,), "seq_lens", dev), _ints(row_start, (n + 1,), "row_start", dev), n,
-        _ints(row_mask, (rows, None), "row_mask", dev),
-        0 if row_mask is None else row_mask.shape[1], qp, q_rs, op, _dt_of(o), o_rs, rows, scale,
+        _ints(row_mask, (rows, words), "row_mask", dev), words, qp, q_rs, op, _dt_of(o), o_rs, rows, scale,
         ws_ptr, ws_bytes), "paged_attend")
 
 
@@ -627,7 +657,7 @@ def paged_accept(pool, row_start, row_slot, tokens, picked, seq_lens, n_accepted
     with: its K/V rows moved together in ``pool``, ``seq_lens`` advanced,
     n_accepted, path and next_token filled; all int32."""
     p = _pool(pool)
-    dev, n, rows = pool.device, seq_lens.shape[0], row_slot.shape[0]
+    dev, n, rows = pool.get_device(), seq_lens.shape[0], row_slot.shape[0]
     _check(_call_on(
         dev, stream, lib.wattn_paged_accept, *p, _ints(row_start, (n + 1,), "row_start", dev), n,
         rows, _ints(parents, (rows,), "parents", dev), _ints(row_slot, (rows,), "row_slot", dev),
