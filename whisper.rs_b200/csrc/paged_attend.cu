@@ -235,15 +235,16 @@ template <> struct PaType<__nv_bfloat16> {
   static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
 };
 
+// (volatile: else the compiler computes the products of a branch not taken)
 template <typename T>
 WATTN_DEVINL void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (__is_same(T, __nv_bfloat16))
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -476,20 +477,20 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
   __syncwarp();
 }
 
-// The products of one item's stages: one or (wide) two tiles of 16 query
-// rows against 32 keys a stage. One body serves all: three specialised ones
-// cost more in instruction fetches than they saved. few (at most 8 rows):
-// rows 8..15 of the tile carry the weights' rounding residuals and cost no
-// further products.
-template <typename T, typename OutT>
+// The products of one item's stages: MT tiles of 16 query rows against 32
+// keys a stage. few (at most 8 rows): rows 8..15 of the tile carry the
+// weights' rounding residuals and cost no further products. (One body for
+// both MT is 14 % slower over single rows, its branches being predicated
+// products; one more for few rows costs more instruction fetches than it saves.)
+template <typename T, typename OutT, int MT>
 WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
                           const CUtensorMap &map_tail, const PaItem &it, uint32_t &pos, int warp,
                           int lane) {
   const int g = lane >> 2, t4 = lane & 3;
-  const bool few = it.nr <= 8, wide = it.nr > 16;
-  uint32_t qa[2][4][4];
+  const bool few = MT == 1 && it.nr <= 8;
+  uint32_t qa[MT][4][4];
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = mt * 16 + h * 8 + g;
@@ -501,9 +502,9 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         qa[mt][ks][2 + h] = r < it.nr ? q[ks * 8 + 4 + t4] : 0u;
       }
     }
-  PaTile a[2];
+  PaTile a[MT];
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
+  for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
     for (int db = 0; db < 8; ++db) a[mt].o[db][0] = a[mt].o[db][1] = a[mt].o[db][2] = a[mt].o[db][3] = 0.f;
     a[mt].m[0] = a[mt].m[1] = -INFINITY;
@@ -516,9 +517,9 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
               (4 << 24) | (1 << 16) | ((pos & 0xff) << 8));
     ++pos;
     const uint32_t ktile = smem_u32(s.k[warp][slot]), vtile = smem_u32(s.v[warp][slot]);
-    float sc[2][4][4];
+    float sc[MT][4][4];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int nb = 0; nb < 4; ++nb) sc[mt][nb][0] = sc[mt][nb][1] = sc[mt][nb][2] = sc[mt][nb][3] = 0.f;
 #pragma unroll
@@ -530,8 +531,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r[nb]);
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        if (mt == 1 && !wide) break;
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -549,8 +549,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
       const uint32_t sees =
           lane < it.nr ? pa_visible(p, it.row0 + lane, it.row + lane, off, left) : 0u;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        if (mt == 1 && !wide) break;
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t vis = __shfl_sync(0xffffffffu, sees, mt * 16 + h * 8 + g) >> (2 * t4);
@@ -562,10 +561,9 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         }
       }
     }
-    float mu[2][2];
+    float mu[MT][2];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-      if (mt == 1 && !wide) break;
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (h == 1 && few) break;
@@ -618,13 +616,13 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
       constexpr uint32_t one2 = PaType<T>::kOne * 0x10001u, inf2 = PaType<T>::kInf * 0x10001u;
 #pragma unroll
       for (int sl = 0; sl < 2; ++sl) {
-        uint32_t sees[2][4];
+        uint32_t sees[MT][4];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int nb = sl * 2 + (e >> 1), h = e & 1;
-            sees[mt][e] = (h && few) || (mt && !wide)
+            sees[mt][e] = h && few
                               ? 0u
                               : ((sc[mt][nb][2 * h] != -INFINITY ? 0xffffu : 0u) |
                                  (sc[mt][nb][2 * h + 1] != -INFINITY ? 0xffff0000u : 0u)) & one2;
@@ -639,7 +637,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
 #pragma unroll
           for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < MT; ++mt) {
               // how many +inf, -inf and NaN values each row sees
               float np[4] = {0, 0, 0, 0}, nm[4] = {0, 0, 0, 0}, nn[4] = {0, 0, 0, 0};
               const uint32_t v0 = vr[2 * half], v1 = vr[2 * half + 1];
@@ -684,8 +682,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
         }
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        if (mt == 1 && !wide) break;
+      for (int mt = 0; mt < MT; ++mt) {
         uint32_t pa[4], pr[4];
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2) {
@@ -733,8 +730,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
   const bool starts = it.from == 0;
   if (!whole && lane == 0) s.cut[warp][starts ? 1 : 0] = it;
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt) {
-    if (mt == 1 && !wide) break;
+  for (int mt = 0; mt < MT; ++mt) {
     if (whole)
       pa_output<OutT>(p, a[mt], it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
     else
@@ -848,7 +844,8 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
 #pragma unroll 1
     for (uint32_t i = 0; i < ld.announced; ++i) {
       const PaItem it = s.queue[warp][i % kPaQueue];
-      pa_item<T, OutT>(p, s, ld, map, map_tail, it, pos, warp, lane);
+      if (it.nr <= 16) pa_item<T, OutT, 1>(p, s, ld, map, map_tail, it, pos, warp, lane);
+      else pa_item<T, OutT, 2>(p, s, ld, map, map_tail, it, pos, warp, lane);
     }
   }
   pa_finish<OutT>(p, s, warp, lane);
