@@ -41,7 +41,6 @@ struct PagedAttendParams {
   float scale_log2;
   int cap;       // positions that the table can hold
   int box_rows;  // rows of a TMA box of whole stages
-  int page_stride, kv_stride;  // head rows from page to page, from K to V
   float *part;   // partials of cut items, two per warp and two per CTA
   int *count;    // finished CTAs of the item that each CTA starts and another ends
   int *status;
@@ -145,8 +144,7 @@ struct PaItem {
 };
 
 struct PaSmem {
-  uint8_t k[kPaWarps][kPaStages][kPaKeys * 128];
-  uint8_t v[kPaWarps][kPaStages][kPaKeys * 128];
+  uint8_t kv[kPaWarps][kPaStages][2][kPaKeys * 128];  // keys, values
   uint64_t full[kPaWarps][kPaStages];
   PaItem queue[kPaWarps][kPaQueue];
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
@@ -249,16 +247,31 @@ WATTN_DEVINL void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-WATTN_DEVINL void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+// The same with D = A B.
+template <typename T>
+WATTN_DEVINL void pa_mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (__is_same(T, __nv_bfloat16))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Four 8x8 matrices at addr + OFF; _t: transposed.
+template <int OFF> WATTN_DEVINL void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4 + %5];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
+               : "r"(addr), "n"(OFF)
                : "memory");
 }
-WATTN_DEVINL void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+template <int OFF> WATTN_DEVINL void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4 + %5];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
+               : "r"(addr), "n"(OFF)
                : "memory");
 }
 
@@ -370,8 +383,8 @@ struct PaLoads {
   int units, stages, weight;  // of the current item
   int t, to, end;        // its next stage, the share's last, its positions
   int page, in_page;     // table index and row of the next box
-  int head_row;          // first row of the head's keys in a page
-  uint32_t issued;       // stages issued
+  int head_row;          // first row of the head in a page's keys (and values)
+  int slot;              // ring slot of the next stage
   uint32_t announced;    // items announced
   int base, entry;       // lane i holds table entry base + i of the request
 };
@@ -390,7 +403,7 @@ WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
   ld.end = pa_end(p, w.q, w.rt);
   ld.page = ld.t * kPaKeys / p.page_rows;
   ld.in_page = ld.t * kPaKeys - ld.page * p.page_rows;
-  ld.head_row = (p.layer * 2 * p.n_heads + w.head) * p.page_rows;
+  ld.head_row = w.head * p.page_rows;
   return ld.t < ld.to;
 }
 
@@ -442,29 +455,32 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
     }
     if (pa_enter(p, ld)) pa_announce<T>(p, s, ld, warp, lane);
   }
-  const int slot = ld.issued % kPaStages;
-  const int rows = min(kPaKeys, ld.end - ld.t * kPaKeys);
+  const int rows = ld.end - ld.t * kPaKeys;
   const bool tail = rows < kPaKeys;
   const int step = tail ? kPaTail : p.box_rows;
-  const int boxes = rows > step ? 2 : 1;  // a step is a stage, or half of one
-  uint64_t *bar = &s.full[warp][slot];
-  if (lane == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);
+  const int boxes = rows > step && step < kPaKeys ? 2 : 1;  // a step is a stage, or half of one
+  uint64_t *bar = &s.full[warp][ld.slot];
 #pragma unroll 1
   for (int b = 0; b < boxes; ++b) {
-    if (ld.page < ld.base || ld.page >= ld.base + 32) {
+    if ((unsigned)(ld.page - ld.base) >= 32u) {
       ld.base = ld.page;
       ld.entry = ld.base + lane < p.max_pages ? p.table[w.s * p.table_stride + ld.base + lane] : 0;
     }
     int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
     if (lane == 0) {
+      if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);
       if ((unsigned)page >= (unsigned)p.n_pages) {
         report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
         page = 0;
       }
-      const int rk = page * p.page_stride + ld.head_row + ld.in_page;
-      const CUtensorMap *m = tail ? &map_tail : &map;
-      tma_load_2d(s.k[warp][slot] + b * step * 128, m, bar, 0, rk);
-      tma_load_2d(s.v[warp][slot] + b * step * 128, m, bar, 0, rk + p.kv_stride);
+      const int c1 = ld.head_row + ld.in_page, c3 = page * p.n_layers + p.layer;
+      uint8_t *dst = &s.kv[warp][ld.slot][0][0] + b * kPaTail * 128;
+      if (step == kPaKeys) {
+        tma_load_4d(dst, &map, bar, 0, c1, 0, c3);  // the keys, and behind them the values
+      } else {  // 16 rows of each
+        tma_load_4d(dst, &map_tail, bar, 0, c1, 0, c3);
+        tma_load_4d(dst + kPaKeys * 128, &map_tail, bar, 0, c1, 1, c3);
+      }
     }
     ld.in_page += step;
     if (ld.in_page >= p.page_rows) {
@@ -472,7 +488,7 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
       ++ld.page;
     }
   }
-  ++ld.issued;
+  ld.slot = ld.slot == kPaStages - 1 ? 0 : ld.slot + 1;
   ++ld.t;
   __syncwarp();
 }
@@ -510,34 +526,36 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
     a[mt].m[0] = a[mt].m[1] = -INFINITY;
     a[mt].l[0] = a[mt].l[1] = 0.f;
   }
+  // Lane offsets: keys in rows of 128 swizzled bytes, values transposed.
+  const uint32_t koff = (lane & 7) * 128 + (((lane >> 3) ^ (lane & 7)) << 4);
+  const uint32_t voff = ((lane >> 3) & 1) * 1024 + (lane & 7) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll 1
   for (int t = it.from; t < it.to; ++t) {
-    const int slot = pos % kPaStages;
-    mbar_wait(&s.full[warp][slot], (pos / kPaStages) & 1, &s.abort, p.status,
-              (4 << 24) | (1 << 16) | ((pos & 0xff) << 8));
-    ++pos;
-    const uint32_t ktile = smem_u32(s.k[warp][slot]), vtile = smem_u32(s.v[warp][slot]);
+    const int slot = pos & 3;
+    mbar_wait(&s.full[warp][slot], pos >> 31, &s.abort, p.status,
+              (4 << 24) | (1 << 16) | ((t & 0xff) << 8));
+    pos = slot == kPaStages - 1 ? (pos & 0x80000000u) ^ 0x80000000u : pos + 1;
+    const uint32_t ktile = smem_u32(&s.kv[warp][slot][0][0]), vtile = ktile + kPaKeys * 128;
     float sc[MT][4][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nb = 0; nb < 4; ++nb) sc[mt][nb][0] = sc[mt][nb][1] = sc[mt][nb][2] = sc[mt][nb][3] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       uint32_t r[4][4];
+      const uint32_t at = ktile + (koff ^ (ks * 64));
+      pa_ldsm<0>(at, r[0]);
+      pa_ldsm<1024>(at, r[1]);
+      pa_ldsm<2048>(at, r[2]);
+      pa_ldsm<3072>(at, r[3]);
 #pragma unroll
-      for (int nb = 0; nb < 4; ++nb) {
-        const int key = nb * 8 + (lane & 7);
-        pa_ldsm(ktile + key * 128 + (((4 * ks + (lane >> 3)) ^ (key & 7)) << 4), r[nb]);
-      }
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int nb = 0; nb < 4; ++nb)
-            pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
-      }
+          for (int nb = 0; nb < 4; ++nb) {
+            if (ks == 0 && half == 0)
+              pa_mma0<T>(sc[mt][nb], qa[mt][0], r[nb][0], r[nb][1]);
+            else
+              pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
+          }
     }
     // The slot of the stage before this one is free (3 slots, 2 in flight).
     pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
@@ -598,12 +616,11 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
       uint32_t nil = 0;  // stays 0 while all is finite
 #pragma unroll
       for (int sl = 0; sl < 2; ++sl) {
-        const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
         const uint32_t keep0 = pa_keep(sl * 16 + 2 * t4, left), keep1 = pa_keep(sl * 16 + 8 + 2 * t4, left);
 #pragma unroll
         for (int d2 = 0; d2 < 4; ++d2) {
           uint32_t vr[4];
-          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+          pa_ldsm_t<0>(vtile + sl * 2048 + (voff ^ (d2 * 32)), vr);
           nil = pa_nil<T>(vr[0] & keep0, nil);
           nil = pa_nil<T>(vr[1] & keep1, nil);
           nil = pa_nil<T>(vr[2] & keep0, nil);
@@ -629,9 +646,8 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           }
 #pragma unroll
         for (int d2 = 0; d2 < 4; ++d2) {
-          const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
           uint32_t vr[4];
-          pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr);
+          pa_ldsm_t<0>(vtile + sl * 2048 + (voff ^ (d2 * 32)), vr);
 #pragma unroll
           for (int e = 0; e < 4; ++e) vr[e] &= pa_keep(sl * 16 + (e & 1) * 8 + 2 * t4, left);
 #pragma unroll
@@ -659,11 +675,13 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
     }
 #pragma unroll
     for (int sl = 0; sl < 2; ++sl) {
-      const int key = sl * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
       uint32_t vr[4][4];
 #pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2)
-        pa_ldsm_t(vtile + key * 128 + (((d2 * 2 + (lane >> 4)) ^ (key & 7)) << 4), vr[d2]);
+      for (int d2 = 0; d2 < 4; ++d2) {
+        const uint32_t at = vtile + (voff ^ (d2 * 32));
+        if (sl == 0) pa_ldsm_t<0>(at, vr[d2]);
+        else pa_ldsm_t<2048>(at, vr[d2]);
+      }
       if (special) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -683,6 +701,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        // (of a tile of few rows the residuals are rows 8..15, where T needs them)
         uint32_t pa[4], pr[4];
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2) {
@@ -691,12 +710,12 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
           const float e1 = ex2(fmaf(x[1], p.scale_log2, -mu[mt][0]));
           a[mt].l[0] += e0 + e1;
           pa[2 * n2] = pack2<T>(e0, e1);
-          if (PaType<T>::kResidual || mt == 0) {
+          if (PaType<T>::kResidual) {
             const float2 r = unpack2<T>(pa[2 * n2]);
             pr[2 * n2] = pack2<T>(e0 - r.x, e1 - r.y);
           }
-          if (mt == 0 && few) {
-            pa[2 * n2 + 1] = pr[2 * n2];
+          if (few) {
+            pa[2 * n2 + 1] = PaType<T>::kResidual ? pr[2 * n2] : 0u;
           } else {
             const float f0 = ex2(fmaf(x[2], p.scale_log2, -mu[mt][1]));
             const float f1 = ex2(fmaf(x[3], p.scale_log2, -mu[mt][1]));
@@ -708,13 +727,22 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
             }
           }
         }
+        // (a loop: as a condition it becomes products that are predicated off)
+#pragma unroll 1
+        for (int rep = 0; rep < (PaType<T>::kResidual && !few && MT == 1 ? 2 : 1); ++rep) {
 #pragma unroll
-        for (int db = 0; db < 8; ++db)
-          pa_mma<T>(a[mt].o[db], pa, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
-        if (PaType<T>::kResidual && !(mt == 0 && few))
+          for (int db = 0; db < 8; ++db)
+            pa_mma<T>(a[mt].o[db], pa, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
+          if (PaType<T>::kResidual) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pa[e] = pr[e];
+          }
+        }
+        if (PaType<T>::kResidual && MT == 2) {
 #pragma unroll
           for (int db = 0; db < 8; ++db)
             pa_mma<T>(a[mt].o[db], pr, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
+        }
       }
     }
     __syncwarp();  // every lane has read the stage
@@ -811,8 +839,8 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int
   }
 }
 
-// `map` has boxes of p.box_rows rows (32 or 16: they lie in one page),
-// `map_tail` boxes of 16.
+// `map` has boxes of a stage's keys and values (used where pages hold whole
+// stages), `map_tail` boxes of 16 rows of either.
 template <typename T, typename OutT>
 __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
     paged_attend_stream_kernel(const __grid_constant__ CUtensorMap map,
@@ -832,7 +860,8 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   grid_dep_launch();
   PaLoads ld;
   ld.w = pa_find_share(p, s);
-  ld.issued = ld.announced = 0;
+  ld.slot = 0;
+  ld.announced = 0;
   ld.base = INT_MIN / 2;
   ld.entry = 0;
   if (ld.w.lo < ld.w.hi) {
@@ -840,7 +869,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
 #pragma unroll 1
     for (int st = 0; st < kPaStages - 1; ++st) pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
     __syncwarp();
-    uint32_t pos = 0;
+    uint32_t pos = 0;  // ring slot of the next stage, and in bit 31 its barrier's phase
 #pragma unroll 1
     for (uint32_t i = 0; i < ld.announced; ++i) {
       const PaItem it = s.queue[warp][i % kPaQueue];
@@ -865,18 +894,21 @@ size_t pa_workspace(int grid) {
 
 template <typename T, typename OutT>
 int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
-  const uint64_t rows = (uint64_t)p.n_pages * p.n_layers * 2 * p.n_heads * p.page_rows;
-  p.kv_stride = p.n_heads * p.page_rows;
-  p.page_stride = p.n_layers * 2 * p.kv_stride;
+  // The pool as [page, layer][K|V][head, row][64]: one box holds a stage's
+  // keys and its values; the tail map's boxes hold 16 rows of either.
+  const uint64_t kv_rows = (uint64_t)p.n_heads * p.page_rows;
   p.box_rows = p.page_rows % kPaKeys == 0 ? kPaKeys : kPaTail;
-  const uint64_t dims[2] = {64, rows}, strides[1] = {128};
-  const uint32_t box[2] = {64, (uint32_t)p.box_rows}, box_tail[2] = {64, kPaTail};
+  const uint64_t dims[4] = {64, kv_rows, 2, (uint64_t)p.n_pages * p.n_layers};
+  const uint64_t strides[3] = {128, kv_rows * 128, kv_rows * 256};
+  const uint32_t box[4] = {64, kPaKeys, 2, 1}, box_tail[4] = {64, kPaTail, 1, 1};
   CUtensorMap map, map_tail;
-  int rc = encode_tmap(&map, tmap_dtype(dtype), 2, p.pool, dims, strides, box,
+  int rc = encode_tmap(&map_tail, tmap_dtype(dtype), 4, p.pool, dims, strides, box_tail,
                        CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == WATTN_OK)
-    rc = encode_tmap(&map_tail, tmap_dtype(dtype), 2, p.pool, dims, strides, box_tail,
+  if (rc == WATTN_OK && p.box_rows == kPaKeys)
+    rc = encode_tmap(&map, tmap_dtype(dtype), 4, p.pool, dims, strides, box,
                      CU_TENSOR_MAP_SWIZZLE_128B);
+  else
+    map = map_tail;  // not used
   if (rc != WATTN_OK) return rc;
   constexpr int smem = (int)sizeof(PaSmem) + 1024;
   auto kern = paged_attend_stream_kernel<T, OutT>;
