@@ -5,14 +5,16 @@
 //
 // 16-bit pools. Bound: HBM (each key's K and V, 256 bytes, meet up to 32
 // query rows: 4 * 64 * 32 products on the tensor cores for 256 bytes). Every
-// warp streams for itself: it has its own ring of two 32-key stages, loads
-// them by TMA through the block table and multiplies with mma.sync; warps
-// meet only when they are done. The unit of work is one stage of one item
-// (request, head, tile of up to 32 rows). The lengths are on the device, so
-// each CTA adds up the requests' units itself and each warp takes an equal
-// share of them, in order, wherever that cuts an item's keys. The parts of a
-// cut item are merged by log-sum-exp in the order of the keys, by its CTA or,
-// where it spans several, by the last of them: same inputs, same bits.
+// compute warp streams for itself: it has its own ring of three 32-key
+// stages, which a load warp of its own fills by TMA through the block table,
+// and multiplies with mma.sync; compute warps meet only when they are done.
+// (A compute warp that issues its own loads spends 660 of 2400 cycles a stage
+// on that.) An item is one (request, head, tile of up to 32 rows). The lengths
+// are on the device, so each CTA adds up the requests' work itself and each
+// compute warp takes an equal share of it, in order, wherever that cuts an
+// item's keys. The parts of a cut item are merged by log-sum-exp in the order
+// of the keys, by its CTA or, where it spans several, by the last of them:
+// same inputs, same bits.
 #include <limits.h>
 
 #include <algorithm>
@@ -52,9 +54,13 @@ constexpr int kPaKeys = 32;       // keys of a stage
 constexpr int kPaTail = 16;       // rows of a tail box: the pool's unit of page rows
 constexpr int kPaRows = 32;       // rows of a row tile
 constexpr int kPaStages = 3;      // stages of a warp's ring
-constexpr int kPaWarps = 4;
-constexpr int kPaThreads = kPaWarps * 32;
+constexpr int kPaWarps = 4;       // compute warps (one warpgroup), and as many load warps
+constexpr int kPaThreads = 2 * kPaWarps * 32;
 constexpr int kPaCtasPerSm = 2;
+// Registers per thread: what the block is launched with, then after the
+// warpgroups' split (whose sum may not exceed twice the launch's).
+constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
+static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
 constexpr int kPaStageUnits = 2, kPaWideUnits = 3, kPaItemUnits = 2;
 constexpr int kPaMinUnits = 8;    // units of a share below which fewer warps work
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
@@ -97,40 +103,31 @@ WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q)
   return stages * kPaWideUnits + full * kPaItemUnits + pa_units(p, q, (int)full);
 }
 
-// (a 64-bit division costs hundreds of cycles: the counts mostly fit 32 bits)
-__device__ __noinline__ long long pa_div64(long long a, long long b) { return a / b; }
-WATTN_DEVINL long long pa_div(long long a, long long b) {
-  return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : pa_div64(a, b);
-}
-
-// `total` units in `parts` shares, in order: the first `more` of them have
-// size + 1 units, the others size.
+// `total` units (below 2^31) in `parts` shares, in order: the first `more` of
+// them have size + 1 units, the others size.
 struct PaShares {
-  long long size;
-  int parts, more;
+  int size, parts, more;
 };
-WATTN_DEVINL PaShares pa_shares(long long total, int max_parts) {
+WATTN_DEVINL PaShares pa_shares(int total, int max_parts) {
   PaShares s;
-  s.parts = (int)max(1ll, min((long long)max_parts, total / kPaMinUnits));
-  s.size = pa_div(total, s.parts);
-  s.more = (int)(total - s.size * s.parts);
+  s.parts = max(1, min(max_parts, total / kPaMinUnits));
+  s.size = total / s.parts;
+  s.more = total - s.size * s.parts;
   return s;
 }
-WATTN_DEVINL long long pa_share_begin(const PaShares &s, int c) {
-  return c * s.size + min(c, s.more);
-}
+WATTN_DEVINL int pa_share_begin(const PaShares &s, int c) { return c * s.size + min(c, s.more); }
 // The share that unit u belongs to.
-WATTN_DEVINL int pa_owner(const PaShares &s, long long u) {
-  const long long big = s.more * (s.size + 1);
-  return u < big ? (int)pa_div(u, s.size + 1) : s.more + (int)pa_div(u - big, s.size);
+WATTN_DEVINL int pa_owner(const PaShares &s, int u) {
+  const int big = s.more * (s.size + 1);
+  return u < big ? u / (s.size + 1) : s.more + (u - big) / s.size;
 }
 
-// Where a warp's share [lo, hi) begins: in units `at` .. `at` + units of the
-// item (s, head, rt).
+// Where a share [lo, hi) begins: its first item (s, head, rt) starts at unit
+// `at` <= lo.
 struct PaStart {
   PaSeq q;
   int s, head, rt;
-  long long at, lo, hi;
+  int at, lo, hi;
 };
 
 // An item of a warp's share, as the loads announce it to the products.
@@ -140,25 +137,26 @@ struct PaItem {
   int len, end;      // cached positions, positions that some row may see
   int head;
   int from, to, stages, weight;  // stages of this share, of the item; units of one
-  long long at;      // the item's first unit
+  int at;            // the item's first unit
 };
 
 struct PaSmem {
   uint8_t kv[kPaWarps][kPaStages][2][kPaKeys * 128];  // keys, values
-  uint64_t full[kPaWarps][kPaStages];
+  uint64_t full[kPaWarps][kPaStages], empty[kPaWarps][kPaStages];
   PaItem queue[kPaWarps][kPaQueue];
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
-  int run_first[kPaWarps];
-  long long run_at[kPaWarps], warp_sums[kPaWarps];
+  int run_first[kPaWarps], run_at[kPaWarps];
+  long long warp_sums[2 * kPaWarps];
   PaShares shares;
+  int total;
   int merge_first[2 * kPaWarps], merge_last[2 * kPaWarps];  // shares to merge, per cut item
   int abort;
 };
 
-// The warps' shares. All threads of the CTA add up the units of a run of
-// requests each; the sums are scanned; then each warp walks, from the first
-// request of the run that holds its share's first unit, to the item there.
-WATTN_DEVINL PaStart pa_find_share(const PagedAttendParams &p, PaSmem &s) {
+// The shares. All threads of the CTA add up the units of a run of requests
+// each; the sums are scanned, and for each share of the CTA the run that
+// holds its first unit is noted.
+WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.n_seqs + kPaThreads - 1) / kPaThreads;
   const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
@@ -180,34 +178,45 @@ WATTN_DEVINL PaStart pa_find_share(const PagedAttendParams &p, PaSmem &s) {
   __syncthreads();
   long long before = inc - mine, total = 0;
 #pragma unroll
-  for (int w = 0; w < kPaWarps; ++w) {
+  for (int w = 0; w < 2 * kPaWarps; ++w) {
     if (w < warp) before += s.warp_sums[w];
     total += s.warp_sums[w];
   }
-  const PaShares shares = pa_shares(total, gridDim.x * kPaWarps);
-  if (tid == 0) s.shares = shares;
+  if (total > INT_MAX) {  // more than a call may ask for
+    if (tid == 0) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
+    total = 0;
+  }
+  const PaShares shares = pa_shares((int)total, gridDim.x * kPaWarps);
+  if (tid == 0) {
+    s.shares = shares;
+    s.total = (int)total;
+  }
   const int c0 = blockIdx.x * kPaWarps;
 #pragma unroll
   for (int k = 0; k < kPaWarps; ++k) {
-    const long long lo = pa_share_begin(shares, c0 + k);
+    const int lo = pa_share_begin(shares, c0 + k);
     if (c0 + k < shares.parts && before <= lo && lo < before + mine) {
       s.run_first[k] = s0;
-      s.run_at[k] = before;
+      s.run_at[k] = (int)before;
     }
   }
   __syncthreads();
+}
+
+// Share blockIdx.x * kPaWarps + k: walks to its first item.
+WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k) {
   PaStart w;
   w.lo = w.hi = 0;
-  const int c = c0 + warp;
-  if (c >= shares.parts || total == 0) return w;
-  w.lo = pa_share_begin(shares, c);
-  w.hi = pa_share_begin(shares, c + 1);
-  w.at = s.run_at[warp];
-  for (w.s = s.run_first[warp];; ++w.s) {
+  const int c = blockIdx.x * kPaWarps + k;
+  if (c >= s.shares.parts || s.total == 0) return w;
+  w.lo = pa_share_begin(s.shares, c);
+  w.hi = pa_share_begin(s.shares, c + 1);
+  w.at = s.run_at[k];
+  for (w.s = s.run_first[k];; ++w.s) {
     w.q = pa_seq(p, w.s, nullptr);
-    const long long u = pa_head_units(p, w.q);
-    if (w.lo < w.at + u * p.n_heads) {
-      w.head = (int)pa_div(w.lo - w.at, u);
+    const int u = (int)pa_head_units(p, w.q);
+    if (w.lo - w.at < (long long)u * p.n_heads) {
+      w.head = (w.lo - w.at) / u;
       w.at += w.head * u;
       break;
     }
@@ -215,7 +224,7 @@ WATTN_DEVINL PaStart pa_find_share(const PagedAttendParams &p, PaSmem &s) {
   }
   for (w.rt = 0;; ++w.rt) {
     const int u = pa_units(p, w.q, w.rt);
-    if (w.lo < w.at + u) break;
+    if (w.lo - w.at < u) break;
     w.at += u;
   }
   return w;
@@ -369,7 +378,7 @@ WATTN_DEVINL void pa_output(const PagedAttendParams &p, const PaTile &a, int row
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if (g + 8 * h >= nr) continue;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
     const int64_t at = (int64_t)(row0 + g + 8 * h) * p.o_rs + head * 64 + 2 * t4;
 #pragma unroll
     for (int db = 0; db < 8; ++db)
@@ -377,15 +386,12 @@ WATTN_DEVINL void pa_output(const PagedAttendParams &p, const PaTile &a, int row
   }
 }
 
-// The loads of a warp's share, running ahead of its products.
+// A load warp's walk over its share.
 struct PaLoads {
   PaStart w;
   int units, stages, weight;  // of the current item
   int t, to, end;        // its next stage, the share's last, its positions
   int page, in_page;     // table index and row of the next box
-  int head_row;          // first row of the head in a page's keys (and values)
-  int slot;              // ring slot of the next stage
-  uint32_t announced;    // items announced
   int base, entry;       // lane i holds table entry base + i of the request
 };
 
@@ -396,24 +402,21 @@ WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
   ld.units = pa_units(p, w.q, w.rt);
   ld.stages = pa_stages(p, w.q, w.rt);
   ld.weight = pa_weight(w.q, w.rt);
-  // (both differences are below an item's units where they are divided)
-  const long long d = w.lo - w.at, e = w.hi - w.at;
-  ld.t = d <= 0 ? 0 : ((int)d + ld.weight - 1) / ld.weight;
-  ld.to = e >= ld.units ? ld.stages : min(ld.stages, ((int)e + ld.weight - 1) / ld.weight);
+  const int d = w.lo - w.at, e = w.hi - w.at;
+  ld.t = d <= 0 ? 0 : (d + ld.weight - 1) / ld.weight;
+  ld.to = e >= ld.units ? ld.stages : min(ld.stages, (e + ld.weight - 1) / ld.weight);
   ld.end = pa_end(p, w.q, w.rt);
   ld.page = ld.t * kPaKeys / p.page_rows;
   ld.in_page = ld.t * kPaKeys - ld.page * p.page_rows;
-  ld.head_row = w.head * p.page_rows;
   return ld.t < ld.to;
 }
 
-// Announces the current item to the products.
+// Announces the current item to the compute warp.
 template <typename T>
-WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, int warp, int lane) {
+WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaItem &it, const PaLoads &ld, int lane) {
   const PaStart &w = ld.w;
   const int row = w.rt * kPaRows, row0 = w.q.first + row, nr = min(kPaRows, w.q.n - row);
   if (lane == 0) {
-    PaItem &it = s.queue[warp][ld.announced % kPaQueue];
     it.row0 = row0;
     it.nr = nr;
     it.row = row;
@@ -426,71 +429,105 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaSmem &s, PaLoads &ld
     it.weight = ld.weight;
     it.at = w.at;
   }
-  if (lane < nr) {  // the products will want the query rows and masks soon
+  if (lane < nr) {  // its query rows and masks will be wanted soon
     asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const T *>(p.q) +
                                                   (int64_t)(row0 + lane) * p.q_rs + w.head * 64));
     if (p.row_mask != nullptr)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(p.row_mask +
                                                     (int64_t)(row0 + lane) * p.mask_words));
   }
-  ++ld.announced;
 }
 
-// Issues the next stage's loads into the ring slot that the products have
-// left, announcing its item if it is the first of it.
+// A load warp: fills the ring of compute warp k, stage by stage over its
+// share's items, each announced before its first stage; an item without rows
+// ends the share.
 template <typename T>
-WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
-                           const CUtensorMap &map_tail, int warp, int lane) {
+WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorMap &map,
+                          const CUtensorMap &map_tail, int k, int lane) {
+  PaLoads ld;
+  ld.w = pa_start(p, s, k);
+  ld.base = INT_MIN / 2;
+  ld.entry = 0;
   PaStart &w = ld.w;
-  while (ld.t >= ld.to) {  // on to the next item of the share
-    w.at += ld.units;
-    if (w.at >= w.hi) return;
-    if (++w.rt * kPaRows >= w.q.n) {
-      w.rt = 0;
-      if (++w.head == p.n_heads) {
-        w.head = 0;
-        do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
-        ld.base = INT_MIN / 2;  // another request's table
-      }
-    }
-    if (pa_enter(p, ld)) pa_announce<T>(p, s, ld, warp, lane);
-  }
-  const int rows = ld.end - ld.t * kPaKeys;
-  const bool tail = rows < kPaKeys;
-  const int step = tail ? kPaTail : p.box_rows;
-  const int boxes = rows > step && step < kPaKeys ? 2 : 1;  // a step is a stage, or half of one
-  uint64_t *bar = &s.full[warp][ld.slot];
+  int slot = 0;
+  uint32_t phase = 1;  // (a wait for the phase before the first passes)
+  uint32_t items = 0;
+  bool fresh = w.lo < w.hi && pa_enter(p, ld);  // an item not yet announced
+  if (w.lo >= w.hi) ld.t = ld.to = ld.units = 0;
 #pragma unroll 1
-  for (int b = 0; b < boxes; ++b) {
-    if ((unsigned)(ld.page - ld.base) >= 32u) {
-      ld.base = ld.page;
-      ld.entry = ld.base + lane < p.max_pages ? p.table[w.s * p.table_stride + ld.base + lane] : 0;
-    }
-    int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
-    if (lane == 0) {
-      if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);
-      if ((unsigned)page >= (unsigned)p.n_pages) {
-        report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
-        page = 0;
+  for (;;) {
+    bool more = w.lo < w.hi;
+    while (more && ld.t >= ld.to) {  // on to the next item of the share
+      w.at += ld.units;
+      if (w.at >= w.hi) {
+        more = false;
+        break;
       }
-      const int c1 = ld.head_row + ld.in_page, c3 = page * p.n_layers + p.layer;
-      uint8_t *dst = &s.kv[warp][ld.slot][0][0] + b * kPaTail * 128;
-      if (step == kPaKeys) {
-        tma_load_4d(dst, &map, bar, 0, c1, 0, c3);  // the keys, and behind them the values
-      } else {  // 16 rows of each
-        tma_load_4d(dst, &map_tail, bar, 0, c1, 0, c3);
-        tma_load_4d(dst + kPaKeys * 128, &map_tail, bar, 0, c1, 1, c3);
+      if (++w.rt * kPaRows >= w.q.n) {
+        w.rt = 0;
+        if (++w.head == p.n_heads) {
+          w.head = 0;
+          do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
+          ld.base = INT_MIN / 2;  // another request's table
+        }
+      }
+      fresh = pa_enter(p, ld);
+    }
+    const bool ok = mbar_wait(&s.empty[k][slot], phase, &s.abort, p.status, (4 << 24) | (3 << 16));
+    if (!__all_sync(0xffffffffu, ok)) return;
+    uint64_t *bar = &s.full[k][slot];
+    PaItem &it = s.queue[k][items % kPaQueue];
+    if (!more) {
+      if (lane == 0) {
+        it.nr = 0;
+        mbar_arrive(bar);
+      }
+      return;
+    }
+    if (fresh) {
+      pa_announce<T>(p, it, ld, lane);
+      ++items;
+      fresh = false;
+    }
+    const int rows = ld.end - ld.t * kPaKeys;
+    const bool tail = rows < kPaKeys;
+    const int step = tail ? kPaTail : p.box_rows;
+    const int boxes = rows > step && step < kPaKeys ? 2 : 1;  // a step is a stage, or half of one
+#pragma unroll 1
+    for (int b = 0; b < boxes; ++b) {
+      if ((unsigned)(ld.page - ld.base) >= 32u) {
+        ld.base = ld.page;
+        ld.entry = ld.base + lane < p.max_pages ? p.table[w.s * p.table_stride + ld.base + lane] : 0;
+      }
+      int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
+      if (lane == 0) {
+        if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);  // (releases the announcement too)
+        if ((unsigned)page >= (unsigned)p.n_pages) {
+          report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
+          page = 0;
+        }
+        const int c1 = w.head * p.page_rows + ld.in_page, c3 = page * p.n_layers + p.layer;
+        uint8_t *dst = &s.kv[k][slot][0][0] + b * kPaTail * 128;
+        if (step == kPaKeys) {
+          tma_load_4d(dst, &map, bar, 0, c1, 0, c3);  // the keys, and behind them the values
+        } else {  // 16 rows of each
+          tma_load_4d(dst, &map_tail, bar, 0, c1, 0, c3);
+          tma_load_4d(dst + kPaKeys * 128, &map_tail, bar, 0, c1, 1, c3);
+        }
+      }
+      ld.in_page += step;
+      if (ld.in_page >= p.page_rows) {
+        ld.in_page = 0;
+        ++ld.page;
       }
     }
-    ld.in_page += step;
-    if (ld.in_page >= p.page_rows) {
-      ld.in_page = 0;
-      ++ld.page;
+    ++ld.t;
+    if (++slot == kPaStages) {
+      slot = 0;
+      phase ^= 1;
     }
+    __syncwarp();
   }
-  ld.slot = ld.slot == kPaStages - 1 ? 0 : ld.slot + 1;
-  ++ld.t;
-  __syncwarp();
 }
 
 // The products of one item's stages: MT tiles of 16 query rows against 32
@@ -499,9 +536,8 @@ WATTN_DEVINL void pa_issue(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, c
 // both MT is 14 % slower over single rows, its branches being predicated
 // products; one more for few rows costs more instruction fetches than it saves.)
 template <typename T, typename OutT, int MT>
-WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, const CUtensorMap &map,
-                          const CUtensorMap &map_tail, const PaItem &it, uint32_t &pos, int warp,
-                          int lane) {
+WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, const PaItem &it, uint32_t &pos,
+                          int warp, int lane) {
   const int g = lane >> 2, t4 = lane & 3;
   const bool few = MT == 1 && it.nr <= 8;
   uint32_t qa[MT][4][4];
@@ -557,8 +593,6 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
               pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
           }
     }
-    // The slot of the stage before this one is free (3 slots, 2 in flight).
-    pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
     const int off = t * kPaKeys - it.len, left = it.end - t * kPaKeys;
     const bool drafts = off + kPaKeys > 0;       // the stage reaches past the cached positions
     const bool special = drafts || left < kPaKeys;
@@ -746,6 +780,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
       }
     }
     __syncwarp();  // every lane has read the stage
+    if (lane == 0) mbar_arrive(&s.empty[warp][slot]);
   }
   if (few) {
 #pragma unroll
@@ -766,6 +801,9 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, PaLoads &ld, co
   }
 }
 
+// Barrier of the compute warps (the load warps have left by then).
+WATTN_DEVINL void pa_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
 // Adds shares c0 .. c1's partials of a cut item, in order (`starts`: c0's is
 // the one that starts it).
 WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c1, bool starts, int mt,
@@ -784,7 +822,7 @@ WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c
 template <typename OutT>
 WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int lane) {
   const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps, ctas = gridDim.x * kPaWarps;
-  __syncthreads();
+  pa_sync();
   if (tid < 2 * kPaWarps) {
     const PaItem &it = s.cut[tid >> 1][tid & 1];
     int w0 = 0, w1 = -1;
@@ -793,12 +831,12 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int
       if (s.cut[i >> 1][i & 1].stages > 0 && s.cut[i >> 1][i & 1].at == it.at) fresh = false;
     if (fresh) {
       w0 = pa_owner(s.shares, it.at);
-      w1 = pa_owner(s.shares, it.at + (long long)(it.stages - 1) * it.weight);
+      w1 = pa_owner(s.shares, it.at + (it.stages - 1) * it.weight);
     }
     s.merge_first[tid] = w0;
     s.merge_last[tid] = w1;
   }
-  __syncthreads();
+  pa_sync();
   int turn = 0;
 #pragma unroll 1
   for (int e = 0; e < 2 * kPaWarps; ++e) {
@@ -849,35 +887,38 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   extern __shared__ uint8_t pa_smem_raw[];
   PaSmem &s = *reinterpret_cast<PaSmem *>(
       (reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (lane == 0) {
-    for (int st = 0; st < kPaStages; ++st) mbar_init(&s.full[warp][st], 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0 && warp < kPaWarps) {
+    for (int st = 0; st < kPaStages; ++st) {
+      mbar_init(&s.full[warp][st], 1);
+      mbar_init(&s.empty[warp][st], 1);
+    }
     s.cut[warp][0].stages = s.cut[warp][1].stages = 0;
     s.abort = 0;
     fence_barrier_init();
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  PaLoads ld;
-  ld.w = pa_find_share(p, s);
-  ld.slot = 0;
-  ld.announced = 0;
-  ld.base = INT_MIN / 2;
-  ld.entry = 0;
-  if (ld.w.lo < ld.w.hi) {
-    if (pa_enter(p, ld)) pa_announce<T>(p, s, ld, warp, lane);
-#pragma unroll 1
-    for (int st = 0; st < kPaStages - 1; ++st) pa_issue<T>(p, s, ld, map, map_tail, warp, lane);
-    __syncwarp();
+  pa_find_shares(p, s);
+  if (warp >= kPaWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaLoadRegs));
+    pa_load<T>(p, s, map, map_tail, warp - kPaWarps, lane);
+    return;
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPaComputeRegs));
     uint32_t pos = 0;  // ring slot of the next stage, and in bit 31 its barrier's phase
 #pragma unroll 1
-    for (uint32_t i = 0; i < ld.announced; ++i) {
+    for (uint32_t i = 0;; ++i) {
+      // The next stage's barrier covers the announcement of its item.
+      if (!mbar_wait(&s.full[warp][pos & 3], pos >> 31, &s.abort, p.status, (4 << 24) | (2 << 16))) break;
       const PaItem it = s.queue[warp][i % kPaQueue];
-      if (it.nr <= 16) pa_item<T, OutT, 1>(p, s, ld, map, map_tail, it, pos, warp, lane);
-      else pa_item<T, OutT, 2>(p, s, ld, map, map_tail, it, pos, warp, lane);
+      if (it.nr == 0) break;
+      if (it.nr <= 16) pa_item<T, OutT, 1>(p, s, it, pos, warp, lane);
+      else pa_item<T, OutT, 2>(p, s, it, pos, warp, lane);
     }
+    __syncwarp();
+    pa_finish<OutT>(p, s, warp, lane);
   }
-  pa_finish<OutT>(p, s, warp, lane);
 }
 
 int pa_grid() {
@@ -912,6 +953,14 @@ int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
   if (rc != WATTN_OK) return rc;
   constexpr int smem = (int)sizeof(PaSmem) + 1024;
   auto kern = paged_attend_stream_kernel<T, OutT>;
+  // Once per process and type: the warpgroups' register split counts on what
+  // the kernel is launched with (with fewer it would wait for ever).
+  static const int regs = [&] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs != kPaRegs)
+    return set_error(WATTN_ERR_CUDA, "paged_attend: built for %d registers a thread, not %d", regs, kPaRegs);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(paged_attend)");
   launch_pdl(kern, dim3(pa_grid()), dim3(kPaThreads), smem, st, map, map_tail, p);
