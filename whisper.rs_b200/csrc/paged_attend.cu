@@ -50,9 +50,8 @@ struct PagedAttendParams {
 
 // ---------------------------------------------------------------- shares of the work
 
-constexpr int kPaKeys = 32;       // keys of a stage
 constexpr int kPaTail = 16;       // rows of a tail box: the pool's unit of page rows
-constexpr int kPaRows = 32;       // rows of a row tile
+constexpr int kPaStageBytes = 8192;  // keys, then values
 constexpr int kPaStages = 3;      // stages of a warp's ring
 constexpr int kPaWarps = 4;       // compute warps (one warpgroup), and as many load warps
 constexpr int kPaThreads = 2 * kPaWarps * 32;
@@ -65,6 +64,23 @@ constexpr int kPaStageUnits = 2, kPaWideUnits = 3, kPaItemUnits = 2;
 constexpr int kPaMinUnits = 8;    // units of a share below which fewer warps work
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
+
+// By type of the pool: keys of a stage (8 KB of keys and values), rows of a
+// row tile.
+template <typename T> struct PaType;
+template <> struct PaType<__half> {
+  static constexpr int kKeys = 32, kRows = 32;
+  static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
+  static constexpr bool kResidual = false;  // f16 weights: 2^-11 each, within the 2e-3 bar
+};
+template <> struct PaType<__nv_bfloat16> {
+  static constexpr int kKeys = 32, kRows = 32;
+  static constexpr uint32_t kOne = 0x3f80u, kInf = 0x7f80u;
+  static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
+};
+template <> struct PaType<float> {
+  static constexpr int kKeys = 16, kRows = 16;
+};
 
 // One request as the kernel sees it. One whose arrays are out of range has
 // no rows here (and is reported).
@@ -80,27 +96,27 @@ WATTN_DEVINL PaSeq pa_seq(const PagedAttendParams &p, int s, bool *bad) {
   return {a, ok ? b - a : 0, len};
 }
 // Positions that rows of tile rt may see.
-WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return q.len + min(q.n, p.row_mask != nullptr ? p.mask_bits : kPaRows * (rt + 1));
+template <typename T> WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return q.len + min(q.n, p.row_mask != nullptr ? p.mask_bits : PaType<T>::kRows * (rt + 1));
 }
-WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return (pa_end(p, q, rt) + kPaKeys - 1) / kPaKeys;
+template <typename T> WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return (pa_end<T>(p, q, rt) + PaType<T>::kKeys - 1) / PaType<T>::kKeys;
 }
 // Units that a stage of row tile rt costs: two tiles of 16 rows cost more
 // than one; kPaItemUnits are what an item costs besides its stages.
-WATTN_DEVINL int pa_weight(const PaSeq &q, int rt) {
-  return q.n - rt * kPaRows > 16 ? kPaWideUnits : kPaStageUnits;
+template <typename T> WATTN_DEVINL int pa_weight(const PaSeq &q, int rt) {
+  return PaType<T>::kRows > 16 && q.n - rt * PaType<T>::kRows > 16 ? kPaWideUnits : kPaStageUnits;
 }
-WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return pa_stages(p, q, rt) * pa_weight(q, rt) + kPaItemUnits;
+template <typename T> WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return pa_stages<T>(p, q, rt) * pa_weight<T>(q, rt) + kPaItemUnits;
 }
 // Units of one head of a request: its full row tiles, then the last.
-WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
-  if (q.n <= kPaRows) return q.n > 0 ? pa_units(p, q, 0) : 0;
-  const long long full = (q.n - 1) / kPaRows;
-  long long stages = full * pa_stages(p, q, 0);
+template <typename T> WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
+  if (q.n <= PaType<T>::kRows) return q.n > 0 ? pa_units<T>(p, q, 0) : 0;
+  const long long full = (q.n - 1) / PaType<T>::kRows;
+  long long stages = full * pa_stages<T>(p, q, 0);
   if (p.row_mask == nullptr) stages += full * (full - 1) / 2;  // one more from tile to tile
-  return stages * kPaWideUnits + full * kPaItemUnits + pa_units(p, q, (int)full);
+  return stages * pa_weight<T>(q, 0) + full * kPaItemUnits + pa_units<T>(p, q, (int)full);
 }
 
 // `total` units (below 2^31) in `parts` shares, in order: the first `more` of
@@ -141,7 +157,7 @@ struct PaItem {
 };
 
 struct PaSmem {
-  uint8_t kv[kPaWarps][kPaStages][2][kPaKeys * 128];  // keys, values
+  uint8_t kv[kPaWarps][kPaStages][kPaStageBytes];
   uint64_t full[kPaWarps][kPaStages], empty[kPaWarps][kPaStages];
   PaItem queue[kPaWarps][kPaQueue];
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
@@ -156,7 +172,7 @@ struct PaSmem {
 // The shares. All threads of the CTA add up the units of a run of requests
 // each; the sums are scanned, and for each share of the CTA the run that
 // holds its first unit is noted.
-WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
+template <typename T> WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.n_seqs + kPaThreads - 1) / kPaThreads;
   const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
@@ -166,7 +182,7 @@ WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
     bool bad;
     const PaSeq q = pa_seq(p, i, &bad);
     if (bad) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
-    mine += pa_head_units(p, q) * p.n_heads;
+    mine += pa_head_units<T>(p, q) * p.n_heads;
   }
   long long inc = mine;
 #pragma unroll
@@ -204,7 +220,7 @@ WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
 }
 
 // Share blockIdx.x * kPaWarps + k: walks to its first item.
-WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k) {
+template <typename T> WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k) {
   PaStart w;
   w.lo = w.hi = 0;
   const int c = blockIdx.x * kPaWarps + k;
@@ -214,7 +230,7 @@ WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k
   w.at = s.run_at[k];
   for (w.s = s.run_first[k];; ++w.s) {
     w.q = pa_seq(p, w.s, nullptr);
-    const int u = (int)pa_head_units(p, w.q);
+    const int u = (int)pa_head_units<T>(p, w.q);
     if (w.lo - w.at < (long long)u * p.n_heads) {
       w.head = (w.lo - w.at) / u;
       w.at += w.head * u;
@@ -223,7 +239,7 @@ WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k
     w.at += u * p.n_heads;
   }
   for (w.rt = 0;; ++w.rt) {
-    const int u = pa_units(p, w.q, w.rt);
+    const int u = pa_units<T>(p, w.q, w.rt);
     if (w.lo - w.at < u) break;
     w.at += u;
   }
@@ -231,16 +247,6 @@ WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k
 }
 
 // ---------------------------------------------------------------- 16-bit pools
-
-template <typename T> struct PaType;
-template <> struct PaType<__half> {
-  static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
-  static constexpr bool kResidual = false;  // f16 weights: 2^-11 each, within the 2e-3 bar
-};
-template <> struct PaType<__nv_bfloat16> {
-  static constexpr uint32_t kOne = 0x3f80u, kInf = 0x7f80u;
-  static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
-};
 
 // (volatile: else the compiler computes the products of a branch not taken)
 template <typename T>
@@ -368,7 +374,7 @@ WATTN_DEVINL void pa_add(PaTile &a, const float4 *part) {
   }
 }
 // The outputs of packed rows row0 + g and + 8 (nr rows exist), head h.
-template <typename OutT>
+template <typename T, typename OutT>
 WATTN_DEVINL void pa_output(const PagedAttendParams &p, const PaTile &a, int row0, int nr, int head,
                             int lane) {
   const int g = lane >> 2, t4 = lane & 3;
@@ -379,10 +385,23 @@ WATTN_DEVINL void pa_output(const PagedAttendParams &p, const PaTile &a, int row
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if (g + 8 * h >= nr) continue;
     const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-    const int64_t at = (int64_t)(row0 + g + 8 * h) * p.o_rs + head * 64 + 2 * t4;
+    const int64_t at = (int64_t)(row0 + g + 8 * h) * p.o_rs + head * 64;
+    if constexpr (sizeof(T) == 4) {  // (the f32 products' order of dims: pa_item)
+      float *o = reinterpret_cast<float *>(p.o) + at + (t4 >> 1) * 32 + (t4 & 1) * 8;
 #pragma unroll
-    for (int db = 0; db < 8; ++db)
-      pa_store2<OutT>(p.o, at + db * 8, a.o[db][2 * h] * inv, a.o[db][2 * h + 1] * inv);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = 2 * h + e;
+          *reinterpret_cast<float4 *>(o + j * 16 + e * 4) =
+              make_float4(a.o[4 * j][c] * inv, a.o[4 * j + 1][c] * inv, a.o[4 * j + 2][c] * inv,
+                          a.o[4 * j + 3][c] * inv);
+        }
+    } else {
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+        pa_store2<OutT>(p.o, at + 2 * t4 + db * 8, a.o[db][2 * h] * inv, a.o[db][2 * h + 1] * inv);
+    }
   }
 }
 
@@ -397,17 +416,17 @@ struct PaLoads {
 
 // The current item's stages that this share holds (a stage belongs to the
 // share that holds its first unit), and where their keys are. False if none.
-WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
+template <typename T> WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
   const PaStart &w = ld.w;
-  ld.units = pa_units(p, w.q, w.rt);
-  ld.stages = pa_stages(p, w.q, w.rt);
-  ld.weight = pa_weight(w.q, w.rt);
+  ld.units = pa_units<T>(p, w.q, w.rt);
+  ld.stages = pa_stages<T>(p, w.q, w.rt);
+  ld.weight = pa_weight<T>(w.q, w.rt);
   const int d = w.lo - w.at, e = w.hi - w.at;
   ld.t = d <= 0 ? 0 : (d + ld.weight - 1) / ld.weight;
   ld.to = e >= ld.units ? ld.stages : min(ld.stages, (e + ld.weight - 1) / ld.weight);
-  ld.end = pa_end(p, w.q, w.rt);
-  ld.page = ld.t * kPaKeys / p.page_rows;
-  ld.in_page = ld.t * kPaKeys - ld.page * p.page_rows;
+  ld.end = pa_end<T>(p, w.q, w.rt);
+  ld.page = ld.t * PaType<T>::kKeys / p.page_rows;
+  ld.in_page = ld.t * PaType<T>::kKeys - ld.page * p.page_rows;
   return ld.t < ld.to;
 }
 
@@ -415,7 +434,7 @@ WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
 template <typename T>
 WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaItem &it, const PaLoads &ld, int lane) {
   const PaStart &w = ld.w;
-  const int row = w.rt * kPaRows, row0 = w.q.first + row, nr = min(kPaRows, w.q.n - row);
+  const int row = w.rt * PaType<T>::kRows, row0 = w.q.first + row, nr = min(PaType<T>::kRows, w.q.n - row);
   if (lane == 0) {
     it.row0 = row0;
     it.nr = nr;
@@ -445,14 +464,14 @@ template <typename T>
 WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorMap &map,
                           const CUtensorMap &map_tail, int k, int lane) {
   PaLoads ld;
-  ld.w = pa_start(p, s, k);
+  ld.w = pa_start<T>(p, s, k);
   ld.base = INT_MIN / 2;
   ld.entry = 0;
   PaStart &w = ld.w;
   int slot = 0;
   uint32_t phase = 1;  // (a wait for the phase before the first passes)
   uint32_t items = 0;
-  bool fresh = w.lo < w.hi && pa_enter(p, ld);  // an item not yet announced
+  bool fresh = w.lo < w.hi && pa_enter<T>(p, ld);  // an item not yet announced
   if (w.lo >= w.hi) ld.t = ld.to = ld.units = 0;
 #pragma unroll 1
   for (;;) {
@@ -463,7 +482,7 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
         more = false;
         break;
       }
-      if (++w.rt * kPaRows >= w.q.n) {
+      if (++w.rt * PaType<T>::kRows >= w.q.n) {
         w.rt = 0;
         if (++w.head == p.n_heads) {
           w.head = 0;
@@ -471,7 +490,7 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
           ld.base = INT_MIN / 2;  // another request's table
         }
       }
-      fresh = pa_enter(p, ld);
+      fresh = pa_enter<T>(p, ld);
     }
     const bool ok = mbar_wait(&s.empty[k][slot], phase, &s.abort, p.status, (4 << 24) | (3 << 16));
     if (!__all_sync(0xffffffffu, ok)) return;
@@ -489,10 +508,11 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
       ++items;
       fresh = false;
     }
-    const int rows = ld.end - ld.t * kPaKeys;
-    const bool tail = rows < kPaKeys;
-    const int step = tail ? kPaTail : p.box_rows;
-    const int boxes = rows > step && step < kPaKeys ? 2 : 1;  // a step is a stage, or half of one
+    constexpr bool kF32 = sizeof(T) == 4;
+    const int rows = ld.end - ld.t * PaType<T>::kKeys;
+    const bool tail = rows < PaType<T>::kKeys;
+    const int step = kF32 || tail ? kPaTail : p.box_rows;
+    const int boxes = rows > step && step < PaType<T>::kKeys ? 2 : 1;  // a step is a stage, or half of one
 #pragma unroll 1
     for (int b = 0; b < boxes; ++b) {
       if ((unsigned)(ld.page - ld.base) >= 32u) {
@@ -501,18 +521,21 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
       }
       int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
       if (lane == 0) {
-        if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 256);  // (releases the announcement too)
+        if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 4 * 32 * sizeof(T));  // (releases the announcement too)
         if ((unsigned)page >= (unsigned)p.n_pages) {
           report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
           page = 0;
         }
         const int c1 = w.head * p.page_rows + ld.in_page, c3 = page * p.n_layers + p.layer;
-        uint8_t *dst = &s.kv[k][slot][0][0] + b * kPaTail * 128;
-        if (step == kPaKeys) {
+        uint8_t *dst = s.kv[k][slot] + b * kPaTail * 128;
+        if (kF32) {  // dims 0 to 31 of the keys and of the values, then the others
+          tma_load_4d(dst, &map, bar, 0, c1, 0, c3);
+          tma_load_4d(dst + kPaStageBytes / 2, &map, bar, 32, c1, 0, c3);
+        } else if (step == PaType<T>::kKeys) {
           tma_load_4d(dst, &map, bar, 0, c1, 0, c3);  // the keys, and behind them the values
         } else {  // 16 rows of each
           tma_load_4d(dst, &map_tail, bar, 0, c1, 0, c3);
-          tma_load_4d(dst + kPaKeys * 128, &map_tail, bar, 0, c1, 1, c3);
+          tma_load_4d(dst + PaType<T>::kKeys * 128, &map_tail, bar, 0, c1, 1, c3);
         }
       }
       ld.in_page += step;
@@ -571,7 +594,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, const PaItem &i
     mbar_wait(&s.full[warp][slot], pos >> 31, &s.abort, p.status,
               (4 << 24) | (1 << 16) | ((t & 0xff) << 8));
     pos = slot == kPaStages - 1 ? (pos & 0x80000000u) ^ 0x80000000u : pos + 1;
-    const uint32_t ktile = smem_u32(&s.kv[warp][slot][0][0]), vtile = ktile + kPaKeys * 128;
+    const uint32_t ktile = smem_u32(s.kv[warp][slot]), vtile = ktile + PaType<T>::kKeys * 128;
     float sc[MT][4][4];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -593,9 +616,9 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, const PaItem &i
               pa_mma<T>(sc[mt][nb], qa[mt][2 * ks + half], r[nb][2 * half], r[nb][2 * half + 1]);
           }
     }
-    const int off = t * kPaKeys - it.len, left = it.end - t * kPaKeys;
-    const bool drafts = off + kPaKeys > 0;       // the stage reaches past the cached positions
-    const bool special = drafts || left < kPaKeys;
+    const int off = t * PaType<T>::kKeys - it.len, left = it.end - t * PaType<T>::kKeys;
+    const bool drafts = off + PaType<T>::kKeys > 0;       // the stage reaches past the cached positions
+    const bool special = drafts || left < PaType<T>::kKeys;
     if (special) {
       // lane r finds what row r sees
       const uint32_t sees =
@@ -795,11 +818,217 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, const PaItem &i
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     if (whole)
-      pa_output<OutT>(p, a[mt], it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+      pa_output<T, OutT>(p, a[mt], it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
     else
       pa_put(pa_part(p, blockIdx.x * kPaWarps + warp, starts, mt, lane), a[mt]);
   }
 }
+
+// ---------------------------------------------------------------- f32 pools
+//
+// The same walk with 16-key stages and tiles of 16 rows on tf32 products,
+// three for each: every operand enters as x = hi + lo, hi its upper 11
+// significant bits and lo those of the rest, and hi hi + hi lo + lo hi leaves
+// out 2^-22 of each product at most.
+WATTN_DEVINL void pa_mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+WATTN_DEVINL void pa_split(float x, uint32_t &hi, uint32_t &lo) {
+  constexpr uint32_t kTf32 = 0xffffe000u;  // sign, exponent, 10 bits
+  hi = __float_as_uint(x) & kTf32;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & kTf32;
+}
+WATTN_DEVINL float4 pa_lds(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// The order of dims in the products is free as long as both operands share
+// it, and chosen so that every lane reads 16 bytes and no bank meets twice:
+// K: step (blk, j, pair) takes dims 32 blk + 8 t4 + 4 j + 2 pair (+ 1);
+// V: column g of tile (j, e) is dim 32 (g >> 2) + 4 ((g & 3) + 4 j) + e.
+WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem &s, const PaItem &it, uint32_t &pos,
+                              int warp, int lane) {
+  constexpr int kKeys = PaType<float>::kKeys;
+  const int g = lane >> 2, t4 = lane & 3;
+  uint32_t qh[8][4], ql[8][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {  // c = 2 blk + j
+      const int r = h * 8 + g;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < it.nr)
+        x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.q) +
+                                              (int64_t)(it.row0 + r) * p.q_rs + it.head * 64 +
+                                              (c >> 1) * 32 + 8 * t4 + (c & 1) * 4);
+      pa_split(x.x, qh[2 * c][h], ql[2 * c][h]);
+      pa_split(x.y, qh[2 * c][2 + h], ql[2 * c][2 + h]);
+      pa_split(x.z, qh[2 * c + 1][h], ql[2 * c + 1][h]);
+      pa_split(x.w, qh[2 * c + 1][2 + h], ql[2 * c + 1][2 + h]);
+    }
+  PaTile a;
+#pragma unroll
+  for (int db = 0; db < 8; ++db) a.o[db][0] = a.o[db][1] = a.o[db][2] = a.o[db][3] = 0.f;
+  a.m[0] = a.m[1] = -INFINITY;
+  a.l[0] = a.l[1] = 0.f;
+#pragma unroll 1
+  for (int t = it.from; t < it.to; ++t) {
+    const int slot = pos & 3;
+    mbar_wait(&s.full[warp][slot], pos >> 31, &s.abort, p.status,
+              (4 << 24) | (1 << 16) | ((t & 0xff) << 8));
+    pos = slot == kPaStages - 1 ? (pos & 0x80000000u) ^ 0x80000000u : pos + 1;
+    const uint32_t ktile = smem_u32(s.kv[warp][slot]), vtile = ktile + kKeys * 128;
+    float sc[2][4], sx[2][4], sy[2][4];  // hi hi, hi lo, lo hi
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[nb][e] = sx[nb][e] = sy[nb][e] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float4 x[2];
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+        x[nb] = pa_lds(ktile + (c >> 1) * (kPaStageBytes / 2) + (nb * 8 + g) * 128 +
+                       (((2 * t4 + (c & 1)) ^ g) << 4));
+#pragma unroll
+      for (int pair = 0; pair < 2; ++pair)
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          uint32_t h0, l0, h1, l1;
+          pa_split(pair ? x[nb].z : x[nb].x, h0, l0);
+          pa_split(pair ? x[nb].w : x[nb].y, h1, l1);
+          pa_mma_tf32(sc[nb], qh[2 * c + pair], h0, h1);
+          pa_mma_tf32(sx[nb], qh[2 * c + pair], l0, l1);
+          pa_mma_tf32(sy[nb], ql[2 * c + pair], h0, h1);
+        }
+    }
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[nb][e] += sx[nb][e] + sy[nb][e];
+    const int off = t * kKeys - it.len, left = it.end - t * kKeys;
+    const bool drafts = off + kKeys > 0;  // the stage reaches past the cached positions
+    const bool special = drafts || left < kKeys;
+    if (special) {
+      const uint32_t sees =
+          lane < it.nr ? pa_visible(p, it.row0 + lane, it.row + lane, off, left) : 0u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t vis = __shfl_sync(0xffffffffu, sees, h * 8 + g) >> (2 * t4);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!(vis >> (nb * 8 + e) & 1u)) sc[nb][2 * h + e] = -INFINITY;
+      }
+    }
+    float mu[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = fmax3(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), sc[1][2 * h], sc[1][2 * h + 1]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mc = mx * p.scale_log2;
+      if (mc > a.m[h] + 8.0f) {
+        const float alpha = ex2(a.m[h] - mc);
+        a.l[h] *= alpha;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+          a.o[db][2 * h] *= alpha;
+          a.o[db][2 * h + 1] *= alpha;
+        }
+        a.m[h] = mc;
+      }
+      mu[h] = a.m[h] == -INFINITY ? 0.f : a.m[h];
+    }
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      // two value rows, of keys 2 t4 and 2 t4 + 1, in column g of the 8 tiles
+      float v[2][8];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int key = nb * 8 + 2 * t4 + b;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float4 x = pa_lds(vtile + (g >> 2) * (kPaStageBytes / 2) + key * 128 +
+                                  ((((g & 3) + 4 * j) ^ (2 * t4 + b)) << 4));
+          v[b][4 * j] = x.x;
+          v[b][4 * j + 1] = x.y;
+          v[b][4 * j + 2] = x.z;
+          v[b][4 * j + 3] = x.w;
+        }
+        if (special && key >= left)  // behind the last position: anything
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[b][i] = 0.f;
+      }
+      if (drafts) {  // a draft's value that is not finite: only for the rows that see it
+        float nil = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) nil = fmaf(v[0][i], 0.f, fmaf(v[1][i], 0.f, nil));
+        if (__any_sync(0xffffffffu, nil != nil)) {
+          const uint32_t one = __float_as_uint(1.f);
+          uint32_t see[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            see[e] = sc[nb][2 * (e & 1) + (e >> 1)] != -INFINITY ? one : 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float np[4] = {0, 0, 0, 0}, nm[4] = {0, 0, 0, 0}, nn[4] = {0, 0, 0, 0};
+            const float x = v[0][i], y = v[1][i];
+            pa_mma_tf32(np, see, x == INFINITY ? one : 0u, y == INFINITY ? one : 0u);
+            pa_mma_tf32(nm, see, x == -INFINITY ? one : 0u, y == -INFINITY ? one : 0u);
+            pa_mma_tf32(nn, see, x != x ? one : 0u, y != y ? one : 0u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (np[e] > 0.f) a.o[i][e] += INFINITY;
+              if (nm[e] > 0.f) a.o[i][e] -= INFINITY;
+              if (nn[e] > 0.f) a.o[i][e] = NAN;
+            }
+            if (!(fabsf(x) < INFINITY)) v[0][i] = 0.f;
+            if (!(fabsf(y) < INFINITY)) v[1][i] = 0.f;
+          }
+        }
+      }
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // row g + 8 (e & 1), key 2 t4 + (e >> 1)
+        const float w = ex2(fmaf(sc[nb][2 * (e & 1) + (e >> 1)], p.scale_log2, -mu[e & 1]));
+        a.l[e & 1] += w;
+        pa_split(w, ph[e], pl[e]);
+      }
+      uint32_t vh[2][8], vl[2][8];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pa_split(v[b][i], vh[b][i], vl[b][i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], ph, vh[0][i], vh[1][i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], ph, vl[0][i], vl[1][i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], pl, vh[0][i], vh[1][i]);
+    }
+    __syncwarp();  // every lane has read the stage
+    if (lane == 0) mbar_arrive(&s.empty[warp][slot]);
+  }
+  const bool starts = it.from == 0;
+  if (starts && it.to == it.stages) {
+    pa_output<float, float>(p, a, it.row0, it.nr, it.head, lane);
+  } else {
+    if (lane == 0) s.cut[warp][starts ? 1 : 0] = it;
+    pa_put(pa_part(p, blockIdx.x * kPaWarps + warp, starts, 0, lane), a);
+  }
+}
+
+// ---------------------------------------------------------------- kernel
 
 // Barrier of the compute warps (the load warps have left by then).
 WATTN_DEVINL void pa_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -819,7 +1048,7 @@ WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c
 // The items cut by the shares of this CTA's warps, after all of them are
 // done, an item per warp: the CTA's parts of an item are merged, and where
 // several CTAs have parts the last of them to arrive merges theirs.
-template <typename OutT>
+template <typename T, typename OutT>
 WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int lane) {
   const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps, ctas = gridDim.x * kPaWarps;
   pa_sync();
@@ -850,7 +1079,7 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int
     for (int mt = 0; mt < tiles; ++mt) {
       PaTile a;
       pa_gather(p, a, first, last, first == w0, mt, lane);
-      if (alone) pa_output<OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+      if (alone) pa_output<T, OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
       else pa_put(pa_part(p, ctas + blockIdx.x, first == w0, mt, lane), a);
     }
     if (alone) continue;
@@ -872,7 +1101,7 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int
     for (int mt = 0; mt < tiles; ++mt) {
       PaTile a;
       pa_gather(p, a, ctas + c0, ctas + c1, true, mt, lane);
-      pa_output<OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+      pa_output<T, OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
     }
   }
 }
@@ -899,7 +1128,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  pa_find_shares(p, s);
+  pa_find_shares<T>(p, s);
   if (warp >= kPaWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaLoadRegs));
     pa_load<T>(p, s, map, map_tail, warp - kPaWarps, lane);
@@ -913,11 +1142,12 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
       if (!mbar_wait(&s.full[warp][pos & 3], pos >> 31, &s.abort, p.status, (4 << 24) | (2 << 16))) break;
       const PaItem it = s.queue[warp][i % kPaQueue];
       if (it.nr == 0) break;
-      if (it.nr <= 16) pa_item<T, OutT, 1>(p, s, it, pos, warp, lane);
+      if constexpr (sizeof(T) == 4) pa_item_f32(p, s, it, pos, warp, lane);
+      else if (it.nr <= 16) pa_item<T, OutT, 1>(p, s, it, pos, warp, lane);
       else pa_item<T, OutT, 2>(p, s, it, pos, warp, lane);
     }
     __syncwarp();
-    pa_finish<OutT>(p, s, warp, lane);
+    pa_finish<T, OutT>(p, s, warp, lane);
   }
 }
 
@@ -937,15 +1167,17 @@ template <typename T, typename OutT>
 int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
   // The pool as [page, layer][K|V][head, row][64]: one box holds a stage's
   // keys and its values; the tail map's boxes hold 16 rows of either.
-  const uint64_t kv_rows = (uint64_t)p.n_heads * p.page_rows;
-  p.box_rows = p.page_rows % kPaKeys == 0 ? kPaKeys : kPaTail;
+  // f32: boxes of half the dims of a stage's 16 keys and values.
+  const uint64_t kv_rows = (uint64_t)p.n_heads * p.page_rows, es = sizeof(T);
+  p.box_rows = p.page_rows % PaType<T>::kKeys == 0 ? PaType<T>::kKeys : kPaTail;
   const uint64_t dims[4] = {64, kv_rows, 2, (uint64_t)p.n_pages * p.n_layers};
-  const uint64_t strides[3] = {128, kv_rows * 128, kv_rows * 256};
-  const uint32_t box[4] = {64, kPaKeys, 2, 1}, box_tail[4] = {64, kPaTail, 1, 1};
+  const uint64_t strides[3] = {64 * es, kv_rows * 64 * es, kv_rows * 128 * es};
+  const uint32_t width = 128 / sizeof(T);
+  const uint32_t box[4] = {width, PaType<T>::kKeys, 2, 1}, box_tail[4] = {width, kPaTail, 1, 1};
   CUtensorMap map, map_tail;
   int rc = encode_tmap(&map_tail, tmap_dtype(dtype), 4, p.pool, dims, strides, box_tail,
                        CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc == WATTN_OK && p.box_rows == kPaKeys)
+  if (rc == WATTN_OK && p.box_rows == PaType<T>::kKeys)
     rc = encode_tmap(&map, tmap_dtype(dtype), 4, p.pool, dims, strides, box,
                      CU_TENSOR_MAP_SWIZZLE_128B);
   else
@@ -964,78 +1196,6 @@ int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(paged_attend)");
   launch_pdl(kern, dim3(pa_grid()), dim3(kPaThreads), smem, st, map, map_tail, p);
-  return check_launch("paged_attend");
-}
-
-// ---------------------------------------------------------------- f32 pools
-
-// One warp per (row, head): two dims a lane, an online softmax over the keys
-// one at a time.
-template <typename T, typename OutT>
-__global__ void paged_attend_simple_kernel(const PagedAttendParams p) {
-  grid_dep_wait();  // (launched with programmatic serialisation)
-  grid_dep_launch();
-  const int lane = threadIdx.x & 31;
-  const int r = blockIdx.x, head = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (head >= p.n_heads || r >= p.row_start[p.n_seqs]) return;
-  int lo = 0, hi = p.n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.row_start[mid] <= r) lo = mid; else hi = mid;
-  }
-  const int first = p.row_start[lo], n = p.row_start[lo + 1] - first, i = r - first;
-  const int len = max(0, p.seq_lens[lo]);
-  if (p.seq_lens[lo] < 0) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
-  if (i < 0 || i >= n) return;
-  const T *q = reinterpret_cast<const T *>(p.q) + (int64_t)r * p.q_rs + head * 64 + 2 * lane;
-  const float q0 = to_f32(q[0]) * p.scale_log2, q1 = to_f32(q[1]) * p.scale_log2;
-  const int64_t kv_off = (int64_t)p.n_heads * p.page_rows * 64;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  int64_t end = (int64_t)len + n;
-  if (end > (int64_t)p.max_pages * p.page_rows) {
-    report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
-    end = (int64_t)p.max_pages * p.page_rows;
-  }
-  for (int64_t at = 0; at < end; ++at) {
-    if (at >= len) {
-      const int j = (int)(at - len);
-      if (p.row_mask == nullptr) {
-        if (j > i) break;
-      } else if (j >= p.mask_words * 32 ||
-                 !(p.row_mask[(int64_t)r * p.mask_words + (j >> 5)] >> (j & 31) & 1)) {
-        continue;
-      }
-    }
-    const int64_t pi = at / p.page_rows;
-    const int page = pi < p.max_pages ? p.table[lo * p.table_stride + pi] : -1;
-    if (page < 0 || page >= p.n_pages) {
-      report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
-      continue;
-    }
-    const T *k = reinterpret_cast<const T *>(p.pool) +
-                 ((int64_t)page * p.n_layers + p.layer) * 2 * kv_off +
-                 ((int64_t)head * p.page_rows + at % p.page_rows) * 64 + 2 * lane;
-    float x = fmaf(q0, to_f32(k[0]), q1 * to_f32(k[1]));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    const float mn = fmaxf(m, x);
-    const float a = m == -INFINITY ? 0.f : ex2(m - mn);
-    const float w = x == -INFINITY ? 0.f : ex2(x - mn);
-    m = mn;
-    l = fmaf(l, a, w);
-    o0 = fmaf(o0, a, w * to_f32(k[kv_off]));
-    o1 = fmaf(o1, a, w * to_f32(k[kv_off + 1]));
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  OutT *o = reinterpret_cast<OutT *>(p.o) + (int64_t)r * p.o_rs + head * 64 + 2 * lane;
-  o[0] = from_f32<OutT>(o0 * inv);
-  o[1] = from_f32<OutT>(o1 * inv);
-}
-
-template <typename T, typename OutT>
-int launch_simple(const PagedAttendParams &p, cudaStream_t st) {
-  launch_pdl(paged_attend_simple_kernel<T, OutT>, dim3(p.max_rows, (p.n_heads + 3) / 4), dim3(128),
-             0, st, p);
   return check_launch("paged_attend");
 }
 
@@ -1105,7 +1265,7 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.o_rs = o_row_stride;
   p.max_rows = max_rows;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 2 * kPaKeys);
+  p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 64);
   p.status = device_status_ptr();
   if (p.status == nullptr) return WATTN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
@@ -1121,7 +1281,7 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   }
   p.count = reinterpret_cast<int *>(workspace);
   p.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + kCounterBytes);
-  if (dtype == WATTN_F32) return launch_simple<float, float>(p, st);
+  if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
   if (dtype == WATTN_F16)
     return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
                                   : launch_stream<__half, __half>(p, dtype, st);
