@@ -519,74 +519,90 @@ class DeviceKvCache:
 # ---------------------------------------------------------------- device-planned paged cache
 # (include/wattn.h, "Device-planned paged cache": the meaning of every array)
 
-# (These run once per layer and step: checks are attribute reads, and what a
-# refusal says is put together only then.)
+# (These calls run once per layer and step: their checks are a few attribute
+# reads a tensor, and what a refusal says is put together only then.)
 
-def _refuse(t, name, expected, device, dense):
+_torch = _int32 = _raw_stream = _current_device = None
+
+
+def _load_torch():
+    global _torch, _int32, _raw_stream, _current_device
+    import torch
+    _torch, _int32 = torch, torch.int32
+    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _device_of(t, name):
+    """The index of a CUDA tensor's device."""
+    if _torch is None:
+        _load_torch()
+    if not getattr(t, "is_cuda", False):
+        raise TypeError(f"{name}: device entry points take CUDA tensors")
+    return t.get_device()
+
+
+def _refuse(t, name, expected, device):
     """Raises what is wrong with tensor ``t``."""
     if not getattr(t, "is_cuda", False):
         raise TypeError(f"{name}: device entry points take CUDA tensors")
     if t.get_device() != device:
         raise WattnError(ERR_INVALID, f"{name} is on {t.device}, not on device {device}")
     raise WattnError(ERR_INVALID, f"{name} is {t.dtype} {tuple(t.shape)} with strides "
-                                  f"{tuple(t.stride())}; expected {expected}, {dense}")
+                                  f"{tuple(t.stride())}; expected {expected}")
 
 
-def _ints(t, shape, name, device):
-    """Address of a contiguous int32 CUDA tensor of ``shape``; None passes."""
+def _ints(t, n, name, device):
+    """Address of a contiguous int32 CUDA tensor of ``n`` elements; None passes."""
     if t is None:
         return None
-    import torch
-    if getattr(t, "dtype", None) is not torch.int32:
+    if getattr(t, "dtype", None) is not _int32:
         raise TypeError(f"{name} must be an int32 tensor, not {getattr(t, 'dtype', type(t))}")
-    if t.shape != shape or not t.is_contiguous() or t.get_device() != device or not t.is_cuda:
-        _refuse(t, name, shape, device, "contiguous")
+    if t.numel() != n or t.get_device() != device or not t.is_contiguous():
+        _refuse(t, name, f"{n} elements, contiguous", device)
     return t.data_ptr()
+
+
+def _mask(t, n_rows, device):
+    """(address, words) of the masks of ``n_rows`` rows; None passes."""
+    if t is None:
+        return None, 0
+    words = t.shape[-1]
+    return _ints(t, n_rows * words, "row_mask", device), words
 
 
 def _table(t, n_seqs, device):
     """(address, row stride, columns) of a block table, whose rows may be strided."""
-    import torch
-    if getattr(t, "dtype", None) is not torch.int32:
+    if getattr(t, "dtype", None) is not _int32:
         raise TypeError(f"block_table must be an int32 tensor, not {getattr(t, 'dtype', type(t))}")
-    if (t.dim() != 2 or t.shape[0] != n_seqs or t.get_device() != device or not t.is_cuda
-            or t.shape[1] > 1 and t.stride(1) != 1):
-        _refuse(t, "block_table", (n_seqs, "max_pages"), device, "dense rows")
+    if t.dim() != 2 or t.shape[0] != n_seqs or t.get_device() != device or t.stride(1) != 1:
+        _refuse(t, "block_table", f"[{n_seqs}][max_pages], dense rows", device)
     n = t.shape[1]
     return t.data_ptr(), t.stride(0) if n_seqs > 1 else n, n
 
 
 def _rows(t, n_rows, width, name, device):
     """(address, row stride) of a 2-D CUDA tensor of dense rows."""
-    if t.shape != (n_rows, width) or t.stride(1) != 1 or t.get_device() != device or not t.is_cuda:
-        _refuse(t, name, (n_rows, width), device, "dense rows")
+    if t.shape != (n_rows, width) or t.stride(1) != 1 or t.get_device() != device:
+        _refuse(t, name, f"[{n_rows}][{width}], dense rows", device)
     return t.data_ptr(), t.stride(0) if n_rows > 1 else width
 
 
 def _pool(pool):
-    """(address, dtype, n_pages, n_layers, n_heads, page_rows) of a page pool."""
-    shape = pool.shape
-    if len(shape) != 6 or shape[2] != 2 or shape[5] != 64 or not pool.is_contiguous() or not pool.is_cuda:
-        _refuse(pool, "pool", "[n_pages][n_layers][2][n_heads][page_rows][64]", pool.get_device(),
-                "contiguous")
-    return pool.data_ptr(), _dt_of(pool), shape[0], shape[1], shape[3], shape[4]
-
-
-def _device_of(t, name):
-    """The index of a CUDA tensor's device."""
-    if not getattr(t, "is_cuda", False):
-        raise TypeError(f"{name}: device entry points take CUDA tensors")
-    return t.get_device()
+    """(device index, (address, dtype, n_pages, n_layers, n_heads, page_rows)) of a page pool."""
+    device, shape = _device_of(pool, "pool"), pool.shape
+    if len(shape) != 6 or shape[2] != 2 or shape[5] != 64 or not pool.is_contiguous():
+        _refuse(pool, "pool", "[n_pages][n_layers][2][n_heads][page_rows][64], contiguous", device)
+    n_pages, n_layers, _, n_heads, page_rows, _ = shape
+    return device, (pool.data_ptr(), _dt_of(pool), n_pages, n_layers, n_heads, page_rows)
 
 
 def _call_on(device, stream, fn, *args):
     """fn(*args, stream) with `device` current; its current stream if none is given."""
-    import torch
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    if device != _current_device():
+        with _torch.cuda.device(device):
             return _call_on(device, stream, fn, *args)
     if stream is None:
-        return fn(*args, torch._C._cuda_getCurrentRawStream(device))
+        return fn(*args, _raw_stream(device))
     return fn(*args, getattr(stream, "cuda_stream", stream))
 
 
@@ -596,32 +612,34 @@ def paged_plan(seq_lens, n_new, block_table, n_held, free_pages, n_free, row_sta
     ``row_mask`` [max_rows][mask_words]) tree masks from the requests'
     lengths. Updates block_table, n_held, free_pages and n_free in place and
     fills row_start, row_pos, row_slot, row_mask and status; all int32."""
-    dev, n, rows = _device_of(seq_lens, "seq_lens"), seq_lens.shape[0], row_pos.shape[0]
+    dev = _device_of(seq_lens, "seq_lens")
+    n, rows, n_pages = seq_lens.numel(), row_pos.numel(), free_pages.numel()
     table, stride, max_pages = _table(block_table, n, dev)
-    words, n_pages = 0 if row_mask is None else row_mask.shape[-1], free_pages.shape[0]
-    _check(_call_on(
-        dev, stream, lib.wattn_paged_plan, _ints(seq_lens, (n,), "seq_lens", dev),
-        _ints(n_new, (n,), "n_new", dev), n, page_rows, n_pages, table, stride, max_pages,
-        _ints(n_held, (n,), "n_held", dev), _ints(free_pages, (n_pages,), "free_pages", dev),
-        _ints(n_free, (1,), "n_free", dev), _ints(parents, (rows,), "parents", dev),
-        _ints(row_start, (n + 1,), "row_start", dev), _ints(row_pos, (rows,), "row_pos", dev),
-        _ints(row_slot, (rows,), "row_slot", dev),
-        _ints(row_mask, (rows, words), "row_mask", dev), words, rows,
-        _ints(status, (1,), "status", dev)), "paged_plan")
+    mask, words = _mask(row_mask, rows, dev)
+    rc = _call_on(
+        dev, stream, lib.wattn_paged_plan, _ints(seq_lens, n, "seq_lens", dev),
+        _ints(n_new, n, "n_new", dev), n, page_rows, n_pages, table, stride, max_pages,
+        _ints(n_held, n, "n_held", dev), _ints(free_pages, n_pages, "free_pages", dev),
+        _ints(n_free, 1, "n_free", dev), _ints(parents, rows, "parents", dev),
+        _ints(row_start, n + 1, "row_start", dev), _ints(row_pos, rows, "row_pos", dev),
+        _ints(row_slot, rows, "row_slot", dev), mask, words, rows, _ints(status, 1, "status", dev))
+    if rc:
+        _check(rc, "paged_plan")
 
 
 def paged_write(pool, layer, row_slot, k_rows, v_rows, *, stream=None) -> None:
     """``wattn_paged_write``: the new rows' K/V ([n_rows][n_heads*64], one row
     stride) into their slots of ``layer``."""
-    p = _pool(pool)
-    dev, n = pool.get_device(), row_slot.shape[0]
+    dev, p = _pool(pool)
+    n = row_slot.numel()
     k, k_rs = _rows(k_rows, n, p[4] * 64, "k_rows", dev)
     v, v_rs = _rows(v_rows, n, p[4] * 64, "v_rows", dev)
     if k_rs != v_rs or k_rows.dtype != v_rows.dtype:
         raise WattnError(ERR_INVALID, "k_rows and v_rows must have one type and one row stride")
-    _check(_call_on(dev, stream, lib.wattn_paged_write, *p, layer,
-                    _ints(row_slot, (n,), "row_slot", dev), n, k, v, _dt_of(k_rows), k_rs),
-           "paged_write")
+    rc = _call_on(dev, stream, lib.wattn_paged_write, *p, layer,
+                  _ints(row_slot, n, "row_slot", dev), n, k, v, _dt_of(k_rows), k_rs)
+    if rc:
+        _check(rc, "paged_write")
 
 
 def paged_attend_workspace_bytes(n_seqs, max_rows, n_heads) -> int:
@@ -634,21 +652,25 @@ def paged_attend(pool, layer, block_table, seq_lens, row_start, q, o, *, row_mas
     requests' pages and, as ``row_mask`` says (None: causally), each other.
     ``workspace``: a zero-filled CUDA tensor of at least
     paged_attend_workspace_bytes() bytes, or None."""
-    p = _pool(pool)
-    dev, n, rows = pool.get_device(), seq_lens.shape[0], q.shape[0]
+    dev, p = _pool(pool)
+    n, rows, width = seq_lens.numel(), q.shape[0], p[4] * 64
     if q.dtype != pool.dtype:
         raise WattnError(ERR_INVALID, f"q is {q.dtype}, the pool {pool.dtype}")
-    qp, q_rs = _rows(q, rows, p[4] * 64, "q", dev)
-    op, o_rs = _rows(o, rows, p[4] * 64, "o", dev)
+    qp, q_rs = _rows(q, rows, width, "q", dev)
+    op, o_rs = _rows(o, rows, width, "o", dev)
     table, stride, max_pages = _table(block_table, n, dev)
-    words = 0 if row_mask is None else row_mask.shape[-1]
-    ws_ptr = _dev(workspace) if workspace is not None else None
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    _check(_call_on(
+    mask, words = _mask(row_mask, rows, dev)
+    ws_ptr = ws_bytes = 0
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            _refuse(workspace, "workspace", "contiguous", dev)
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    rc = _call_on(
         dev, stream, lib.wattn_paged_attend, *p, layer, table, stride, max_pages,
-        _ints(seq_lens, (n,), "seq_lens", dev), _ints(row_start, (n + 1,), "row_start", dev), n,
-        _ints(row_mask, (rows, words), "row_mask", dev), words, qp, q_rs, op, _dt_of(o), o_rs, rows, scale,
-        ws_ptr, ws_bytes), "paged_attend")
+        _ints(seq_lens, n, "seq_lens", dev), _ints(row_start, n + 1, "row_start", dev), n, mask,
+        words, qp, q_rs, op, _dt_of(o), o_rs, rows, scale, ws_ptr, ws_bytes)
+    if rc:
+        _check(rc, "paged_attend")
 
 
 def paged_accept(pool, row_start, row_slot, tokens, picked, seq_lens, n_accepted, path,
@@ -656,12 +678,13 @@ def paged_accept(pool, row_start, row_slot, tokens, picked, seq_lens, n_accepted
     """``wattn_paged_accept``: the longest path of drafts the model agrees
     with: its K/V rows moved together in ``pool``, ``seq_lens`` advanced,
     n_accepted, path and next_token filled; all int32."""
-    p = _pool(pool)
-    dev, n, rows = pool.get_device(), seq_lens.shape[0], row_slot.shape[0]
-    _check(_call_on(
-        dev, stream, lib.wattn_paged_accept, *p, _ints(row_start, (n + 1,), "row_start", dev), n,
-        rows, _ints(parents, (rows,), "parents", dev), _ints(row_slot, (rows,), "row_slot", dev),
-        _ints(tokens, (rows,), "tokens", dev), _ints(picked, (rows,), "picked", dev),
-        _ints(seq_lens, (n,), "seq_lens", dev), _ints(n_accepted, (n,), "n_accepted", dev),
-        _ints(path, (rows,), "path", dev), _ints(next_token, (n,), "next_token", dev)),
-        "paged_accept")
+    dev, p = _pool(pool)
+    n, rows = seq_lens.numel(), row_slot.numel()
+    rc = _call_on(
+        dev, stream, lib.wattn_paged_accept, *p, _ints(row_start, n + 1, "row_start", dev), n,
+        rows, _ints(parents, rows, "parents", dev), _ints(row_slot, rows, "row_slot", dev),
+        _ints(tokens, rows, "tokens", dev), _ints(picked, rows, "picked", dev),
+        _ints(seq_lens, n, "seq_lens", dev), _ints(n_accepted, n, "n_accepted", dev),
+        _ints(path, rows, "path", dev), _ints(next_token, n, "next_token", dev))
+    if rc:
+        _check(rc, "paged_accept")
