@@ -37,7 +37,7 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;            // the portable cluster size
 constexpr int kPlanSeqs = 2048;         // requests whose first rows and lengths a CTA keeps at hand
 constexpr int kPlanParents = 16384;     // parents that a CTA keeps at hand
-constexpr int kPlanRowsPerCta = 1024;   // rows and requests below which another CTA does not pay
+constexpr int kPlanRowsPerCta = 1024;   // rows (a request counts as 4) below which another CTA does not pay
 constexpr int kPlanRowsApart = 16384;   // rows beyond which a launch of their own pays
 
 // What one request asks of the plan: new rows, pages taken and given back.
@@ -60,11 +60,23 @@ WATTN_DEVINL PlanSum warp_scan(PlanSum x, int lane) {
   return x;
 }
 
+// The last of n ascending numbers that is at most x (at[0] <= x): of a row,
+// the request that it belongs to, given the requests' first rows.
+WATTN_DEVINL int last_not_above(const int *at, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 struct PlanSmem {
   PlanSum warp_sums[32];
   PlanSum total;          // of this CTA's requests
   int bad;                // 1: invalid, 2: out of range
   int first[kPlanSeqs + 1], len[kPlanSeqs];
+  int page_from[kPlanThreads], page_at[kPlanThreads];
   int parents[kPlanParents];
 };
 
@@ -115,30 +127,21 @@ WATTN_DEVINL long long cluster_word64(const long long *p, int rank) {
   return (long long)cluster_word(w, rank) | (long long)cluster_word(w + 1, rank) << 32;
 }
 
-// Hands this thread's pages [from, to) to the warp, 32 at a time: f(i, s,
-// rank) for page i of request s, the rank-th after `base` in the order of all.
+// Hands the pages [from, from + count) of each thread's request, all of the
+// CTA's `total`, to its threads: f(i, t, rank) for page i of thread t's
+// request, the rank-th in the order of threads and of pages (at: this
+// thread's first rank).
 template <typename F>
-WATTN_DEVINL void each_page(int s, int from, int to, int base, F f) {
-  const int lane = threadIdx.x & 31;
-  unsigned todo = __ballot_sync(0xffffffffu, from < to);
-  while (todo) {
-    const int src = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const int a = __shfl_sync(0xffffffffu, from, src), b = __shfl_sync(0xffffffffu, to, src);
-    const int at = __shfl_sync(0xffffffffu, base, src), ss = __shfl_sync(0xffffffffu, s, src);
-    for (int i = a + lane; i < b; i += 32) f(i, ss, at + i - a);
+WATTN_DEVINL void each_page(PlanSmem &s, int from, int at, int total, F f) {
+  if (total == 0) return;  // (the same for all threads)
+  __syncthreads();
+  s.page_from[threadIdx.x] = from;
+  s.page_at[threadIdx.x] = at;
+  __syncthreads();
+  for (int g = threadIdx.x; g < total; g += kPlanThreads) {
+    const int t = last_not_above(s.page_at, kPlanThreads, g);
+    f(s.page_from[t] + g - s.page_at[t], t, g);
   }
-}
-
-// The request that packed row r belongs to (first ascending, first[0] <= r <
-// first[n]).
-WATTN_DEVINL int seq_of_row(const int *first, int n, int r) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (first[mid] <= r) lo = mid; else hi = mid;
-  }
-  return lo;
 }
 
 // Position, slot and tree mask of packed row r, of request q whose rows
@@ -199,17 +202,20 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
   const int n_free = *p.n_free;
   __syncthreads();
   // ---- sums and checks
+  // (a CTA with no more requests than threads reads and adds them up once)
+  const bool once = s1 - s0 <= kPlanThreads;
   PlanSum mine = {0, 0, 0};
+  PlanSeq q = {0, 0, 0, 0};
   int bad = n_free < 0 ? 1 : 0;
   for (int b = s0; b < s1; b += kPlanThreads) {
-    const PlanSeq q = plan_seq(p, b + tid, s1);
+    q = plan_seq(p, b + tid, s1);
     if ((q.len | q.fresh | q.held) < 0 || q.held > p.max_pages) bad |= 1;
     else if (q.need > p.max_pages || (p.row_mask != nullptr && q.fresh > (long long)p.mask_words * 32)) bad |= 2;
     mine = mine + plan_sum(q);
   }
   if (bad) atomicOr(&s.bad, bad);
   PlanSum sum;
-  block_scan(mine, s.warp_sums, sum);
+  const PlanSum only = block_scan(mine, s.warp_sums, sum);
   if (tid == 0) s.total = sum;
   PlanSum before = {0, 0, 0}, total = sum;
   if (ctas > 1) {
@@ -241,23 +247,27 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     if (ok) *p.n_free = top - (int)total.take;
   }
   // ---- pages given back
-  PlanSum base = before, chunk;
+  PlanSum base = before, chunk = sum;
   for (int b = s0; b < s1; b += kPlanThreads) {
     const int i = b + tid;
-    const PlanSeq q = plan_seq(p, i, s1);
-    const PlanSum at = base + block_scan(plan_sum(q), s.warp_sums, chunk);
-    base = base + chunk;
-    if (i < s1) p.row_start[i] = ok ? (int)at.rows : 0;
+    PlanSum in = only;  // sums before this thread's request, within the chunk
+    if (!once) {
+      q = plan_seq(p, i, s1);
+      in = block_scan(plan_sum(q), s.warp_sums, chunk);
+    }
+    const int first = (int)(base.rows + in.rows);
+    if (i < s1) p.row_start[i] = ok ? first : 0;
     if (i < s1 && i - s0 < kPlanSeqs) {
-      s.first[i - s0] = (int)at.rows;
+      s.first[i - s0] = first;
       s.len[i - s0] = q.len;
     }
     if (ok)
-      each_page(i, (int)q.need, q.held, (int)at.give, [&](int pi, int seq, int g) {
-        int *e = p.table + seq * p.table_stride + pi;
-        p.free_pages[top - 1 - g] = *e;
+      each_page(s, (int)q.need, (int)in.give, (int)chunk.give, [&](int pi, int t, int g) {
+        int *e = p.table + (b + t) * p.table_stride + pi;
+        p.free_pages[top - 1 - ((int)base.give + g)] = *e;
         *e = -1;
       });
+    base = base + chunk;
   }
   if (tid == 0 && s1 - s0 <= kPlanSeqs) s.first[s1 - s0] = (int)base.rows;
   if (ctas > 1) cluster_sync(); else __syncthreads();  // the stack holds what was given back
@@ -266,13 +276,16 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     base = before;
     for (int b = s0; b < s1; b += kPlanThreads) {
       const int i = b + tid;
-      const PlanSeq q = plan_seq(p, i, s1);
-      const PlanSum at = base + block_scan(plan_sum(q), s.warp_sums, chunk);
-      base = base + chunk;
-      each_page(i, q.held, (int)q.need, (int)at.take, [&](int pi, int seq, int g) {
-        p.table[seq * p.table_stride + pi] = p.free_pages[top - 1 - g];
+      PlanSum in = only;
+      if (!once) {
+        q = plan_seq(p, i, s1);
+        in = block_scan(plan_sum(q), s.warp_sums, chunk);
+      }
+      each_page(s, q.held, (int)in.take, (int)chunk.take, [&](int pi, int t, int g) {
+        p.table[(b + t) * p.table_stride + pi] = p.free_pages[top - 1 - ((int)base.take + g)];
       });
       if (i < s1 && q.held != (int)q.need) p.n_held[i] = (int)q.need;
+      base = base + chunk;
     }
   }
   // ---- rows: here, or (p.rows_apart) by a kernel of the whole GPU
@@ -285,9 +298,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
   __syncthreads();  // the table has its new pages
   for (int i = tid; i < n_rows; i += kPlanThreads) {
     const int r = row0 + i;
-    const int q = near ? seq_of_row(s.first, s1 - s0, r) : seq_of_row(p.row_start + s0, s1 - s0, r);
-    const int first = near ? s.first[q] : p.row_start[s0 + q];
-    plan_row(p, r, s0 + q, first, near ? s.len[q] : p.seq_lens[s0 + q],
+    const int k = near ? last_not_above(s.first, s1 - s0, r) : last_not_above(p.row_start + s0, s1 - s0, r);
+    const int first = near ? s.first[k] : p.row_start[s0 + k];
+    plan_row(p, r, s0 + k, first, near ? s.len[k] : p.seq_lens[s0 + k],
              near_parents ? s.parents + (first - row0) : p.parents + first);
   }
   for (long long r = (ok ? total.rows : 0) + (long long)rank * kPlanThreads + tid; r < p.max_rows;
@@ -304,7 +317,7 @@ __global__ void __launch_bounds__(256) paged_plan_rows_kernel(const PlanParams p
     plan_padding(p, r);
     return;
   }
-  const int q = seq_of_row(p.row_start, p.n_seqs, (int)r);
+  const int q = last_not_above(p.row_start, p.n_seqs, (int)r);
   const int first = p.row_start[q];
   plan_row(p, (int)r, q, first, p.seq_lens[q], p.parents + first);
 }
@@ -608,7 +621,7 @@ int wattn_paged_plan(const int *seq_lens, const int *n_new, int n_seqs, int page
   // worth another launch (230,000 rows: 78 us by eight CTAs).
   PlanParams q = p;
   q.rows_apart = max_rows > kPlanRowsApart;
-  const int64_t work = n_seqs + (q.rows_apart ? 0 : (int64_t)max_rows);
+  const int64_t work = 4LL * n_seqs + (q.rows_apart ? max_rows / page_rows : (int64_t)max_rows);
   const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(kPlanCtas, work / kPlanRowsPerCta));
   launch_pdl_cluster(paged_plan_kernel, dim3(grid), dim3(kPlanThreads), smem, st, grid, q);
   if (q.rows_apart) {
