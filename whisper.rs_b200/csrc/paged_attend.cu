@@ -15,42 +15,16 @@
 // item's keys. The parts of a cut item are merged by log-sum-exp in the order
 // of the keys, by its CTA or, where it spans several, by the last of them:
 // same inputs, same bits.
-#include <limits.h>
-
 #include <algorithm>
 
-#include "wattn_common.cuh"
-#include "wattn_internal.h"
+#include "paged_attend.cuh"
 
 namespace wattn {
 
 namespace {
 
-struct PagedAttendParams {
-  const void *pool;
-  int n_pages, n_layers, n_heads, page_rows, layer;
-  const int *table;
-  int64_t table_stride;
-  int max_pages;
-  const int *seq_lens, *row_start;
-  int n_seqs;
-  const int *row_mask;
-  int mask_words, mask_bits;
-  const void *q;
-  void *o;
-  int64_t q_rs, o_rs;
-  int max_rows;
-  float scale_log2;
-  int cap;       // positions that the table can hold
-  int box_rows;  // rows of a TMA box of whole stages
-  float *part;   // partials of cut items, two per warp and two per CTA
-  int *count;    // finished CTAs of the item that each CTA starts and another ends
-  int *status;
-};
-
 // ---------------------------------------------------------------- shares of the work
 
-constexpr int kPaTail = 16;       // rows of a tail box: the pool's unit of page rows
 constexpr int kPaStageBytes = 8192;  // keys, then values
 constexpr int kPaStages = 3;      // stages of a warp's ring
 constexpr int kPaWarps = 4;       // compute warps (one warpgroup), and as many load warps
@@ -60,191 +34,44 @@ constexpr int kPaCtasPerSm = 2;
 // warpgroups' split (whose sum may not exceed twice the launch's).
 constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
 static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
-constexpr int kPaStageUnits = 2, kPaWideUnits = 3, kPaItemUnits = 2;
-constexpr int kPaMinUnits = 8;    // units of a share below which fewer warps work
+// New rows of a request, averaged over the row buffer (the counts themselves
+// are on the device), from which the wide kernel is the faster one.
+constexpr int kPaWideRows = 20;
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
 
-// By type of the pool: keys of a stage (8 KB of keys and values), rows of a
-// row tile.
+// A stage is 8 KB of keys and values. Units: measured, two tiles of 16 rows
+// cost half as much again as one.
+struct PaShape {
+  static constexpr int kShares = kPaWarps, kThreads = kPaThreads;
+  static constexpr int kStageUnits = 2, kWideUnits = 3, kItemUnits = 2;
+  static constexpr int kMinUnits = 8;  // units of a share below which fewer warps work
+};
 template <typename T> struct PaType;
-template <> struct PaType<__half> {
+template <> struct PaType<__half> : PaShape {
   static constexpr int kKeys = 32, kRows = 32;
   static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
   static constexpr bool kResidual = false;  // f16 weights: 2^-11 each, within the 2e-3 bar
 };
-template <> struct PaType<__nv_bfloat16> {
+template <> struct PaType<__nv_bfloat16> : PaShape {
   static constexpr int kKeys = 32, kRows = 32;
   static constexpr uint32_t kOne = 0x3f80u, kInf = 0x7f80u;
   static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
 };
-template <> struct PaType<float> {
+template <> struct PaType<float> : PaShape {
   static constexpr int kKeys = 16, kRows = 16;
 };
 
-// One request as the kernel sees it. One whose arrays are out of range has
-// no rows here (and is reported).
-struct PaSeq {
-  int first, n;   // packed rows
-  int len;        // cached positions, all seen
-};
-
-WATTN_DEVINL PaSeq pa_seq(const PagedAttendParams &p, int s, bool *bad) {
-  const int a = p.row_start[s], b = p.row_start[s + 1], len = p.seq_lens[s];
-  const bool ok = a >= 0 && b >= a && b <= p.max_rows && len >= 0 && len <= p.cap && b - a <= p.cap - len;
-  if (bad != nullptr) *bad = !ok;
-  return {a, ok ? b - a : 0, len};
-}
-// Positions that rows of tile rt may see.
-template <typename T> WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return q.len + min(q.n, p.row_mask != nullptr ? p.mask_bits : PaType<T>::kRows * (rt + 1));
-}
-template <typename T> WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return (pa_end<T>(p, q, rt) + PaType<T>::kKeys - 1) / PaType<T>::kKeys;
-}
-// Units that a stage of row tile rt costs: two tiles of 16 rows cost more
-// than one; kPaItemUnits are what an item costs besides its stages.
-template <typename T> WATTN_DEVINL int pa_weight(const PaSeq &q, int rt) {
-  return PaType<T>::kRows > 16 && q.n - rt * PaType<T>::kRows > 16 ? kPaWideUnits : kPaStageUnits;
-}
-template <typename T> WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
-  return pa_stages<T>(p, q, rt) * pa_weight<T>(q, rt) + kPaItemUnits;
-}
-// Units of one head of a request: its full row tiles, then the last.
-template <typename T> WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
-  if (q.n <= PaType<T>::kRows) return q.n > 0 ? pa_units<T>(p, q, 0) : 0;
-  const long long full = (q.n - 1) / PaType<T>::kRows;
-  long long stages = full * pa_stages<T>(p, q, 0);
-  if (p.row_mask == nullptr) stages += full * (full - 1) / 2;  // one more from tile to tile
-  return stages * pa_weight<T>(q, 0) + full * kPaItemUnits + pa_units<T>(p, q, (int)full);
-}
-
-// `total` units (below 2^31) in `parts` shares, in order: the first `more` of
-// them have size + 1 units, the others size.
-struct PaShares {
-  int size, parts, more;
-};
-WATTN_DEVINL PaShares pa_shares(int total, int max_parts) {
-  PaShares s;
-  s.parts = max(1, min(max_parts, total / kPaMinUnits));
-  s.size = total / s.parts;
-  s.more = total - s.size * s.parts;
-  return s;
-}
-WATTN_DEVINL int pa_share_begin(const PaShares &s, int c) { return c * s.size + min(c, s.more); }
-// The share that unit u belongs to.
-WATTN_DEVINL int pa_owner(const PaShares &s, int u) {
-  const int big = s.more * (s.size + 1);
-  return u < big ? u / (s.size + 1) : s.more + (u - big) / s.size;
-}
-
-// Where a share [lo, hi) begins: its first item (s, head, rt) starts at unit
-// `at` <= lo.
-struct PaStart {
-  PaSeq q;
-  int s, head, rt;
-  int at, lo, hi;
-};
-
-// An item of a warp's share, as the loads announce it to the products.
-struct PaItem {
-  int row0, nr;      // packed rows of the tile
-  int row;           // the tile's first row in the request
-  int len, end;      // cached positions, positions that some row may see
-  int head;
-  int from, to, stages, weight;  // stages of this share, of the item; units of one
-  int at;            // the item's first unit
-};
-
+template <typename T>
 struct PaSmem {
   uint8_t kv[kPaWarps][kPaStages][kPaStageBytes];
   uint64_t full[kPaWarps][kPaStages], empty[kPaWarps][kPaStages];
   PaItem queue[kPaWarps][kPaQueue];
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
-  int run_first[kPaWarps], run_at[kPaWarps];
-  long long warp_sums[2 * kPaWarps];
-  PaShares shares;
-  int total;
+  PaFind<PaType<T>> find;
   int merge_first[2 * kPaWarps], merge_last[2 * kPaWarps];  // shares to merge, per cut item
   int abort;
 };
-
-// The shares. All threads of the CTA add up the units of a run of requests
-// each; the sums are scanned, and for each share of the CTA the run that
-// holds its first unit is noted.
-template <typename T> WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaSmem &s) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.n_seqs + kPaThreads - 1) / kPaThreads;
-  const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
-  long long mine = 0;
-#pragma unroll 4
-  for (int i = s0; i < s1; ++i) {
-    bool bad;
-    const PaSeq q = pa_seq(p, i, &bad);
-    if (bad) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
-    mine += pa_head_units<T>(p, q) * p.n_heads;
-  }
-  long long inc = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += y;
-  }
-  if (lane == 31) s.warp_sums[warp] = inc;
-  __syncthreads();
-  long long before = inc - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < 2 * kPaWarps; ++w) {
-    if (w < warp) before += s.warp_sums[w];
-    total += s.warp_sums[w];
-  }
-  if (total > INT_MAX) {  // more than a call may ask for
-    if (tid == 0) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
-    total = 0;
-  }
-  const PaShares shares = pa_shares((int)total, gridDim.x * kPaWarps);
-  if (tid == 0) {
-    s.shares = shares;
-    s.total = (int)total;
-  }
-  const int c0 = blockIdx.x * kPaWarps;
-#pragma unroll
-  for (int k = 0; k < kPaWarps; ++k) {
-    const int lo = pa_share_begin(shares, c0 + k);
-    if (c0 + k < shares.parts && before <= lo && lo < before + mine) {
-      s.run_first[k] = s0;
-      s.run_at[k] = (int)before;
-    }
-  }
-  __syncthreads();
-}
-
-// Share blockIdx.x * kPaWarps + k: walks to its first item.
-template <typename T> WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaSmem &s, int k) {
-  PaStart w;
-  w.lo = w.hi = 0;
-  const int c = blockIdx.x * kPaWarps + k;
-  if (c >= s.shares.parts || s.total == 0) return w;
-  w.lo = pa_share_begin(s.shares, c);
-  w.hi = pa_share_begin(s.shares, c + 1);
-  w.at = s.run_at[k];
-  for (w.s = s.run_first[k];; ++w.s) {
-    w.q = pa_seq(p, w.s, nullptr);
-    const int u = (int)pa_head_units<T>(p, w.q);
-    if (w.lo - w.at < (long long)u * p.n_heads) {
-      w.head = (w.lo - w.at) / u;
-      w.at += w.head * u;
-      break;
-    }
-    w.at += u * p.n_heads;
-  }
-  for (w.rt = 0;; ++w.rt) {
-    const int u = pa_units<T>(p, w.q, w.rt);
-    if (w.lo - w.at < u) break;
-    w.at += u;
-  }
-  return w;
-}
 
 // ---------------------------------------------------------------- 16-bit pools
 
@@ -288,24 +115,6 @@ template <int OFF> WATTN_DEVINL void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) 
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr), "n"(OFF)
                : "memory");
-}
-
-// Which of the 32 positions from seq_lens + off on row i sees, as bits: all
-// of the cached ones (off < 0), then the row's mask, or the rows up to itself;
-// `left` positions of them exist.
-WATTN_DEVINL uint32_t pa_mask_word(const PagedAttendParams &p, int packed, int i, int w) {
-  if (w < 0) return 0xffffffffu;
-  if (p.row_mask == nullptr) {
-    const int up = i + 1 - 32 * w;
-    return up >= 32 ? 0xffffffffu : up <= 0 ? 0u : (1u << up) - 1u;
-  }
-  return w < p.mask_words ? (uint32_t)p.row_mask[(int64_t)packed * p.mask_words + w] : 0u;
-}
-WATTN_DEVINL uint32_t pa_visible(const PagedAttendParams &p, int packed, int i, int off, int left) {
-  const int w = off >> 5;
-  const uint32_t bits = __funnelshift_r(pa_mask_word(p, packed, i, w),
-                                        pa_mask_word(p, packed, i, w + 1), off & 31);
-  return left >= 32 ? bits : bits & ((1u << left) - 1u);
 }
 
 // The two halves of a word that are infinite or NaN, as 0xffff each.
@@ -405,55 +214,17 @@ WATTN_DEVINL void pa_output(const PagedAttendParams &p, const PaTile &a, int row
   }
 }
 
-// A load warp's walk over its share.
-struct PaLoads {
-  PaStart w;
-  int units, stages, weight;  // of the current item
-  int t, to, end;        // its next stage, the share's last, its positions
-  int page, in_page;     // table index and row of the next box
-  int base, entry;       // lane i holds table entry base + i of the request
-};
-
-// The current item's stages that this share holds (a stage belongs to the
-// share that holds its first unit), and where their keys are. False if none.
-template <typename T> WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
-  const PaStart &w = ld.w;
-  ld.units = pa_units<T>(p, w.q, w.rt);
-  ld.stages = pa_stages<T>(p, w.q, w.rt);
-  ld.weight = pa_weight<T>(w.q, w.rt);
-  const int d = w.lo - w.at, e = w.hi - w.at;
-  ld.t = d <= 0 ? 0 : (d + ld.weight - 1) / ld.weight;
-  ld.to = e >= ld.units ? ld.stages : min(ld.stages, (e + ld.weight - 1) / ld.weight);
-  ld.end = pa_end<T>(p, w.q, w.rt);
-  ld.page = ld.t * PaType<T>::kKeys / p.page_rows;
-  ld.in_page = ld.t * PaType<T>::kKeys - ld.page * p.page_rows;
-  return ld.t < ld.to;
-}
-
 // Announces the current item to the compute warp.
 template <typename T>
-WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaItem &it, const PaLoads &ld, int lane) {
-  const PaStart &w = ld.w;
-  const int row = w.rt * PaType<T>::kRows, row0 = w.q.first + row, nr = min(PaType<T>::kRows, w.q.n - row);
-  if (lane == 0) {
-    it.row0 = row0;
-    it.nr = nr;
-    it.row = row;
-    it.len = w.q.len;
-    it.end = ld.end;
-    it.head = w.head;
-    it.from = ld.t;
-    it.to = ld.to;
-    it.stages = ld.stages;
-    it.weight = ld.weight;
-    it.at = w.at;
-  }
-  if (lane < nr) {  // its query rows and masks will be wanted soon
+WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaItem &to, const PaLoads &ld, int lane) {
+  const PaItem it = pa_item_of<PaType<T>>(ld);
+  if (lane == 0) to = it;
+  if (lane < it.nr) {  // its query rows and masks will be wanted soon
     asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const T *>(p.q) +
-                                                  (int64_t)(row0 + lane) * p.q_rs + w.head * 64));
+                                                  (int64_t)(it.row0 + lane) * p.q_rs + it.head * 64));
     if (p.row_mask != nullptr)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(p.row_mask +
-                                                    (int64_t)(row0 + lane) * p.mask_words));
+                                                    (int64_t)(it.row0 + lane) * p.mask_words));
   }
 }
 
@@ -461,39 +232,36 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaItem &it, const PaLo
 // share's items, each announced before its first stage; an item without rows
 // ends the share.
 template <typename T>
-WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorMap &map,
+WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem<T> &s, const CUtensorMap &map,
                           const CUtensorMap &map_tail, int k, int lane) {
+  using C = PaType<T>;
   PaLoads ld;
-  ld.w = pa_start<T>(p, s, k);
-  ld.base = INT_MIN / 2;
-  ld.entry = 0;
+  ld.w = pa_start<C>(p, s.find, k);
   PaStart &w = ld.w;
+  int base = INT_MIN / 2, entry = 0;  // lane i holds table entry base + i of the request
   int slot = 0;
   uint32_t phase = 1;  // (a wait for the phase before the first passes)
-  uint32_t items = 0;
-  bool fresh = w.lo < w.hi && pa_enter<T>(p, ld);  // an item not yet announced
-  if (w.lo >= w.hi) ld.t = ld.to = ld.units = 0;
+  uint32_t items = 0, issued = 0;
+  bool fresh = false;  // an item not yet announced
+  const bool some = w.lo < w.hi;
+  if (some) fresh = pa_enter<C>(p, ld);
 #pragma unroll 1
   for (;;) {
-    bool more = w.lo < w.hi;
-    while (more && ld.t >= ld.to) {  // on to the next item of the share
-      w.at += ld.units;
-      if (w.at >= w.hi) {
-        more = false;
-        break;
-      }
-      if (++w.rt * PaType<T>::kRows >= w.q.n) {
-        w.rt = 0;
-        if (++w.head == p.n_heads) {
-          w.head = 0;
-          do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
-          ld.base = INT_MIN / 2;  // another request's table
-        }
-      }
-      fresh = pa_enter<T>(p, ld);
-    }
+    bool moved = false;
+    const bool more = some && pa_advance<C>(p, ld, fresh, moved);
+    if (moved) base = INT_MIN / 2;  // another request's table
     const bool ok = mbar_wait(&s.empty[k][slot], phase, &s.abort, p.status, (4 << 24) | (3 << 16));
-    if (!__all_sync(0xffffffffu, ok)) return;
+    if (!__all_sync(0xffffffffu, ok)) {
+      // winding down: the copies in flight land before the block leaves
+      volatile int no_abort = 0;
+      for (int st = 0; st < kPaStages; ++st)
+        if (st < (int)min(issued, (uint32_t)kPaStages)) {
+          const uint32_t c = issued - 1 - st;
+          mbar_wait(&s.full[k][c % kPaStages], (c / kPaStages) & 1, &no_abort, p.status,
+                    (4 << 24) | (4 << 16));
+        }
+      return;
+    }
     uint64_t *bar = &s.full[k][slot];
     PaItem &it = s.queue[k][items % kPaQueue];
     if (!more) {
@@ -515,11 +283,11 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
     const int boxes = rows > step && step < PaType<T>::kKeys ? 2 : 1;  // a step is a stage, or half of one
 #pragma unroll 1
     for (int b = 0; b < boxes; ++b) {
-      if ((unsigned)(ld.page - ld.base) >= 32u) {
-        ld.base = ld.page;
-        ld.entry = ld.base + lane < p.max_pages ? p.table[w.s * p.table_stride + ld.base + lane] : 0;
+      if ((unsigned)(ld.page - base) >= 32u) {
+        base = ld.page;
+        entry = base + lane < p.max_pages ? p.table[w.s * p.table_stride + base + lane] : 0;
       }
-      int page = __shfl_sync(0xffffffffu, ld.entry, ld.page - ld.base);
+      int page = __shfl_sync(0xffffffffu, entry, ld.page - base);
       if (lane == 0) {
         if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 4 * 32 * sizeof(T));  // (releases the announcement too)
         if ((unsigned)page >= (unsigned)p.n_pages) {
@@ -545,6 +313,7 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
       }
     }
     ++ld.t;
+    ++issued;
     if (++slot == kPaStages) {
       slot = 0;
       phase ^= 1;
@@ -559,7 +328,7 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem &s, const CUtensorM
 // both MT is 14 % slower over single rows, its branches being predicated
 // products; one more for few rows costs more instruction fetches than it saves.)
 template <typename T, typename OutT, int MT>
-WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem &s, const PaItem &it, uint32_t &pos,
+WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem &it, uint32_t &pos,
                           int warp, int lane) {
   const int g = lane >> 2, t4 = lane & 3;
   const bool few = MT == 1 && it.nr <= 8;
@@ -854,7 +623,7 @@ WATTN_DEVINL float4 pa_lds(uint32_t addr) {
 // it, and chosen so that every lane reads 16 bytes and no bank meets twice:
 // K: step (blk, j, pair) takes dims 32 blk + 8 t4 + 4 j + 2 pair (+ 1);
 // V: column g of tile (j, e) is dim 32 (g >> 2) + 4 ((g & 3) + 4 j) + e.
-WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem &s, const PaItem &it, uint32_t &pos,
+WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, const PaItem &it, uint32_t &pos,
                               int warp, int lane) {
   constexpr int kKeys = PaType<float>::kKeys;
   const int g = lane >> 2, t4 = lane & 3;
@@ -1049,7 +818,7 @@ WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c
 // done, an item per warp: the CTA's parts of an item are merged, and where
 // several CTAs have parts the last of them to arrive merges theirs.
 template <typename T, typename OutT>
-WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int lane) {
+WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, int lane) {
   const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps, ctas = gridDim.x * kPaWarps;
   pa_sync();
   if (tid < 2 * kPaWarps) {
@@ -1059,8 +828,8 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem &s, int warp, int
     for (int i = 0; i < tid; ++i)
       if (s.cut[i >> 1][i & 1].stages > 0 && s.cut[i >> 1][i & 1].at == it.at) fresh = false;
     if (fresh) {
-      w0 = pa_owner(s.shares, it.at);
-      w1 = pa_owner(s.shares, it.at + (it.stages - 1) * it.weight);
+      w0 = pa_owner(s.find.shares, it.at);
+      w1 = pa_owner(s.find.shares, it.at + (it.stages - 1) * it.weight);
     }
     s.merge_first[tid] = w0;
     s.merge_last[tid] = w1;
@@ -1114,7 +883,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
                                const __grid_constant__ CUtensorMap map_tail,
                                const PagedAttendParams p) {
   extern __shared__ uint8_t pa_smem_raw[];
-  PaSmem &s = *reinterpret_cast<PaSmem *>(
+  PaSmem<T> &s = *reinterpret_cast<PaSmem<T> *>(
       (reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (lane == 0 && warp < kPaWarps) {
@@ -1128,7 +897,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  pa_find_shares<T>(p, s);
+  pa_find_shares<PaType<T>>(p, s.find);
   if (warp >= kPaWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaLoadRegs));
     pa_load<T>(p, s, map, map_tail, warp - kPaWarps, lane);
@@ -1151,16 +920,20 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   }
 }
 
-int pa_grid() {
+// SMs of the current device.
+int pa_sms() {
   static int sms[64] = {0};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   if (sms[dev] == 0) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-  return sms[dev] * kPaCtasPerSm;
+  return sms[dev];
 }
 
-size_t pa_workspace(int grid) {
-  return kCounterBytes + (size_t)grid * (kPaWarps + 1) * 4 * kPaTileFloats * sizeof(float);
+// Workspace of either kernel.
+size_t pa_workspace(int n_sm) {
+  const size_t narrow = kCounterBytes + (size_t)n_sm * kPaCtasPerSm * (kPaWarps + 1) * 4 * kPaTileFloats *
+                                            sizeof(float);
+  return std::max(narrow, paged_attend_wide_workspace(n_sm));
 }
 
 template <typename T, typename OutT>
@@ -1183,7 +956,7 @@ int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
   else
     map = map_tail;  // not used
   if (rc != WATTN_OK) return rc;
-  constexpr int smem = (int)sizeof(PaSmem) + 1024;
+  constexpr int smem = (int)sizeof(PaSmem<T>) + 1024;
   auto kern = paged_attend_stream_kernel<T, OutT>;
   // Once per process and type: the warpgroups' register split counts on what
   // the kernel is launched with (with fewer it would wait for ever).
@@ -1192,10 +965,10 @@ int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
     return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
   }();
   if (regs != kPaRegs)
-    return set_error(WATTN_ERR_CUDA, "paged_attend: built for %d registers a thread, not %d", regs, kPaRegs);
+    return set_error(WATTN_ERR_CUDA, "paged_attend: built for %d registers a thread, not %d", kPaRegs, regs);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_launch("cudaFuncSetAttribute(paged_attend)");
-  launch_pdl(kern, dim3(pa_grid()), dim3(kPaThreads), smem, st, map, map_tail, p);
+  launch_pdl(kern, dim3(p.n_sm * kPaCtasPerSm), dim3(kPaThreads), smem, st, map, map_tail, p);
   return check_launch("paged_attend");
 }
 
@@ -1208,7 +981,7 @@ extern "C" {
 
 size_t wattn_paged_attend_workspace_bytes(int n_seqs, int max_rows, int n_heads) {
   if (n_seqs <= 0 || max_rows <= 0 || n_heads <= 0) return 0;
-  return pa_workspace(pa_grid());
+  return pa_workspace(pa_sms());
 }
 
 int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, int n_heads,
@@ -1269,7 +1042,8 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.status = device_status_ptr();
   if (p.status == nullptr) return WATTN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
-  const size_t need = pa_workspace(pa_grid());
+  p.n_sm = pa_sms();
+  const size_t need = pa_workspace(p.n_sm);
   if (workspace == nullptr) {
     workspace = thread_workspace(need, st);
     if (workspace == nullptr) return set_error(WATTN_ERR_NOMEM, "paged_attend: workspace allocation failed");
@@ -1282,6 +1056,7 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.count = reinterpret_cast<int *>(workspace);
   p.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + kCounterBytes);
   if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
+  if (max_rows >= (int64_t)kPaWideRows * n_seqs) return launch_paged_attend_wide(p, dtype, out_dtype, st);
   if (dtype == WATTN_F16)
     return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
                                   : launch_stream<__half, __half>(p, dtype, st);

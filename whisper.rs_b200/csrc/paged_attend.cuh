@@ -1,0 +1,289 @@
+// paged_attend.cuh -- what the attention kernels over a device-planned paged
+// cache share (paged_attend.cu, paged_attend_wide.cu): which rows see what,
+// how the work is shared out, and the walk over a share.
+//
+// An item is one (request, head, tile of rows), a stage some keys of it. Each
+// kernel's configuration C gives kKeys of a stage, kRows of a row tile, kShares
+// per CTA, kThreads that share the work out, and the units that a stage, a
+// stage of more than 16 rows and an item besides its stages count for.
+#pragma once
+
+#include <limits.h>
+
+#include "wattn_common.cuh"
+#include "wattn_internal.h"
+
+namespace wattn {
+
+struct PagedAttendParams {
+  const void *pool;
+  int n_pages, n_layers, n_heads, page_rows, layer;
+  const int *table;
+  int64_t table_stride;
+  int max_pages;
+  const int *seq_lens, *row_start;
+  int n_seqs;
+  const int *row_mask;
+  int mask_words, mask_bits;
+  const void *q;
+  void *o;
+  int64_t q_rs, o_rs;
+  int max_rows;
+  float scale_log2;
+  int cap;       // positions that the table can hold
+  int box_rows;  // rows of a TMA box of whole stages
+  float *part;   // partials of cut items
+  int *count;    // finished CTAs of the item that each CTA starts and another ends
+  int *status;
+  int n_sm;
+};
+
+constexpr int kPaTail = 16;  // rows of a tail box: the pool's unit of page rows
+
+// One request as the kernel sees it. One whose arrays are out of range has
+// no rows here (and is reported).
+struct PaSeq {
+  int first, n;   // packed rows
+  int len;        // cached positions, all seen
+};
+
+WATTN_DEVINL PaSeq pa_seq(const PagedAttendParams &p, int s, bool *bad) {
+  const int a = p.row_start[s], b = p.row_start[s + 1], len = p.seq_lens[s];
+  const bool ok = a >= 0 && b >= a && b <= p.max_rows && len >= 0 && len <= p.cap && b - a <= p.cap - len;
+  if (bad != nullptr) *bad = !ok;
+  return {a, ok ? b - a : 0, len};
+}
+// Positions that rows of tile rt may see.
+template <typename C> WATTN_DEVINL int pa_end(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return q.len + min(q.n, p.row_mask != nullptr ? p.mask_bits : C::kRows * (rt + 1));
+}
+template <typename C> WATTN_DEVINL int pa_stages(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return (pa_end<C>(p, q, rt) + C::kKeys - 1) / C::kKeys;
+}
+// Units that a stage of row tile rt costs: two tiles of 16 rows cost more
+// than one; C::kItemUnits are what an item costs besides its stages.
+template <typename C> WATTN_DEVINL int pa_weight(const PaSeq &q, int rt) {
+  return C::kRows > 16 && q.n - rt * C::kRows > 16 ? C::kWideUnits : C::kStageUnits;
+}
+template <typename C> WATTN_DEVINL int pa_units(const PagedAttendParams &p, const PaSeq &q, int rt) {
+  return pa_stages<C>(p, q, rt) * pa_weight<C>(q, rt) + C::kItemUnits;
+}
+// Units of one head of a request: its full row tiles, then the last.
+template <typename C> WATTN_DEVINL long long pa_head_units(const PagedAttendParams &p, const PaSeq &q) {
+  if (q.n <= C::kRows) return q.n > 0 ? pa_units<C>(p, q, 0) : 0;
+  const long long full = (q.n - 1) / C::kRows;
+  long long stages = full * pa_stages<C>(p, q, 0);
+  if (p.row_mask == nullptr) stages += full * (full - 1) / 2;  // one more from tile to tile
+  return stages * pa_weight<C>(q, 0) + full * C::kItemUnits + pa_units<C>(p, q, (int)full);
+}
+
+// `total` units (below 2^31) in `parts` shares, in order: the first `more` of
+// them have size + 1 units, the others size.
+struct PaShares {
+  int size, parts, more;
+};
+template <typename C> WATTN_DEVINL PaShares pa_shares(int total, int max_parts) {
+  PaShares s;
+  s.parts = max(1, min(max_parts, total / C::kMinUnits));
+  s.size = total / s.parts;
+  s.more = total - s.size * s.parts;
+  return s;
+}
+WATTN_DEVINL int pa_share_begin(const PaShares &s, int c) { return c * s.size + min(c, s.more); }
+// The share that unit u belongs to.
+WATTN_DEVINL int pa_owner(const PaShares &s, int u) {
+  const int big = s.more * (s.size + 1);
+  return u < big ? u / (s.size + 1) : s.more + (u - big) / s.size;
+}
+
+// Where a share [lo, hi) begins: its first item (s, head, rt) starts at unit
+// `at` <= lo.
+struct PaStart {
+  PaSeq q;
+  int s, head, rt;
+  int at, lo, hi;
+};
+
+// An item of a warp's share, as the loads announce it to the products.
+struct PaItem {
+  int row0, nr;      // packed rows of the tile
+  int row;           // the tile's first row in the request
+  int len, end;      // cached positions, positions that some row may see
+  int head;
+  int from, to, stages, weight;  // stages of this share, of the item; units of one
+  int at;            // the item's first unit
+};
+
+// What finding the shares leaves behind (shared memory).
+template <typename C> struct PaFind {
+  int run_first[C::kShares], run_at[C::kShares];
+  long long warp_sums[C::kThreads / 32];
+  PaShares shares;
+  int total;
+};
+
+// The shares. All threads of the CTA add up the units of a run of requests
+// each; the sums are scanned, and for each share of the CTA the run that
+// holds its first unit is noted.
+template <typename C> WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaFind<C> &s) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
+  const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
+  long long mine = 0;
+#pragma unroll 4
+  for (int i = s0; i < s1; ++i) {
+    bool bad;
+    const PaSeq q = pa_seq(p, i, &bad);
+    if (bad) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
+    mine += pa_head_units<C>(p, q) * p.n_heads;
+  }
+  long long inc = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += y;
+  }
+  if (lane == 31) s.warp_sums[warp] = inc;
+  __syncthreads();
+  long long before = inc - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < C::kThreads / 32; ++w) {
+    if (w < warp) before += s.warp_sums[w];
+    total += s.warp_sums[w];
+  }
+  if (total > INT_MAX) {  // more than a call may ask for
+    if (tid == 0) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
+    total = 0;
+  }
+  const PaShares shares = pa_shares<C>((int)total, gridDim.x * C::kShares);
+  if (tid == 0) {
+    s.shares = shares;
+    s.total = (int)total;
+  }
+  const int c0 = blockIdx.x * C::kShares;
+#pragma unroll
+  for (int k = 0; k < C::kShares; ++k) {
+    const int lo = pa_share_begin(shares, c0 + k);
+    if (c0 + k < shares.parts && before <= lo && lo < before + mine) {
+      s.run_first[k] = s0;
+      s.run_at[k] = (int)before;
+    }
+  }
+  __syncthreads();
+}
+
+// Share blockIdx.x * C::kShares + k: walks to its first item.
+template <typename C> WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, const PaFind<C> &s, int k) {
+  PaStart w;
+  w.lo = w.hi = 0;
+  const int c = blockIdx.x * C::kShares + k;
+  if (c >= s.shares.parts || s.total == 0) return w;
+  w.lo = pa_share_begin(s.shares, c);
+  w.hi = pa_share_begin(s.shares, c + 1);
+  w.at = s.run_at[k];
+  for (w.s = s.run_first[k];; ++w.s) {
+    w.q = pa_seq(p, w.s, nullptr);
+    const int u = (int)pa_head_units<C>(p, w.q);
+    if (w.lo - w.at < (long long)u * p.n_heads) {
+      w.head = (w.lo - w.at) / u;
+      w.at += w.head * u;
+      break;
+    }
+    w.at += u * p.n_heads;
+  }
+  for (w.rt = 0;; ++w.rt) {
+    const int u = pa_units<C>(p, w.q, w.rt);
+    if (w.lo - w.at < u) break;
+    w.at += u;
+  }
+  return w;
+}
+
+// Which of the 32 positions from seq_lens + off on row i sees, as bits: all
+// of the cached ones (off < 0), then the row's mask, or the rows up to itself;
+// `left` positions of them exist.
+WATTN_DEVINL uint32_t pa_mask_word(const PagedAttendParams &p, int packed, int i, int w) {
+  if (w < 0) return 0xffffffffu;
+  if (p.row_mask == nullptr) {
+    const int up = i + 1 - 32 * w;
+    return up >= 32 ? 0xffffffffu : up <= 0 ? 0u : (1u << up) - 1u;
+  }
+  return w < p.mask_words ? (uint32_t)p.row_mask[(int64_t)packed * p.mask_words + w] : 0u;
+}
+WATTN_DEVINL uint32_t pa_visible(const PagedAttendParams &p, int packed, int i, int off, int left) {
+  const int w = off >> 5;
+  const uint32_t bits = __funnelshift_r(pa_mask_word(p, packed, i, w),
+                                        pa_mask_word(p, packed, i, w + 1), off & 31);
+  return left >= 32 ? bits : bits & ((1u << left) - 1u);
+}
+
+// A walk over a share.
+struct PaLoads {
+  PaStart w;
+  int units, stages, weight;  // of the current item
+  int t, to, end;        // its next stage, the share's last, its positions
+  int page, in_page;     // table index and row of the next box
+};
+
+// The current item's stages that this share holds (a stage belongs to the
+// share that holds its first unit), and where their keys are. False if none.
+template <typename C> WATTN_DEVINL bool pa_enter(const PagedAttendParams &p, PaLoads &ld) {
+  const PaStart &w = ld.w;
+  ld.units = pa_units<C>(p, w.q, w.rt);
+  ld.stages = pa_stages<C>(p, w.q, w.rt);
+  ld.weight = pa_weight<C>(w.q, w.rt);
+  const int d = w.lo - w.at, e = w.hi - w.at;
+  ld.t = d <= 0 ? 0 : (d + ld.weight - 1) / ld.weight;
+  ld.to = e >= ld.units ? ld.stages : min(ld.stages, (e + ld.weight - 1) / ld.weight);
+  ld.end = pa_end<C>(p, w.q, w.rt);
+  ld.page = ld.t * C::kKeys / p.page_rows;
+  ld.in_page = ld.t * C::kKeys - ld.page * p.page_rows;
+  return ld.t < ld.to;
+}
+
+// On to the next item of the share that has stages in it; false at the end.
+// `fresh` is set on entering an item, `moved` on entering another request.
+template <typename C>
+WATTN_DEVINL bool pa_advance(const PagedAttendParams &p, PaLoads &ld, bool &fresh, bool &moved) {
+  PaStart &w = ld.w;
+  while (ld.t >= ld.to) {
+    w.at += ld.units;
+    if (w.at >= w.hi) return false;
+    if (++w.rt * C::kRows >= w.q.n) {
+      w.rt = 0;
+      if (++w.head == p.n_heads) {
+        w.head = 0;
+        do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
+        moved = true;
+      }
+    }
+    fresh = pa_enter<C>(p, ld);
+  }
+  return true;
+}
+
+// The current item, as the loads announce it.
+template <typename C>
+WATTN_DEVINL PaItem pa_item_of(const PaLoads &ld) {
+  const PaStart &w = ld.w;
+  const int row = w.rt * C::kRows;
+  PaItem it;
+  it.row0 = w.q.first + row;
+  it.nr = min(C::kRows, w.q.n - row);
+  it.row = row;
+  it.len = w.q.len;
+  it.end = ld.end;
+  it.head = w.head;
+  it.from = ld.t;
+  it.to = ld.to;
+  it.stages = ld.stages;
+  it.weight = ld.weight;
+  it.at = w.at;
+  return it;
+}
+
+// The kernel for many new rows a request (paged_attend_wide.cu), 16-bit pools.
+int launch_paged_attend_wide(const PagedAttendParams &p, int dtype, int out_dtype, cudaStream_t st);
+size_t paged_attend_wide_workspace(int n_sm);
+
+}  // namespace wattn

@@ -9,7 +9,7 @@
 use std::{env, fs, path::PathBuf, process::Command};
 
 /// Every CUDA source of the library (csrc/<name>.cu).
-const SOURCES: [&str; 9] = [
+const SOURCES: [&str; 10] = [
     "api",
     "attn_f32",
     "attn_tc",
@@ -19,6 +19,7 @@ const SOURCES: [&str; 9] = [
     "linear_tc",
     "paged",
     "paged_attend",
+    "paged_attend_wide",
 ];
 
 const ARCH: [&str; 2] = ["-gencode", "arch=compute_100a,code=sm_100a"];
