@@ -36,9 +36,11 @@ constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
 static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
 // New rows of a request, averaged over the row buffer (the counts themselves
 // are on the device), from which the wide kernel is the faster one.
-constexpr int kPaWideRows = 20;
+constexpr int kPaWideRows = 64;
+constexpr int kPaMergeAll = 8;    // CTAs beyond the first from which all warps merge an item
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
+static_assert(kPaStages * kPaStageBytes >= kPaWarps * kPaTileFloats * 4, "a ring holds the warps' sums");
 
 // A stage is 8 KB of keys and values. Units: measured, two tiles of 16 rows
 // cost half as much again as one.
@@ -70,6 +72,7 @@ struct PaSmem {
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
   PaFind<PaType<T>> find;
   int merge_first[2 * kPaWarps], merge_last[2 * kPaWarps];  // shares to merge, per cut item
+  int final[2 * kPaWarps];  // this CTA merges the parts of them all
   int abort;
 };
 
@@ -159,11 +162,11 @@ WATTN_DEVINL void pa_put(float4 *part, const PaTile &a) {
   for (int db = 0; db < 8; ++db) part[db * 32] = make_float4(a.o[db][0], a.o[db][1], a.o[db][2], a.o[db][3]);
   part[8 * 32] = make_float4(a.m[0], a.m[1], a.l[0], a.l[1]);
 }
-// Adds a partial to `a` (log-sum-exp).
-WATTN_DEVINL void pa_add(PaTile &a, const float4 *part) {
+// Adds a partial to `a` (log-sum-exp). L2: it is other threads', in global memory.
+template <bool L2 = true> WATTN_DEVINL void pa_add(PaTile &a, const float4 *part) {
   float4 x[9];
 #pragma unroll
-  for (int i = 0; i < 9; ++i) x[i] = __ldcg(part + i * 32);
+  for (int i = 0; i < 9; ++i) x[i] = L2 ? __ldcg(part + i * 32) : part[i * 32];
   float wa[2], wb[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -802,21 +805,24 @@ WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, cons
 // Barrier of the compute warps (the load warps have left by then).
 WATTN_DEVINL void pa_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// Adds shares c0 .. c1's partials of a cut item, in order (`starts`: c0's is
-// the one that starts it).
-WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c1, bool starts, int mt,
-                            int lane) {
+// Adds partials c0, c0 + step, ... up to c1 of a cut item, in order (`starts`:
+// c0's is the one that starts it).
+WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c1, int step, bool starts,
+                            int mt, int lane) {
 #pragma unroll
   for (int db = 0; db < 8; ++db) a.o[db][0] = a.o[db][1] = a.o[db][2] = a.o[db][3] = 0.f;
   a.m[0] = a.m[1] = -INFINITY;
   a.l[0] = a.l[1] = 0.f;
 #pragma unroll 2
-  for (int c = c0; c <= c1; ++c) pa_add(a, pa_part(p, c, starts && c == c0, mt, lane));
+  for (int c = c0; c <= c1; c += step) pa_add(a, pa_part(p, c, starts && c == c0, mt, lane));
 }
 
 // The items cut by the shares of this CTA's warps, after all of them are
-// done, an item per warp: the CTA's parts of an item are merged, and where
-// several CTAs have parts the last of them to arrive merges theirs.
+// done: the CTA's parts of an item are merged, an item per warp, and where
+// several CTAs have parts the last of them to arrive merges theirs. (A few
+// by the same warp: 41 us against 44 us with all warps for trees of 33 rows
+// over 448 tokens; many with all: 81,000 cycles to 68,000 for one request of
+// 32768 tokens, whose heads lie in 37 CTAs each.)
 template <typename T, typename OutT>
 WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, int lane) {
   const int tid = threadIdx.x, cta0 = blockIdx.x * kPaWarps, ctas = gridDim.x * kPaWarps;
@@ -833,12 +839,15 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, 
     }
     s.merge_first[tid] = w0;
     s.merge_last[tid] = w1;
+    s.final[tid] = 0;
   }
   pa_sync();
   int turn = 0;
+  bool far = false;  // an item here lies in many CTAs
 #pragma unroll 1
   for (int e = 0; e < 2 * kPaWarps; ++e) {
     const int w0 = s.merge_first[e], w1 = s.merge_last[e];
+    far |= w1 / kPaWarps - w0 / kPaWarps >= kPaMergeAll;
     if (w1 < w0 || (turn++ & (kPaWarps - 1)) != warp) continue;
     const PaItem &it = s.cut[e >> 1][e & 1];
     const int first = max(w0, cta0), last = min(w1, cta0 + kPaWarps - 1);
@@ -847,7 +856,7 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, 
 #pragma unroll 1
     for (int mt = 0; mt < tiles; ++mt) {
       PaTile a;
-      pa_gather(p, a, first, last, first == w0, mt, lane);
+      pa_gather(p, a, first, last, 1, first == w0, mt, lane);
       if (alone) pa_output<T, OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
       else pa_put(pa_part(p, ctas + blockIdx.x, first == w0, mt, lane), a);
     }
@@ -866,11 +875,39 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, 
       }
     }
     if (!__shfl_sync(0xffffffffu, mine, 0)) continue;
+    if (c1 - c0 >= kPaMergeAll) {
+      if (lane == 0) s.final[e] = 1;
+      continue;
+    }
 #pragma unroll 1
     for (int mt = 0; mt < tiles; ++mt) {
       PaTile a;
-      pa_gather(p, a, ctas + c0, ctas + c1, true, mt, lane);
+      pa_gather(p, a, ctas + c0, ctas + c1, 1, true, mt, lane);
       pa_output<T, OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+    }
+  }
+  if (!far) return;  // (the same for all warps)
+  pa_sync();
+#pragma unroll 1
+  for (int e = 0; e < 2 * kPaWarps; ++e) {
+    if (s.final[e] == 0) continue;
+    const PaItem &it = s.cut[e >> 1][e & 1];
+    const int c0 = s.merge_first[e] / kPaWarps, c1 = s.merge_last[e] / kPaWarps;
+    const int tiles = it.nr > 16 ? 2 : 1;
+#pragma unroll 1
+    for (int mt = 0; mt < tiles; ++mt) {
+      // each warp every fourth CTA's, then the first warp the four sums (in
+      // the ring, where no loads are under way any more)
+      PaTile a;
+      pa_gather(p, a, ctas + c0 + warp, ctas + c1, kPaWarps, warp == 0, mt, lane);
+      float4 *sums = reinterpret_cast<float4 *>(s.kv[0][0]) + lane;
+      if (warp > 0) pa_put(sums + warp * (kPaTileFloats / 4), a);
+      pa_sync();
+      if (warp == 0) {
+        for (int w = 1; w < kPaWarps; ++w) pa_add<false>(a, sums + w * (kPaTileFloats / 4));
+        pa_output<T, OutT>(p, a, it.row0 + mt * 16, it.nr - mt * 16, it.head, lane);
+      }
+      pa_sync();
     }
   }
 }
