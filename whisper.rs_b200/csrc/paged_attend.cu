@@ -36,7 +36,7 @@ constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
 static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
 // New rows of a request, averaged over the row buffer (the counts themselves
 // are on the device), from which the wide kernel is the faster one.
-constexpr int kPaWideRows = 64;
+constexpr int kPaWideRows = 64, kPaWideKeys = 0;
 constexpr int kPaMergeAll = 8;    // CTAs beyond the first from which all warps merge an item
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
@@ -1093,7 +1093,8 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.count = reinterpret_cast<int *>(workspace);
   p.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + kCounterBytes);
   if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
-  if (max_rows >= (int64_t)kPaWideRows * n_seqs) return launch_paged_attend_wide(p, dtype, out_dtype, st);
+  if (dtype == WATTN_F16 && max_rows >= (int64_t)kPaWideRows * n_seqs && p.cap >= kPaWideKeys)
+    return launch_paged_attend_wide(p, out_dtype, st);
   if (dtype == WATTN_F16)
     return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
                                   : launch_stream<__half, __half>(p, dtype, st);

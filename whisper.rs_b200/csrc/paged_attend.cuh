@@ -282,8 +282,8 @@ WATTN_DEVINL PaItem pa_item_of(const PaLoads &ld) {
   return it;
 }
 
-// The kernel for many new rows a request (paged_attend_wide.cu), 16-bit pools.
-int launch_paged_attend_wide(const PagedAttendParams &p, int dtype, int out_dtype, cudaStream_t st);
+// The kernel for many new rows a request (paged_attend_wide.cu), f16 pools.
+int launch_paged_attend_wide(const PagedAttendParams &p, int out_dtype, cudaStream_t st);
 size_t paged_attend_wide_workspace(int n_sm);
 
 }  // namespace wattn

@@ -1,22 +1,25 @@
 // paged_attend_wide.cu -- attention of many new rows a request over a
-// device-planned paged cache, on the tcgen05 tensor cores (16-bit pools).
+// device-planned paged cache, on the tcgen05 tensor cores (f16 pools).
 //
 // The narrow kernel (paged_attend.cu) multiplies tiles of up to 32 rows with
 // mma.sync and reads a request's keys once for each; here one tile takes 128
-// rows (f16) or 64 (bf16), so that wide trees and prompts read them once.
+// rows, so that wide trees and the chunks of a long prompt read them once.
 //
 // One CTA per share, two CTAs on an SM (256 TMEM columns each): four softmax
 // warps with a query row per thread, and a warpgroup that leaves them its
 // registers, of which one warp loads (TMA through the block table, rings of
-// two 128-key K tiles and three V tiles) and one issues the products. S = Q K^T lands in TMEM, the softmax writes the
-// weights back to TMEM as the A operand of O += P V, and S of the next tile
-// runs under the softmax of this one.
+// two 128-key K tiles and three V tiles) and one issues the products. S = Q
+// K^T lands in TMEM, the softmax writes the weights (f16: 2^-11 each, within
+// the 2e-3 bar) back to TMEM as the A operand of O += P V, and S of the next
+// tile runs under the softmax of this one.
 //
-// bf16 weights alone (2^-8 each) would not hold the 2e-3 bar, so their
-// rounding's residual goes into the product too, at no extra cost: the
-// tile's lower 64 TMEM lanes hold the same 64 queries again, their softmax
-// (the same numbers) stores the residuals, and the two halves of O are added
-// at the end. f16 weights (2^-11) need none.
+// bf16 pools stay with the narrow kernel: bf16 weights (2^-8 each) need their
+// residuals in the product, here as a second set of 64 rows of the tile, and
+// then it was no faster (64 rows 78 us against 81, 256 rows 232 against 227).
+//
+// Bound: the chain of one tile, about 4500 cycles a CTA (S 460 to wait for,
+// scores and maximum 900, weights 1900 with the SFU shared by two CTAs, the
+// last product 590, stores 670), not HBM (1424 a tile and SM).
 
 #include <algorithm>
 
@@ -37,18 +40,19 @@ constexpr int kPwRegs = 128, kPwSoftmaxRegs = 216, kPwOtherRegs = 40;
 static_assert(kPwSoftmaxRegs + kPwOtherRegs <= 2 * kPwRegs, "a larger split never gets its registers");
 constexpr int kPwCtasPerSm = 2;
 constexpr int kPwQueue = 2;        // items announced
+// One pair of exponentials in so many runs on the FMA pipe instead of the SFU
+// (7.5e-5 off at most, less than the weights' rounding to f16).
+constexpr int kPwFmaPairs = 4;
 constexpr uint32_t kPwCols = 256;  // TMEM: S 128, P 64, O 64
 constexpr int kPwPartFloats = 66 * 128;  // a partial: O [64][row], m, l
 
-template <typename T> struct PwShape {
-  static constexpr bool kResidual = __is_same(T, __nv_bfloat16);
-  static constexpr int kKeys = kPwKeys, kRows = kResidual ? 64 : 128;
+struct PwShape {
+  static constexpr int kKeys = kPwKeys, kRows = 128;
   static constexpr int kShares = 1, kThreads = kPwThreads;
   static constexpr int kStageUnits = 2, kWideUnits = 2, kItemUnits = 3;
   static constexpr int kMinUnits = 4;
 };
 
-template <typename T>
 struct PwSmem {
   uint8_t q[kPwTile];
   uint8_t k[kPwK][kPwTile];
@@ -58,7 +62,7 @@ struct PwSmem {
   uint64_t item_full[kPwQueue], item_empty[kPwQueue];
   uint64_t drain, done;
   PaItem queue[kPwQueue];
-  PaFind<PwShape<T>> find;
+  PaFind<PwShape> find;
   uint32_t odd[4];  // keys of a tile with values that are infinite or NaN
   uint32_t tmem;
   int abort, last;
@@ -73,8 +77,7 @@ WATTN_DEVINL void pw_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // Winding down after a wait that ran out: the copies in flight (of n_k and
 // n_v tiles issued) land before the block leaves.
-template <typename T>
-WATTN_DEVINL void pw_drain(const PagedAttendParams &p, PwSmem<T> &s, uint32_t n_k, uint32_t n_v) {
+WATTN_DEVINL void pw_drain(const PagedAttendParams &p, PwSmem &s, uint32_t n_k, uint32_t n_v) {
   volatile int no_abort = 0;
   for (uint32_t c = n_k > kPwK ? n_k - kPwK : 0; c < n_k; ++c)
     mbar_wait(&s.k_full[c % kPwK], (c / kPwK) & 1, &no_abort, p.status, PW_SITE(0, 5));
@@ -82,10 +85,9 @@ WATTN_DEVINL void pw_drain(const PagedAttendParams &p, PwSmem<T> &s, uint32_t n_
     mbar_wait(&s.v_full[c % kPwV], (c / kPwV) & 1, &no_abort, p.status, PW_SITE(0, 6));
 }
 
-template <typename T>
-WATTN_DEVINL void pw_load(const PagedAttendParams &p, PwSmem<T> &s, const CUtensorMap &map,
+WATTN_DEVINL void pw_load(const PagedAttendParams &p, PwSmem &s, const CUtensorMap &map,
                           const CUtensorMap &map_tail, int lane) {
-  using C = PwShape<T>;
+  using C = PwShape;
   PaLoads ld;
   ld.w = pa_start<C>(p, s.find, 0);
   PaStart &w = ld.w;
@@ -109,6 +111,9 @@ WATTN_DEVINL void pw_load(const PagedAttendParams &p, PwSmem<T> &s, const CUtens
         s.queue[slot] = it;
         mbar_arrive(&s.item_full[slot]);
       }
+      for (int r = lane; r < it.nr; r += 32)  // its query rows will be wanted soon
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(reinterpret_cast<const __half *>(p.q) +
+                                                      (int64_t)(it.row0 + r) * p.q_rs + it.head * 64));
       ++items;
       fresh = false;
       if (!more) return;
@@ -156,11 +161,9 @@ WATTN_DEVINL void pw_load(const PagedAttendParams &p, PwSmem<T> &s, const CUtens
 
 // ---------------------------------------------------------------- product warp
 
-template <typename T>
-WATTN_DEVINL void pw_products(const PagedAttendParams &p, PwSmem<T> &s, uint32_t tmem) {
-  constexpr uint32_t ab = __is_same(T, __nv_bfloat16) ? 1u : 0u;
-  constexpr uint32_t idesc_s = idesc_f16(ab, 128, kPwKeys, 0, 0);  // Q and K K-major
-  constexpr uint32_t idesc_o = idesc_f16(ab, 128, 64, 0, 1);       // P from TMEM, V MN-major
+WATTN_DEVINL void pw_products(const PagedAttendParams &p, PwSmem &s, uint32_t tmem) {
+  constexpr uint32_t idesc_s = idesc_f16(0, 128, kPwKeys, 0, 0);  // Q and K K-major
+  constexpr uint32_t idesc_o = idesc_f16(0, 128, 64, 0, 1);       // P from TMEM, V MN-major
   const uint64_t dq = smem_desc_sw128(smem_u32(s.q), 16, 1024);
   const uint64_t dk0 = smem_desc_sw128(smem_u32(s.k[0]), 16, 1024);
   const uint64_t dv0 = smem_desc_sw128(smem_u32(s.v[0]), 16384, 1024);
@@ -242,14 +245,10 @@ WATTN_DEVINL uint32_t pw_visible(const PagedAttendParams &p, const PaItem &it, i
   return left > 0 ? pa_visible(p, it.row0 + r, it.row + r, off, left) : 0u;
 }
 
-template <typename T, typename OutT>
-WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t tmem, int tid) {
-  using C = PwShape<T>;
-  constexpr bool kRes = C::kResidual;
+template <typename OutT>
+WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tmem, int tid) {
   const int wq = tid >> 5, lane = tid & 31;
-  const int r = kRes ? tid & 63 : tid;            // row of the tile
-  const bool low = kRes && tid >= 64;             // this thread's weights are the residuals
-  const int warp_row = kRes ? (wq & 1) * 32 : wq * 32;
+  const int r = tid;  // row of the tile
   const uint32_t t_s = tmem + (uint32_t(wq * 32) << 16), t_p = t_s + 128, t_o = t_s + 192;
   uint32_t n = 0;  // tiles so far
 #pragma unroll 1
@@ -263,11 +262,11 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
     if (lane == 0) mbar_arrive(&s.item_empty[islot]);
     if (it.nr == 0) return;
     const bool mine = r < it.nr;           // this thread has a row
-    const bool warp_has = warp_row < it.nr;  // (one of) its warp has
+    const bool warp_has = wq * 32 < it.nr;  // (one of) its warp has
     // ---- the query row, 128-byte swizzled, zeros behind the last; O = 0
     {
       const uint4 *src = reinterpret_cast<const uint4 *>(
-          reinterpret_cast<const T *>(p.q) + (int64_t)(it.row0 + r) * p.q_rs + it.head * 64);
+          reinterpret_cast<const __half *>(p.q) + (int64_t)(it.row0 + r) * p.q_rs + it.head * 64);
 #pragma unroll
       for (int c = 0; c < 8; ++c)
         *reinterpret_cast<uint4 *>(s.q + tid * 128 + ((c ^ (tid & 7)) << 4)) =
@@ -335,14 +334,14 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
         for (int e = 0; e < 64; ++e) {
           const float2 y = __ffma2_rn(make_float2(x(2 * e), x(2 * e + 1)), c2, nmu2);
           float2 w;
-          w.x = ex2(y.x);
-          w.y = ex2(y.y);
-          acc[e & 1] = __fadd2_rn(acc[e & 1], w);
-          pk[e] = pack2<T>(w.x, w.y);
-          if (kRes && low) {  // (the same branch for the whole warp)
-            const float2 hi = unpack2<T>(pk[e]);
-            pk[e] = pack2<T>(w.x - hi.x, w.y - hi.y);
+          if (e % kPwFmaPairs == kPwFmaPairs - 1) {
+            w = exp2_fma2(y);
+          } else {
+            w.x = ex2(y.x);
+            w.y = ex2(y.y);
           }
+          acc[e & 1] = __fadd2_rn(acc[e & 1], w);
+          pk[e] = pack2<__half>(w.x, w.y);
         }
         l += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
       }
@@ -372,7 +371,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
                                                PW_SITE(2, 3))))
           return;
         uint8_t *tile = s.v[vslot], *vrow = tile + tid * 128;
-        constexpr uint32_t kInf2 = (kRes ? 0x7f80u : 0x7c00u) * 0x10001u;
+        constexpr uint32_t kInf2 = 0x7c007c00u;
         bool odd = false;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -396,7 +395,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
               tmem_ld32(t_o + 32 * h, o);
               tmem_wait_ld();
               reg_fence(o);
-              if (mine && !low)
+              if (mine)
 #pragma unroll 1
                 for (int k = 0; k < kPwKeys; ++k) {
                   if (!(s.odd[k >> 5] >> (k & 31) & 1u)) continue;
@@ -404,7 +403,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
 #pragma unroll
                   for (int e = 0; e < 32; ++e) {
                     const int d = h * 32 + e;
-                    const float v = to_f32(*reinterpret_cast<const T *>(
+                    const float v = to_f32(*reinterpret_cast<const __half *>(
                         tile + k * 128 + (((d >> 3) ^ (k & 7)) << 4) + (d & 7) * 2));
                     if (!(fabsf(v) < INFINITY)) o[e] = __float_as_uint(__uint_as_float(o[e]) + v);
                   }
@@ -449,28 +448,16 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
 #pragma unroll
       for (int e = 0; e < 64; ++e) o[e] = __uint_as_float(u[e >> 5][e & 31]);
     }
-    if constexpr (kRes) {
-      // the residuals' half through the query tile, whose last S is done
-      float *half = reinterpret_cast<float *>(s.q);
-      if (low && mine)
-#pragma unroll
-        for (int e = 0; e < 64; ++e) half[e * 64 + r] = o[e];
-      pw_sync();
-      if (!low && mine)
-#pragma unroll
-        for (int e = 0; e < 64; ++e) o[e] += half[e * 64 + r];
-      pw_sync();  // read before the next query rows come
-    }
     const bool starts = it.from == 0;
     if (starts && it.to == it.stages) {
-      if (mine && !low)
+      if (mine)
         pw_store_row<OutT>(p, o, l == 0.f ? 0.f : __fdividef(1.f, l), it.row0 + r, it.head);
       continue;
     }
     // A cut item: this share's part, merged by the last of its shares.
     const int c0 = pa_owner(s.find.shares, it.at);
     const int c1 = pa_owner(s.find.shares, it.at + (it.stages - 1) * it.weight);
-    if (mine && !low) {
+    if (mine) {
       float *part = pw_part(p, blockIdx.x, starts) + r;
 #pragma unroll
       for (int e = 0; e < 64; ++e) part[e * 128] = o[e];
@@ -489,7 +476,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
       }
     }
     pw_sync();
-    if (s.last && mine && !low) {
+    if (s.last && mine) {
       float M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int e = 0; e < 64; ++e) o[e] = 0.f;
@@ -512,12 +499,12 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem<T> &s, uint32_t 
 
 // ---------------------------------------------------------------- kernel
 
-template <typename T, typename OutT>
+template <typename OutT>
 __global__ void __launch_bounds__(kPwThreads, kPwCtasPerSm)
     paged_attend_wide_kernel(const __grid_constant__ CUtensorMap map,
                              const __grid_constant__ CUtensorMap map_tail, const PagedAttendParams p) {
   extern __shared__ uint8_t pw_smem_raw[];
-  PwSmem<T> &s = *reinterpret_cast<PwSmem<T> *>(
+  PwSmem &s = *reinterpret_cast<PwSmem *>(
       (reinterpret_cast<uintptr_t>(pw_smem_raw) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -553,13 +540,13 @@ __global__ void __launch_bounds__(kPwThreads, kPwCtasPerSm)
   tc_fence_after();
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  pa_find_shares<PwShape<T>>(p, s.find);
+  pa_find_shares<PwShape>(p, s.find);
   const uint32_t tmem = s.tmem;
   if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPwOtherRegs));
-    if (warp == kPwLoadWarp) pw_load<T>(p, s, map, map_tail, lane);
+    if (warp == kPwLoadWarp) pw_load(p, s, map, map_tail, lane);
     if (warp == kPwMmaWarp) {
-      if (lane == 0) pw_products<T>(p, s, tmem);
+      if (lane == 0) pw_products(p, s, tmem);
       __syncwarp();
       // the softmax warps are done with the columns (bounded, like all waits)
       volatile int no_abort = 0;
@@ -571,13 +558,13 @@ __global__ void __launch_bounds__(kPwThreads, kPwCtasPerSm)
     return;
   }
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPwSoftmaxRegs));
-  pw_softmax<T, OutT>(p, s, tmem, tid);
+  pw_softmax<OutT>(p, s, tmem, tid);
   tc_fence_before();
   mbar_arrive(&s.done);
 }
 
-template <typename T, typename OutT>
-int launch_wide(PagedAttendParams p, int dtype, cudaStream_t st) {
+template <typename OutT>
+int launch_wide(PagedAttendParams p, cudaStream_t st) {
   // The pool as [page, layer][K|V][head, row][64]; boxes of rows within a page.
   const uint64_t kv_rows = (uint64_t)p.n_heads * p.page_rows;
   p.box_rows = p.page_rows % 128 == 0 ? 128 : p.page_rows % 64 == 0 ? 64 : p.page_rows % 32 == 0 ? 32 : kPaTail;
@@ -585,13 +572,13 @@ int launch_wide(PagedAttendParams p, int dtype, cudaStream_t st) {
   const uint64_t strides[3] = {128, kv_rows * 128, kv_rows * 256};
   const uint32_t box[4] = {64, (uint32_t)p.box_rows, 1, 1}, box_tail[4] = {64, kPaTail, 1, 1};
   CUtensorMap map, map_tail;
-  int rc = encode_tmap(&map, tmap_dtype(dtype), 4, p.pool, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  int rc = encode_tmap(&map, tmap_dtype(WATTN_F16), 4, p.pool, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == WATTN_OK)
-    rc = encode_tmap(&map_tail, tmap_dtype(dtype), 4, p.pool, dims, strides, box_tail,
+    rc = encode_tmap(&map_tail, tmap_dtype(WATTN_F16), 4, p.pool, dims, strides, box_tail,
                      CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc != WATTN_OK) return rc;
-  constexpr int smem = (int)sizeof(PwSmem<T>) + 1024;
-  auto kern = paged_attend_wide_kernel<T, OutT>;
+  constexpr int smem = (int)sizeof(PwSmem) + 1024;
+  auto kern = paged_attend_wide_kernel<OutT>;
   // Once per process and type: the warpgroups' register split counts on what
   // the kernel is launched with (with fewer it would wait for ever).
   static const int regs = [&] {
@@ -608,12 +595,8 @@ int launch_wide(PagedAttendParams p, int dtype, cudaStream_t st) {
 
 }  // namespace
 
-int launch_paged_attend_wide(const PagedAttendParams &p, int dtype, int out_dtype, cudaStream_t st) {
-  if (dtype == WATTN_F16)
-    return out_dtype == WATTN_F32 ? launch_wide<__half, float>(p, dtype, st)
-                                  : launch_wide<__half, __half>(p, dtype, st);
-  return out_dtype == WATTN_F32 ? launch_wide<__nv_bfloat16, float>(p, dtype, st)
-                                : launch_wide<__nv_bfloat16, __nv_bfloat16>(p, dtype, st);
+int launch_paged_attend_wide(const PagedAttendParams &p, int out_dtype, cudaStream_t st) {
+  return out_dtype == WATTN_F32 ? launch_wide<float>(p, st) : launch_wide<__half>(p, st);
 }
 
 size_t paged_attend_wide_workspace(int n_sm) {
