@@ -932,6 +932,10 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
     s.abort = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x == kPaWarps * 32) {
+    tma_prefetch_desc(&map);
+    tma_prefetch_desc(&map_tail);
+  }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
   pa_find_shares<PaType<T>>(p, s.find);

@@ -530,6 +530,10 @@ __global__ void __launch_bounds__(kPwThreads, kPwCtasPerSm)
     s.abort = 0;
     fence_barrier_init();
   }
+  if (tid == kPwLoadWarp * 32) {
+    tma_prefetch_desc(&map);
+    tma_prefetch_desc(&map_tail);
+  }
   if (warp == kPwMmaWarp) {
     __syncwarp();
     tmem_alloc(&s.tmem, kPwCols);
