@@ -181,7 +181,13 @@ template <typename C> WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, 
   w.lo = pa_share_begin(s.shares, c);
   w.hi = pa_share_begin(s.shares, c + 1);
   w.at = s.run_at[k];
+  // (The walks end with the requests and row tiles even if another stream
+  // changes the arrays meanwhile.)
   for (w.s = s.run_first[k];; ++w.s) {
+    if (w.s >= p.n_seqs) {
+      w.hi = w.lo;
+      return w;
+    }
     w.q = pa_seq(p, w.s, nullptr);
     const int u = (int)pa_head_units<C>(p, w.q);
     if (w.lo - w.at < (long long)u * p.n_heads) {
@@ -192,6 +198,10 @@ template <typename C> WATTN_DEVINL PaStart pa_start(const PagedAttendParams &p, 
     w.at += u * p.n_heads;
   }
   for (w.rt = 0;; ++w.rt) {
+    if (w.rt * C::kRows >= w.q.n) {
+      w.hi = w.lo;
+      return w;
+    }
     const int u = pa_units<C>(p, w.q, w.rt);
     if (w.lo - w.at < u) break;
     w.at += u;
@@ -253,7 +263,10 @@ WATTN_DEVINL bool pa_advance(const PagedAttendParams &p, PaLoads &ld, bool &fres
       w.rt = 0;
       if (++w.head == p.n_heads) {
         w.head = 0;
-        do w.q = pa_seq(p, ++w.s, nullptr); while (w.q.n == 0);
+        do {
+          if (++w.s >= p.n_seqs) return false;
+          w.q = pa_seq(p, w.s, nullptr);
+        } while (w.q.n == 0);
         moved = true;
       }
     }
