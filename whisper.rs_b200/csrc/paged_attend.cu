@@ -15,6 +15,11 @@
 // item's keys. The parts of a cut item are merged by log-sum-exp in the order
 // of the keys, by its CTA or, where it spans several, by the last of them:
 // same inputs, same bits.
+//
+// Many small items (a step of beams: 448 requests x 12 heads) are not cut but
+// taken one by one from a counter: the warps of an SM share what it can read,
+// so equal shares end unequally, and taken ones even that out. 361 MB of keys
+// and values: 73 us (4.9 TB/s) against 87.5 in equal shares.
 #include <algorithm>
 
 #include "paged_attend.cuh"
@@ -35,8 +40,12 @@ constexpr int kPaCtasPerSm = 2;
 constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
 static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
 // New rows of a request, averaged over the row buffer (the counts themselves
-// are on the device), from which the wide kernel is the faster one.
-constexpr int kPaWideRows = 64, kPaWideKeys = 0;
+// are on the device), and positions that a request may hold, from which the
+// wide kernel is the faster one. f16, wide / narrow: 16 requests of 8 heads,
+// 4096 cached, 96 rows 71 us / 83, 128 rows 70 / 107, 256 rows 113 / 193; 16
+// heads, 500 cached, 128 rows 47 / 53; but 1000 cached, 96 rows 64 / 58, and
+// 32 requests of 20 heads with nothing cached, 128 rows 44 / 37.
+constexpr int kPaWideRows = 112, kPaWideKeys = 512;
 constexpr int kPaMergeAll = 8;    // CTAs beyond the first from which all warps merge an item
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
@@ -46,6 +55,11 @@ static_assert(kPaStages * kPaStageBytes >= kPaWarps * kPaTileFloats * 4, "a ring
 // cost half as much again as one.
 struct PaShape {
   static constexpr int kShares = kPaWarps, kThreads = kPaThreads;
+  // Items to a compute warp from which they are taken one by one (cached
+  // lengths from 1 to 440, f16, taken / in equal shares: 400 requests of 12
+  // heads 68.6 us / 76.8, 600 88.3 / 103.4, 300 of 20 heads and 40 new rows
+  // 235 / 273; of 200 or 300 requests of 12 heads the lookup alone costs 2 us).
+  static constexpr int kQueueItems = 4;
   static constexpr int kStageUnits = 2, kWideUnits = 3, kItemUnits = 2;
   static constexpr int kMinUnits = 8;  // units of a share below which fewer warps work
 };
@@ -234,24 +248,46 @@ WATTN_DEVINL void pa_announce(const PagedAttendParams &p, PaItem &to, const PaLo
 // A load warp: fills the ring of compute warp k, stage by stage over its
 // share's items, each announced before its first stage; an item without rows
 // ends the share.
-template <typename T>
+template <typename T, bool QUEUE>
 WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem<T> &s, const CUtensorMap &map,
                           const CUtensorMap &map_tail, int k, int lane) {
   using C = PaType<T>;
   PaLoads ld;
-  ld.w = pa_start<C>(p, s.find, k);
+  const bool queue = QUEUE && s.find.queue;
+  if (!queue) ld.w = pa_start<C>(p, s.find, k);
   PaStart &w = ld.w;
   int base = INT_MIN / 2, entry = 0;  // lane i holds table entry base + i of the request
   int slot = 0;
   uint32_t phase = 1;  // (a wait for the phase before the first passes)
   uint32_t items = 0, issued = 0;
   bool fresh = false;  // an item not yet announced
-  const bool some = w.lo < w.hi;
+  const bool some = !queue && w.lo < w.hi;
   if (some) fresh = pa_enter<C>(p, ld);
+  bool first = true;
+  if (queue) ld.t = ld.to = 0;
 #pragma unroll 1
   for (;;) {
     bool moved = false;
-    const bool more = some && pa_advance<C>(p, ld, fresh, moved);
+    bool more = some && pa_advance<C>(p, ld, fresh, moved);
+    if (queue) {
+      more = ld.t < ld.to;
+      while (!more) {
+        const int warps = gridDim.x * kPaWarps;
+        int i = blockIdx.x * kPaWarps + k;  // the first by the warp's place
+        if (first) {
+          first = false;
+        } else {
+          if (lane == 0) i = warps + atomicAdd(p.taken, 1);
+          i = __shfl_sync(0xffffffffu, i, 0);
+        }
+        if (i >= s.find.items) {
+          // The last warp to find nothing left sets the count back for the next call.
+          if (lane == 0 && i == s.find.items + warps - 1) *p.taken = 0;
+          break;
+        }
+        more = fresh = moved = pa_take<C>(p, s.find, ld, i, lane);
+      }
+    }
     if (moved) base = INT_MIN / 2;  // another request's table
     const bool ok = mbar_wait(&s.empty[k][slot], phase, &s.abort, p.status, (4 << 24) | (3 << 16));
     if (!__all_sync(0xffffffffu, ok)) {
@@ -914,7 +950,7 @@ WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, 
 
 // `map` has boxes of a stage's keys and values (used where pages hold whole
 // stages), `map_tail` boxes of 16 rows of either.
-template <typename T, typename OutT>
+template <typename T, typename OutT, bool QUEUE>
 __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
     paged_attend_stream_kernel(const __grid_constant__ CUtensorMap map,
                                const __grid_constant__ CUtensorMap map_tail,
@@ -938,10 +974,10 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  pa_find_shares<PaType<T>>(p, s.find);
+  pa_find_shares<PaType<T>, QUEUE>(p, s.find);
   if (warp >= kPaWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaLoadRegs));
-    pa_load<T>(p, s, map, map_tail, warp - kPaWarps, lane);
+    pa_load<T, QUEUE>(p, s, map, map_tail, warp - kPaWarps, lane);
     return;
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPaComputeRegs));
@@ -977,8 +1013,8 @@ size_t pa_workspace(int n_sm) {
   return std::max(narrow, paged_attend_wide_workspace(n_sm));
 }
 
-template <typename T, typename OutT>
-int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
+template <typename T, typename OutT, bool QUEUE>
+int launch_stream_as(PagedAttendParams p, int dtype, cudaStream_t st) {
   // The pool as [page, layer][K|V][head, row][64]: one box holds a stage's
   // keys and its values; the tail map's boxes hold 16 rows of either.
   // f32: boxes of half the dims of a stage's 16 keys and values.
@@ -998,7 +1034,7 @@ int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
     map = map_tail;  // not used
   if (rc != WATTN_OK) return rc;
   constexpr int smem = (int)sizeof(PaSmem<T>) + 1024;
-  auto kern = paged_attend_stream_kernel<T, OutT>;
+  auto kern = paged_attend_stream_kernel<T, OutT, QUEUE>;
   // Once per process and type: the warpgroups' register split counts on what
   // the kernel is launched with (with fewer it would wait for ever).
   static const int regs = [&] {
@@ -1011,6 +1047,14 @@ int launch_stream(PagedAttendParams p, int dtype, cudaStream_t st) {
     return check_launch("cudaFuncSetAttribute(paged_attend)");
   launch_pdl(kern, dim3(p.n_sm * kPaCtasPerSm), dim3(kPaThreads), smem, st, map, map_tail, p);
   return check_launch("paged_attend");
+}
+
+template <typename T, typename OutT>
+int launch_stream(const PagedAttendParams &p, int max_rows, int dtype, cudaStream_t st) {
+  // (No more items than this.)
+  const int64_t items = ((int64_t)max_rows / PaType<T>::kRows + p.n_seqs) * p.n_heads;
+  const bool queue = items >= (int64_t)PaShape::kQueueItems * p.n_sm * kPaCtasPerSm * kPaWarps;
+  return queue ? launch_stream_as<T, OutT, true>(p, dtype, st) : launch_stream_as<T, OutT, false>(p, dtype, st);
 }
 
 }  // namespace
@@ -1095,15 +1139,16 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
     return set_error(WATTN_ERR_INVALID, "paged_attend: the workspace must be 16-byte aligned");
   }
   p.count = reinterpret_cast<int *>(workspace);
+  p.taken = p.count + kMaxSplitCounters - 1;
   p.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + kCounterBytes);
-  if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
+  if (dtype == WATTN_F32) return launch_stream<float, float>(p, max_rows, dtype, st);
   if (dtype == WATTN_F16 && max_rows >= (int64_t)kPaWideRows * n_seqs && p.cap >= kPaWideKeys)
     return launch_paged_attend_wide(p, out_dtype, st);
   if (dtype == WATTN_F16)
-    return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
-                                  : launch_stream<__half, __half>(p, dtype, st);
-  return out_dtype == WATTN_F32 ? launch_stream<__nv_bfloat16, float>(p, dtype, st)
-                                : launch_stream<__nv_bfloat16, __nv_bfloat16>(p, dtype, st);
+    return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, max_rows, dtype, st)
+                                  : launch_stream<__half, __half>(p, max_rows, dtype, st);
+  return out_dtype == WATTN_F32 ? launch_stream<__nv_bfloat16, float>(p, max_rows, dtype, st)
+                                : launch_stream<__nv_bfloat16, __nv_bfloat16>(p, max_rows, dtype, st);
 }
 
 }  // extern "C"

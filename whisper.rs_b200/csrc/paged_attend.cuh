@@ -34,6 +34,7 @@ struct PagedAttendParams {
   int box_rows;  // rows of a TMA box of whole stages
   float *part;   // partials of cut items
   int *count;    // finished CTAs of the item that each CTA starts and another ends
+  int *taken;    // items taken from the queue
   int *status;
   int n_sm;
 };
@@ -120,22 +121,51 @@ template <typename C> struct PaFind {
   long long warp_sums[C::kThreads / 32];
   PaShares shares;
   int total;
+  // Of a queue: (items and the units of the largest, of each warp's requests.)
+  int warp_items[C::kThreads / 32], warp_most[C::kThreads / 32];
+  // Whether the items are taken one by one; their number, that of the large
+  // ones (over `small` units), and for each thread's run of requests the
+  // large and the other items before its own.
+  bool queue;
+  int items, large, small;
+  int run_large[C::kThreads], run_small[C::kThreads];
 };
+
+// The row tiles of a request, and the units of its largest item.
+template <typename C> WATTN_DEVINL int pa_tiles(const PaSeq &q) { return (q.n + C::kRows - 1) / C::kRows; }
+template <typename C> WATTN_DEVINL int pa_most(const PagedAttendParams &p, const PaSeq &q) {
+  return q.n > 0 ? max(pa_units<C>(p, q, 0), pa_units<C>(p, q, pa_tiles<C>(q) - 1)) : 0;
+}
 
 // The shares. All threads of the CTA add up the units of a run of requests
 // each; the sums are scanned, and for each share of the CTA the run that
-// holds its first unit is noted.
-template <typename C> WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaFind<C> &s) {
+// holds its first unit is noted. With QUEUE, many items of about the same size
+// are left whole, for the warps to take one by one: those of more than half
+// the largest's units first, so that short ones even out the end.
+template <typename C, bool QUEUE = false> WATTN_DEVINL void pa_find_shares(const PagedAttendParams &p, PaFind<C> &s) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
   const int s0 = min(tid * per, p.n_seqs), s1 = min(s0 + per, p.n_seqs);
   long long mine = 0;
+  int items = 0, most = 0;
 #pragma unroll 4
   for (int i = s0; i < s1; ++i) {
     bool bad;
     const PaSeq q = pa_seq(p, i, &bad);
     if (bad) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
     mine += pa_head_units<C>(p, q) * p.n_heads;
+    if constexpr (QUEUE) {
+      items += pa_tiles<C>(q) * p.n_heads;
+      most = max(most, pa_most<C>(p, q));
+    }
+  }
+  if constexpr (QUEUE) {
+    items = __reduce_add_sync(0xffffffffu, items);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+      s.warp_items[warp] = items;
+      s.warp_most[warp] = most;
+    }
   }
   long long inc = mine;
 #pragma unroll
@@ -154,6 +184,52 @@ template <typename C> WATTN_DEVINL void pa_find_shares(const PagedAttendParams &
   if (total > INT_MAX) {  // more than a call may ask for
     if (tid == 0) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
     total = 0;
+  }
+  if constexpr (QUEUE) {
+    items = most = 0;
+#pragma unroll
+    for (int w = 0; w < C::kThreads / 32; ++w) {
+      items += s.warp_items[w];
+      most = max(most, s.warp_most[w]);
+    }
+    const int parts = gridDim.x * C::kShares;
+    // (the same for all CTAs)
+    const bool queue = total > 0 && items >= C::kQueueItems * parts && most <= total / parts / 2;
+    if (tid == 0) s.queue = queue;
+    if (queue) {
+      int large = 0, small = 0;
+      for (int i = s0; i < s1; ++i) {
+        const PaSeq q = pa_seq(p, i, nullptr);
+        (pa_most<C>(p, q) > most / 2 ? large : small) += pa_tiles<C>(q) * p.n_heads;
+      }
+      int a = large, b = small;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, b, d);
+        if (lane >= d) a += x, b += y;
+      }
+      __syncthreads();  // (warp_items has been read)
+      if (lane == 31) {
+        s.warp_items[warp] = a;
+        s.warp_most[warp] = b;
+      }
+      __syncthreads();
+      int la = 0, lb = 0, all = 0;
+#pragma unroll
+      for (int w = 0; w < C::kThreads / 32; ++w) {
+        all += s.warp_items[w];
+        if (w < warp) la += s.warp_items[w], lb += s.warp_most[w];
+      }
+      s.run_large[tid] = la + a - large;
+      s.run_small[tid] = all + lb + b - small;
+      if (tid == 0) {
+        s.items = items;
+        s.large = all;
+        s.small = most / 2;
+      }
+      __syncthreads();
+      return;
+    }
   }
   const PaShares shares = pa_shares<C>((int)total, gridDim.x * C::kShares);
   if (tid == 0) {
@@ -273,6 +349,53 @@ WATTN_DEVINL bool pa_advance(const PagedAttendParams &p, PaLoads &ld, bool &fres
     fresh = pa_enter<C>(p, ld);
   }
   return true;
+}
+
+// Item k of those taken one by one, whole: the large ones in the order of
+// requests, heads and row tiles, then the others. False if there is none (the
+// arrays were changed meanwhile).
+template <typename C>
+WATTN_DEVINL bool pa_take(const PagedAttendParams &p, const PaFind<C> &s, PaLoads &ld, int k, int lane) {
+  const bool large = k < s.large;
+  const int *run = large ? s.run_large : s.run_small;
+  int lo = 0, hi = C::kThreads;  // the last run with at most k items before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (run[mid] <= k) lo = mid; else hi = mid;
+  }
+  const int per = (p.n_seqs + C::kThreads - 1) / C::kThreads;
+  PaStart &w = ld.w;
+  int left = k - run[lo];
+  for (int first = lo * per; first < p.n_seqs; first += 32) {
+    // (32 requests at a time)
+    int here = 0;
+    if (first + lane < p.n_seqs) {
+      const PaSeq q = pa_seq(p, first + lane, nullptr);
+      if ((pa_most<C>(p, q) > s.small) == large) here = pa_tiles<C>(q) * p.n_heads;
+    }
+    int upto = here;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, upto > left);
+    if (over != 0) {
+      const int at = __ffs(over) - 1;
+      left -= __shfl_sync(0xffffffffu, upto - here, at);
+      w.s = first + at;
+      w.q = pa_seq(p, w.s, nullptr);
+      const int tiles = pa_tiles<C>(w.q);
+      if (tiles == 0) return false;
+      w.head = left / tiles;
+      w.rt = left - w.head * tiles;
+      w.at = w.lo = 0;
+      w.hi = INT_MAX;
+      return w.head < p.n_heads && pa_enter<C>(p, ld);
+    }
+    left -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
 }
 
 // The current item, as the loads announce it.

@@ -49,6 +49,7 @@ constexpr int kPwPartFloats = 66 * 128;  // a partial: O [64][row], m, l
 struct PwShape {
   static constexpr int kKeys = kPwKeys, kRows = 128;
   static constexpr int kShares = 1, kThreads = kPwThreads;
+  static constexpr int kQueueItems = 0;  // (no queue)
   static constexpr int kStageUnits = 2, kWideUnits = 2, kItemUnits = 3;
   static constexpr int kMinUnits = 4;
 };
