@@ -385,8 +385,8 @@ int wattn_kv_stats(const wattn_kv_cache *cache, int *pages_used,
  * parents [max_rows], packed as the rows: the index within its request of each
  * new row's parent, -1 for a root. Parents come before their children; a row
  * for which this fails, or whose ancestor it fails for, is dead: position -1,
- * mask 0 (it keeps its slot, where an accepted row may land). parents and row_mask are both given or both NULL (the
- * new rows then follow each other).
+ * mask 0 (it keeps its slot, where an accepted row may land). parents and
+ * row_mask are both given or both NULL (the new rows then follow each other).
  * status [1] receives WATTN_OK; WATTN_ERR_INVALID (negative lengths, n_held
  * outside [0, max_pages], a stack that would overflow), WATTN_ERR_RANGE (a
  * request needs more than max_pages pages or, with a tree, has more than
@@ -416,12 +416,19 @@ int wattn_paged_write(void *pool, int dtype, int n_pages, int n_layers, int n_he
  * hold; a row that sees nothing gives 0. q and o: packed rows [max_rows]
  * [n_heads*64], q of the pool's type, o of out_dtype (WATTN_F32 or the pool's
  * type), 16-byte aligned with row strides (elements) that are multiples of 16
- * bytes. A table entry outside the pool, lengths beyond max_pages pages or row
+ * bytes; o overlaps none of the inputs. Cached keys and values are seen by
+ * every row: one that is infinite or NaN may make any of its request's outputs
+ * NaN. A table entry outside the pool, lengths beyond max_pages pages or row
  * starts outside [0, max_rows] make that request's rows unspecified, and
- * wattn_device_status() reports WATTN_ERR_RANGE. workspace as for
- * wattn_decode_fwd (wattn_paged_attend_workspace_bytes(), zero-filled before
- * its first use), or NULL; calls that may overlap, captured graphs among them,
- * need one each. */
+ * wattn_device_status() reports WATTN_ERR_RANGE; so does a call of 2^31 units
+ * of work or more (about three for every 16 keys of each head and tile of 16
+ * rows), which writes no rows. workspace as for wattn_decode_fwd
+ * (wattn_paged_attend_workspace_bytes(), zero-filled before its first use),
+ * or NULL. Calls that may overlap, captured graphs among them, need one each;
+ * a call that is captured with NULL gets one of its graph's own, at the price
+ * of a memset in it. After WATTN_ERR_TIMEOUT a workspace is zero-filled again
+ * before its next use (wattn_device_status() does so for the calling thread's
+ * own). */
 size_t wattn_paged_attend_workspace_bytes(int n_seqs, int max_rows, int n_heads);
 int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, int n_heads,
                        int page_rows, int layer, const int *block_table, int64_t table_stride,

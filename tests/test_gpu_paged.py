@@ -651,6 +651,42 @@ def test_runs_on_the_callers_stream(W):
             assert np.array_equal(o[:30].float().cpu().numpy(), x)
 
 
+@pytest.mark.parametrize("kind", ["cut", "taken", "wide"])
+def test_graphs_without_a_workspace(W, kind):
+    """Two graphs captured without a workspace, replayed at once on two streams
+    and next to an eager call, which uses the thread's."""
+    import torch
+    if kind == "cut":
+        batches = [Batch(80 + i, "bf16", [400, 30, 1800], [20, 3, 7], 4, 64) for i in range(2)]
+    elif kind == "taken":
+        batches = [many(82 + i, "f16") for i in range(2)]
+    else:
+        batches = [wide_batch(84 + i, [600, 20, 0], [150, 190, 1], 3, 64) for i in range(2)]
+    work = []
+    for b in batches:
+        want = torch.zeros(b.max_rows, b.heads * 64, device="cuda")
+        a = dict(zip(("block_table", "seq_lens", "row_start", "row_mask"), b.device()))
+        W.paged_attend(b.pool, 0, q=b.q, o=want, **a)
+        o, s, g = torch.zeros_like(want), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            for _ in range(3):
+                W.paged_attend(b.pool, 0, q=b.q, o=o, **a)
+        work.append((b, a, want, o, s, g))
+    for _ in range(4):
+        for b, a, want, o, s, g in work:
+            with torch.cuda.stream(s):
+                o.zero_()
+                g.replay()
+        b, a, want, *_ = work[0]
+        again = torch.zeros_like(want)
+        W.paged_attend(b.pool, 0, q=b.q, o=again, **a)
+        torch.cuda.synchronize()
+        assert torch.equal(again, want)
+        for b, a, want, o, s, g in work:
+            assert torch.equal(o, want)
+
+
 def test_repeats_are_bit_exact(W):
     rng = np.random.default_rng(40)
     new = [20, 1, 33, 64]
@@ -896,6 +932,26 @@ def test_bad_tables_are_reported_and_harmless(W):
         assert W.device_status() == -6, what
         # (not bit for bit: the lengths of the others move the cuts of the keys)
         assert (np.abs(o[:3].cpu().numpy() - ref) <= lim).all(), what
+
+
+@pytest.mark.parametrize("dtype,rows", [("f16", 3), ("f16", 130), ("f32", 3)])
+def test_more_work_than_can_be_counted(W, dtype, rows):
+    """Lengths that are in range but make 2^31 units of work: reported, and
+    no row is written."""
+    import torch
+    P_, heads = 4096, 64
+    pages = (1 << 30) // P_
+    pool = torch.zeros(1, 1, 2, heads, P_, 64, dtype=tdt(dtype), device="cuda")
+    table = torch.zeros(1, pages, dtype=torch.int32, device="cuda")
+    q = torch.zeros(rows, heads * 64, dtype=tdt(dtype), device="cuda")
+    o = torch.full((rows, heads * 64), 7.0, device="cuda")
+    W.paged_attend(pool, 0, table, cu(np.array([(1 << 30) - rows])), cu(np.array([0, rows])), q, o)
+    torch.cuda.synchronize()
+    assert W.device_status() == -6
+    assert (o == 7).all()
+    W.paged_attend(pool, 0, table, cu(np.array([50])), cu(np.array([0, rows])), q, o)
+    torch.cuda.synchronize()
+    assert W.device_status() == 0 and (o == 0).all()
 
 
 def test_refusals(W):

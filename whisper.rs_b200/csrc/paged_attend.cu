@@ -1050,11 +1050,22 @@ int launch_stream_as(PagedAttendParams p, int dtype, cudaStream_t st) {
 }
 
 template <typename T, typename OutT>
-int launch_stream(const PagedAttendParams &p, int max_rows, int dtype, cudaStream_t st) {
+int launch_stream(const PagedAttendParams &p, int dtype, cudaStream_t st) {
   // (No more items than this.)
-  const int64_t items = ((int64_t)max_rows / PaType<T>::kRows + p.n_seqs) * p.n_heads;
+  const int64_t items = ((int64_t)p.max_rows / PaType<T>::kRows + p.n_seqs) * p.n_heads;
   const bool queue = items >= (int64_t)PaShape::kQueueItems * p.n_sm * kPaCtasPerSm * kPaWarps;
   return queue ? launch_stream_as<T, OutT, true>(p, dtype, st) : launch_stream_as<T, OutT, false>(p, dtype, st);
+}
+
+int launch_attend(const PagedAttendParams &p, int dtype, int out_dtype, cudaStream_t st) {
+  if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
+  if (dtype == WATTN_F16 && p.max_rows >= (int64_t)kPaWideRows * p.n_seqs && p.cap >= kPaWideKeys)
+    return launch_paged_attend_wide(p, out_dtype, st);
+  if (dtype == WATTN_F16)
+    return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
+                                  : launch_stream<__half, __half>(p, dtype, st);
+  return out_dtype == WATTN_F32 ? launch_stream<__nv_bfloat16, float>(p, dtype, st)
+                                : launch_stream<__nv_bfloat16, __nv_bfloat16>(p, dtype, st);
 }
 
 }  // namespace
@@ -1129,8 +1140,20 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   cudaStream_t st = (cudaStream_t)stream;
   p.n_sm = pa_sms();
   const size_t need = pa_workspace(p.n_sm);
+  void *own = nullptr;
   if (workspace == nullptr) {
-    workspace = thread_workspace(need, st);
+    // A captured call gets a workspace of its graph's: the thread's may be in
+    // use by another graph or call when this one is replayed, or be replaced.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();
+    if (capture == cudaStreamCaptureStatusActive) {
+      if (cudaMallocAsync(&own, need, st) != cudaSuccess ||
+          cudaMemsetAsync(own, 0, kCounterBytes, st) != cudaSuccess)
+        return check_launch("paged_attend: a captured call's workspace");
+      workspace = own;
+    } else {
+      workspace = thread_workspace(need, st);
+    }
     if (workspace == nullptr) return set_error(WATTN_ERR_NOMEM, "paged_attend: workspace allocation failed");
   } else if (workspace_bytes < need) {
     return set_error(WATTN_ERR_INVALID, "paged_attend: workspace of %zu bytes, %zu needed",
@@ -1141,14 +1164,10 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.count = reinterpret_cast<int *>(workspace);
   p.taken = p.count + kMaxSplitCounters - 1;
   p.part = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(workspace) + kCounterBytes);
-  if (dtype == WATTN_F32) return launch_stream<float, float>(p, max_rows, dtype, st);
-  if (dtype == WATTN_F16 && max_rows >= (int64_t)kPaWideRows * n_seqs && p.cap >= kPaWideKeys)
-    return launch_paged_attend_wide(p, out_dtype, st);
-  if (dtype == WATTN_F16)
-    return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, max_rows, dtype, st)
-                                  : launch_stream<__half, __half>(p, max_rows, dtype, st);
-  return out_dtype == WATTN_F32 ? launch_stream<__nv_bfloat16, float>(p, max_rows, dtype, st)
-                                : launch_stream<__nv_bfloat16, __nv_bfloat16>(p, max_rows, dtype, st);
+  rc = launch_attend(p, dtype, out_dtype, st);
+  if (own != nullptr && cudaFreeAsync(own, st) != cudaSuccess && rc == WATTN_OK)
+    rc = check_launch("paged_attend: a captured call's workspace");
+  return rc;
 }
 
 }  // extern "C"

@@ -651,7 +651,8 @@ def paged_attend(pool, layer, block_table, seq_lens, row_start, q, o, *, row_mas
     """``wattn_paged_attend``: attention of the packed rows ``q`` over their
     requests' pages and, as ``row_mask`` says (None: causally), each other.
     ``workspace``: a zero-filled CUDA tensor of at least
-    paged_attend_workspace_bytes() bytes, or None."""
+    paged_attend_workspace_bytes() bytes, one for each stream and graph, or
+    None (the calling thread's; in a captured call the graph's own)."""
     dev, p = _pool(pool)
     n, rows, width = seq_lens.numel(), q.shape[0], p[4] * 64
     if q.dtype != pool.dtype:
