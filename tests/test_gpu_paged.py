@@ -687,6 +687,41 @@ def test_graphs_without_a_workspace(W, kind):
             assert torch.equal(o, want)
 
 
+CONCURRENT = {
+    "cut": lambda: Batch(90, "f16", [700, 30, 1801, 77] * 12, [20, 3, 7, 33] * 12, 6, 64),
+    "bf16": lambda: Batch(91, "bf16", [70, 204, 76] * 30, [1, 2, 17] * 30, 20, 48),
+    "f32": lambda: Batch(92, "f32", [70, 204, 1000] * 8, [1, 20, 7] * 8, 6, 16),
+    "taken": lambda: many(93, "bf16"),
+    "wide": lambda: wide_batch(94, [600, 20, 0, 1030], [150, 190, 1, 131], 8, 32),
+}
+
+
+@pytest.mark.parametrize("kind", CONCURRENT)
+def test_repeats_beside_another_kernel(W, kind):
+    """The same call 200 times while attention of its own runs on another stream."""
+    import torch
+    b = CONCURRENT[kind]()
+    a = dict(zip(("block_table", "seq_lens", "row_start", "row_mask"), b.device()))
+    want = torch.zeros(b.max_rows, b.heads * 64, device="cuda")
+    W.paged_attend(b.pool, 0, q=b.q, o=want, **a)
+    x = torch.randn(4 * 700 * 384, device="cuda").half()
+    y = torch.empty_like(x)
+    ws = torch.zeros(max(16, W.paged_attend_workspace_bytes(len(b.lens), b.max_rows, b.heads)),
+                     dtype=torch.uint8, device="cuda")
+    o, differ = torch.empty_like(want), torch.zeros((), dtype=torch.int64, device="cuda")
+    side, main = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(200):
+        W.attention_fwd(x, x, x, y, batch=4, t_q=700, t_kv=700, n_heads=6, scale=0.125, stream=side)
+        with torch.cuda.stream(main):
+            o.copy_(want)
+            o[:int(b.start[-1])] = 0
+            W.paged_attend(b.pool, 0, q=b.q, o=o, workspace=ws, **a)
+            differ += (o != want).any()
+    torch.cuda.synchronize()
+    assert int(differ) == 0
+
+
 def test_repeats_are_bit_exact(W):
     rng = np.random.default_rng(40)
     new = [20, 1, 33, 64]
