@@ -19,7 +19,7 @@
 // Many small items (a step of beams: 448 requests x 12 heads) are not cut but
 // taken one by one from a counter: the warps of an SM share what it can read,
 // so equal shares end unequally, and taken ones even that out. 361 MB of keys
-// and values: 73 us (4.9 TB/s) against 87.5 in equal shares.
+// and values: 71 us (5.1 TB/s) against 87.5 in equal shares.
 #include <algorithm>
 
 #include "paged_attend.cuh"
@@ -444,7 +444,8 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
         }
       }
     }
-    float mu[MT][2];
+    float mu[MT][2], mc[MT][2];
+    bool grows = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -455,9 +456,20 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
         for (int nb = 0; nb < 4; ++nb) mx = fmax3(mx, sc[mt][nb][2 * h], sc[mt][nb][2 * h + 1]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mc = mx * p.scale_log2;
-        if (mc > a[mt].m[h] + 8.0f) {  // rescale only when the running max grows by more than 2^8
-          const float alpha = ex2(a[mt].m[h] - mc);
+        mc[mt][h] = mx * p.scale_log2;
+        grows |= mc[mt][h] > a[mt].m[h] + 8.0f;
+      }
+    }
+    // (one branch for all rows: with four, trees of 64 rows over 32768 tokens take 5 % longer)
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 1 && few) break;
+          // rescale only when the running max grows by more than 2^8
+          if (!(mc[mt][h] > a[mt].m[h] + 8.0f)) continue;
+          const float alpha = ex2(a[mt].m[h] - mc[mt][h]);
           a[mt].l[h] *= alpha;
 #pragma unroll
           for (int db = 0; db < 8; ++db) {
@@ -468,11 +480,13 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
               a[0].o[db][3] *= alpha;
             }
           }
-          a[mt].m[h] = mc;
+          a[mt].m[h] = mc[mt][h];
         }
-        mu[mt][h] = a[mt].m[h] == -INFINITY ? 0.f : a[mt].m[h];
-      }
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) mu[mt][h] = a[mt].m[h] == -INFINITY ? 0.f : a[mt].m[h];
     // Value rows behind the last position hold anything: zero for the
     // product. A draft's value that is infinite or NaN belongs to the rows
     // that see it and would, as 0 times it, spoil those that do not.
@@ -538,15 +552,13 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
         }
       }
     }
-#pragma unroll
+    // (Not unrolled: a third of the body is this loop's, and the warps of an SM
+    // run three bodies: trees of up to 33 rows over 448 tokens 38 us against 43.)
+#pragma unroll 1
     for (int sl = 0; sl < 2; ++sl) {
       uint32_t vr[4][4];
 #pragma unroll
-      for (int d2 = 0; d2 < 4; ++d2) {
-        const uint32_t at = vtile + (voff ^ (d2 * 32));
-        if (sl == 0) pa_ldsm_t<0>(at, vr[d2]);
-        else pa_ldsm_t<2048>(at, vr[d2]);
-      }
+      for (int d2 = 0; d2 < 4; ++d2) pa_ldsm_t<0>(vtile + sl * 2048 + (voff ^ (d2 * 32)), vr[d2]);
       if (special) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -570,7 +582,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
         uint32_t pa[4], pr[4];
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2) {
-          const float *x = sc[mt][sl * 2 + n2];
+          const float *x = sc[mt][n2];
           const float e0 = ex2(fmaf(x[0], p.scale_log2, -mu[mt][0]));
           const float e1 = ex2(fmaf(x[1], p.scale_log2, -mu[mt][0]));
           a[mt].l[0] += e0 + e1;
@@ -609,6 +621,10 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
             pa_mma<T>(a[mt].o[db], pr, vr[db >> 1][(db & 1) * 2], vr[db >> 1][(db & 1) * 2 + 1]);
         }
       }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[mt][e >> 2][e & 3] = sc[mt][2 + (e >> 2)][e & 3];
     }
     __syncwarp();  // every lane has read the stage
     if (lane == 0) mbar_arrive(&s.empty[warp][slot]);
