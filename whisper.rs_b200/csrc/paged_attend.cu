@@ -651,19 +651,32 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
 // ---------------------------------------------------------------- f32 pools
 //
 // The same walk with 16-key stages and tiles of 16 rows on tf32 products,
-// three for each: every operand enters as x = hi + lo, hi its upper 11
-// significant bits and lo those of the rest, and hi hi + hi lo + lo hi leaves
-// out 2^-22 of each product at most.
+// three for each: every operand enters as x = hi + lo, 11 significant bits
+// each, and hi hi + hi lo + lo hi leaves out 2^-21 of each product at most.
 WATTN_DEVINL void pa_mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-WATTN_DEVINL void pa_split(float x, uint32_t &hi, uint32_t &lo) {
-  constexpr uint32_t kTf32 = 0xffffe000u;  // sign, exponent, 10 bits
-  hi = __float_as_uint(x) & kTf32;
+constexpr uint32_t kTf32 = 0xffffe000u;  // sign, exponent, 10 bits
+// x to its nearest such (finite x stay finite; FAR: x may be near the largest).
+template <bool FAR> WATTN_DEVINL uint32_t pa_tf32(float x) {
+  const uint32_t u = __float_as_uint(x);
+  if (!FAR) return (u + 0x1000u) & kTf32;
+  return (min((u & 0x7fffffffu) + 0x1000u, 0x7f7fffffu) & kTf32) | (u & 0x80000000u);
+}
+// Queries, keys and weights are split to nearest, so that lo has either sign
+// and what is left out of the products does not add up; values, of any size
+// where they are masked, cut off and their lo to nearest. (Cut off throughout,
+// scores and outputs come out too small: 1.1e-6 of the output against 5e-7.)
+template <bool FAR> WATTN_DEVINL void pa_split(float x, uint32_t &hi, uint32_t &lo) {
+  hi = pa_tf32<FAR>(x);
   lo = __float_as_uint(x - __uint_as_float(hi)) & kTf32;
+}
+WATTN_DEVINL void pa_split_value(float x, uint32_t &hi, uint32_t &lo) {
+  hi = __float_as_uint(x) & kTf32;
+  lo = pa_tf32<false>(x - __uint_as_float(hi));
 }
 WATTN_DEVINL float4 pa_lds(uint32_t addr) {
   float4 v;
@@ -693,10 +706,10 @@ WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, cons
         x = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p.q) +
                                               (int64_t)(it.row0 + r) * p.q_rs + it.head * 64 +
                                               (c >> 1) * 32 + 8 * t4 + (c & 1) * 4);
-      pa_split(x.x, qh[2 * c][h], ql[2 * c][h]);
-      pa_split(x.y, qh[2 * c][2 + h], ql[2 * c][2 + h]);
-      pa_split(x.z, qh[2 * c + 1][h], ql[2 * c + 1][h]);
-      pa_split(x.w, qh[2 * c + 1][2 + h], ql[2 * c + 1][2 + h]);
+      pa_split<true>(x.x, qh[2 * c][h], ql[2 * c][h]);
+      pa_split<true>(x.y, qh[2 * c][2 + h], ql[2 * c][2 + h]);
+      pa_split<true>(x.z, qh[2 * c + 1][h], ql[2 * c + 1][h]);
+      pa_split<true>(x.w, qh[2 * c + 1][2 + h], ql[2 * c + 1][2 + h]);
     }
   PaTile a;
 #pragma unroll
@@ -727,8 +740,8 @@ WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, cons
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
           uint32_t h0, l0, h1, l1;
-          pa_split(pair ? x[nb].z : x[nb].x, h0, l0);
-          pa_split(pair ? x[nb].w : x[nb].y, h1, l1);
+          pa_split<true>(pair ? x[nb].z : x[nb].x, h0, l0);
+          pa_split<true>(pair ? x[nb].w : x[nb].y, h1, l1);
           pa_mma_tf32(sc[nb], qh[2 * c + pair], h0, h1);
           pa_mma_tf32(sx[nb], qh[2 * c + pair], l0, l1);
           pa_mma_tf32(sy[nb], ql[2 * c + pair], h0, h1);
@@ -826,13 +839,13 @@ WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, cons
       for (int e = 0; e < 4; ++e) {  // row g + 8 (e & 1), key 2 t4 + (e >> 1)
         const float w = ex2(fmaf(sc[nb][2 * (e & 1) + (e >> 1)], p.scale_log2, -mu[e & 1]));
         a.l[e & 1] += w;
-        pa_split(w, ph[e], pl[e]);
+        pa_split<false>(w, ph[e], pl[e]);
       }
       uint32_t vh[2][8], vl[2][8];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pa_split(v[b][i], vh[b][i], vl[b][i]);
+        for (int i = 0; i < 8; ++i) pa_split_value(v[b][i], vh[b][i], vl[b][i]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], ph, vh[0][i], vh[1][i]);
 #pragma unroll
