@@ -739,8 +739,8 @@ WIDE = 2 * 7.5e-5
 WIDE_SHAPES = [
     # lens, new, heads, page_rows
     ([600], [128], 1, 64), ([0, 700, 33], [260, 2, 130], 3, 64), ([1500, 511], [129, 127], 2, 48),
-    ([513] * 3, [112] * 3, 5, 16), ([5000], [224], 2, 128), ([900, 0, 0, 0], [640, 0, 1, 3], 2, 32),
-    ([400] * 10, [115] * 10, 12, 64), ([127, 128, 129], [128, 384, 127], 2, 32),
+    ([513] * 3, [112] * 3, 5, 16), ([5000], [224], 2, 128), ([900, 0, 0, 0], [500, 0, 1, 3], 2, 32),
+    ([400] * 10, [115] * 10, 12, 64), ([127, 700, 129], [256, 100, 20], 2, 32),
 ]
 
 
@@ -748,7 +748,8 @@ def wide_batch(seed, lens, new, heads, page_rows, kind="tree", dead=0.0, **kw):
     rng = np.random.default_rng(seed)
     par = sum((tree(rng, k, dead) for k in new), []) if kind == "tree" else None
     b = Batch(seed, "f16", lens, new, heads, page_rows, par, words=-(-max(new) // 32), **kw)
-    assert b.max_rows >= 112 * len(lens) and b.st.table.shape[1] * page_rows >= 512
+    rows = b.max_rows // len(lens)  # the rule by which the kernel for many rows is chosen
+    assert rows * 8 >= 7 * 128 * ((rows + 119) // 128) and b.st.table.shape[1] * page_rows - rows >= 448
     return b
 
 
@@ -772,8 +773,8 @@ def test_wide_random(W, seed):
     n = int(rng.integers(1, 8))
     lens = (2 ** rng.uniform(0, 10, n)).astype(int) - 1
     lens[0] = 600
-    new = np.where(rng.random(n) < .2, 0, rng.integers(1, 300, n))
-    new[-1] += max(0, 112 * n - int(new.sum()))
+    new = np.where(rng.random(n) < .2, 0, rng.integers(1, 130, n))
+    new[-1] += 120 * n - int(new.sum())
     b = wide_batch(2100 + seed, lens, new, int(rng.integers(1, 6)), int(rng.choice([16, 32, 48, 64, 80, 128])),
                    "tree" if seed % 3 else "chain", 0.05, stride=int(rng.integers(0, 3)) * 8)
     b.check(W, out="f32" if seed % 2 else "f16", stride=int(rng.integers(0, 3)) * 8, more=WIDE)
@@ -826,7 +827,7 @@ def test_wide_rows_that_see_nothing_are_zero(W):
 
 
 def test_wide_large_scores(W):
-    b = wide_batch(64, [600, 10], [200, 130], 2, 64, "chain")
+    b = wide_batch(64, [600, 10], [200, 60], 2, 64, "chain")
     b.pool *= 20
     b.q *= 20
     got = b.attend(W, 1, "f32")

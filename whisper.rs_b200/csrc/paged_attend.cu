@@ -39,13 +39,20 @@ constexpr int kPaCtasPerSm = 2;
 // warpgroups' split (whose sum may not exceed twice the launch's).
 constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
 static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
-// New rows of a request, averaged over the row buffer (the counts themselves
-// are on the device), and positions that a request may hold, from which the
-// wide kernel is the faster one. f16, wide / narrow: 16 requests of 8 heads,
-// 4096 cached, 96 rows 71 us / 83, 128 rows 70 / 107, 256 rows 113 / 193; 16
-// heads, 500 cached, 128 rows 47 / 53; but 1000 cached, 96 rows 64 / 58, and
-// 32 requests of 20 heads with nothing cached, 128 rows 44 / 37.
-constexpr int kPaWideRows = 112, kPaWideKeys = 512;
+// Whether the wide kernel is the faster one, from what the host knows: the
+// rows of a request, averaged over the row buffer, fill tiles of 128 to 7/8
+// (8 rows of padding aside), over this many cached positions. f16, wide /
+// narrow: 16 requests of 8 heads, 4096 cached: 64 rows 66 us / 74, 112 rows 70
+// / 96, 128 rows 70 / 104, 160 rows 111 / 129, 256 rows 111 / 188. 16 requests
+// of 16 heads: 500 cached, 96 rows 47 / 41, 112 rows 45 / 55, 128 rows 47 / 53,
+// 160 rows 86 / 59, 256 rows 88 / 94; 2000 cached, 96 rows 84 / 84, 112 rows 80
+// / 111, 160 rows 137 / 129, 224 rows 158 / 174. 64 requests of 20 heads, 300
+// cached, 128 rows 129 / 119; 32 of them, nothing cached, 45 / 35.
+constexpr int kPaWideKeys = 448;
+inline bool pa_wide(int64_t max_rows, int n_seqs, int cap) {
+  const int64_t rows = max_rows / n_seqs, tiles = (rows + 119) / 128;
+  return tiles > 0 && rows * 8 >= tiles * 128 * 7 && cap - rows >= kPaWideKeys;
+}
 constexpr int kPaMergeAll = 8;    // CTAs beyond the first from which all warps merge an item
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
@@ -553,7 +560,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
       }
     }
     // (Not unrolled: a third of the body is this loop's, and the warps of an SM
-    // run three bodies: trees of up to 33 rows over 448 tokens 38 us against 43.)
+    // run three bodies: trees of up to 33 rows over 448 tokens 39 us against 43.)
 #pragma unroll 1
     for (int sl = 0; sl < 2; ++sl) {
       uint32_t vr[4][4];
@@ -885,8 +892,8 @@ WATTN_DEVINL void pa_gather(const PagedAttendParams &p, PaTile &a, int c0, int c
 // The items cut by the shares of this CTA's warps, after all of them are
 // done: the CTA's parts of an item are merged, an item per warp, and where
 // several CTAs have parts the last of them to arrive merges theirs. (A few
-// by the same warp: 41 us against 44 us with all warps for trees of 33 rows
-// over 448 tokens; many with all: 81,000 cycles to 68,000 for one request of
+// by the same warp: with all warps trees of 33 rows over 448 tokens take 7 %
+// longer; many with all: 81,000 cycles to 68,000 for one request of
 // 32768 tokens, whose heads lie in 37 CTAs each.)
 template <typename T, typename OutT>
 WATTN_DEVINL void pa_finish(const PagedAttendParams &p, PaSmem<T> &s, int warp, int lane) {
@@ -1088,7 +1095,7 @@ int launch_stream(const PagedAttendParams &p, int dtype, cudaStream_t st) {
 
 int launch_attend(const PagedAttendParams &p, int dtype, int out_dtype, cudaStream_t st) {
   if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
-  if (dtype == WATTN_F16 && p.max_rows >= (int64_t)kPaWideRows * p.n_seqs && p.cap >= kPaWideKeys)
+  if (dtype == WATTN_F16 && pa_wide(p.max_rows, p.n_seqs, p.cap))
     return launch_paged_attend_wide(p, out_dtype, st);
   if (dtype == WATTN_F16)
     return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
