@@ -184,7 +184,9 @@ WATTN_DEVINL void plan_padding(const PlanParams &p, long long r) {
 }
 
 // The plan, by one cluster of up to eight CTAs (bound by latency: three
-// dependent passes over the requests). Each CTA has a run of the requests.
+// dependent passes over the requests; 5.4 us for 320 requests of one row, 13 us
+// for 2048 requests with 16,000 pages, of which 229,000 rows take 7 more in a
+// launch of their own). Each CTA has a run of the requests.
 // First all are checked, so that a refused plan changes nothing; then pages
 // are given back to the stack, then taken from it, then the rows are filled
 // in. The g-th page given back (in the order of requests and of pages) lands
@@ -330,7 +332,8 @@ struct WriteParams {
 };
 
 // One thread per 8 elements of a row's keys and of its values: 16 bytes of a
-// 16-bit pool. VEC: the source rows are 16-byte aligned. Bound: HBM.
+// 16-bit pool. VEC: the source rows are 16-byte aligned. Bound: HBM (64
+// prompts of up to 224 rows x 1280, f32 into bf16, 121 MB: 20.3 us, 6.0 TB/s).
 template <typename T> WATTN_DEVINL void load8(const T *src, float (&f)[8]) {
   if constexpr (sizeof(T) == 4) {
     const float4 a = reinterpret_cast<const float4 *>(src)[0];
@@ -448,7 +451,9 @@ struct AcceptSmem {
 // token is the one picked at its parent, until there is none, and moves its
 // columns of the accepted rows. Path rows ascend and row j of the path lands
 // at or before its own place, so no store overwrites what a later load of
-// the same column reads. Bound: latency for a few requests, then HBM.
+// the same column reads. Bound: latency for a few requests (6.4 us for one of
+// 16 drafts), then HBM (32 requests of up to 64 drafts in 32 layers of 20
+// heads, 25 MB moved: 11.9 us, the walk included).
 __global__ void __launch_bounds__(kAcceptThreads) paged_accept_kernel(const AcceptParams p) {
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
