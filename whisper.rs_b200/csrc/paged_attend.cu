@@ -424,7 +424,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
       pa_ldsm<0>(at, r[0]);
       pa_ldsm<1024>(at, r[1]);
       pa_ldsm<2048>(at, r[2]);
-      pa_ldsm<3072>(at, r[3]);
+      pa_ldsm<3 * 1024>(at, r[3]);
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
