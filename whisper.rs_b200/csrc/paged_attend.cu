@@ -799,6 +799,12 @@ WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, cons
       }
       mu[h] = a.m[h] == -INFINITY ? 0.f : a.m[h];
     }
+    // The stage's own sums: the tensor cores cut off what they add up, which
+    // makes the outputs too small (one request of 32768 tokens: by 1.0e-6 of
+    // their size, with sums of their own 4.2e-7).
+    float o[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
       // two value rows, of keys 2 t4 and 2 t4 + 1, in column g of the 8 tiles
@@ -860,12 +866,16 @@ WATTN_DEVINL void pa_item_f32(const PagedAttendParams &p, PaSmem<float> &s, cons
 #pragma unroll
         for (int i = 0; i < 8; ++i) pa_split_value(v[b][i], vh[b][i], vl[b][i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], ph, vh[0][i], vh[1][i]);
+      for (int i = 0; i < 8; ++i) pa_mma_tf32(o[i], ph, vh[0][i], vh[1][i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], ph, vl[0][i], vl[1][i]);
+      for (int i = 0; i < 8; ++i) pa_mma_tf32(o[i], ph, vl[0][i], vl[1][i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) pa_mma_tf32(a.o[i], pl, vh[0][i], vh[1][i]);
+      for (int i = 0; i < 8; ++i) pa_mma_tf32(o[i], pl, vh[0][i], vh[1][i]);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a.o[i][e] += o[i][e];
     __syncwarp();  // every lane has read the stage
     if (lane == 0) mbar_arrive(&s.empty[warp][slot]);
   }
