@@ -421,7 +421,7 @@ int wattn_paged_write(void *pool, int dtype, int n_pages, int n_layers, int n_he
  * NaN. A table entry outside the pool, lengths beyond max_pages pages or row
  * starts outside [0, max_rows] make that request's rows unspecified, and
  * wattn_device_status() reports WATTN_ERR_RANGE; so does a call of 2^31 units
- * of work or more (about three for every 16 keys of each head and tile of 16
+ * of work or more (about five for every 16 keys of each head and tile of 16
  * rows), which writes no rows. workspace as for wattn_decode_fwd
  * (wattn_paged_attend_workspace_bytes(), zero-filled before its first use),
  * or NULL. Calls that may overlap, captured graphs among them, need one each;

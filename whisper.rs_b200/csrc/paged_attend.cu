@@ -23,8 +23,8 @@
 //
 // Elsewhere the chain of one stage bounds (scores, maximum, weights, products,
 // with eight compute warps on an SM): 64 trees of up to 33 rows over up to 448
-// tokens, 20 heads, f16 39 us (82 MB); 8 trees of up to 64 rows over up to
-// 32768 tokens, 8 heads, bf16 82 us (238 MB); one tree of 16 rows 10 us, of
+// tokens, 20 heads, f16 37 us (82 MB); 8 trees of up to 64 rows over up to
+// 32768 tokens, 8 heads, bf16 77 us (238 MB); one tree of 16 rows 11 us, of
 // which 3 are the launch.
 #include <algorithm>
 
@@ -64,8 +64,9 @@ constexpr int kPaQueue = 8;       // items a warp may have loads for, and one mo
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
 static_assert(kPaStages * kPaStageBytes >= kPaWarps * kPaTileFloats * 4, "a ring holds the warps' sums");
 
-// A stage is 8 KB of keys and values. Units: measured, two tiles of 16 rows
-// cost half as much again as one.
+// A stage is 8 KB of keys and values. Units, measured: two tiles of 16 rows
+// cost a quarter more than one, an item as much as three stages (with 2, 3 and
+// 2 units trees of 64 rows over 32768 tokens take 82 us instead of 77).
 struct PaShape {
   static constexpr int kShares = kPaWarps, kThreads = kPaThreads;
   // Items to a compute warp from which they are taken one by one (cached
@@ -73,8 +74,8 @@ struct PaShape {
   // heads 68.6 us / 76.8, 600 88.3 / 103.4, 300 of 20 heads and 40 new rows
   // 235 / 273; of 200 or 300 requests of 12 heads the lookup alone costs 2 us).
   static constexpr int kQueueItems = 4;
-  static constexpr int kStageUnits = 2, kWideUnits = 3, kItemUnits = 2;
-  static constexpr int kMinUnits = 8;  // units of a share below which fewer warps work
+  static constexpr int kStageUnits = 4, kWideUnits = 5, kItemUnits = 12;
+  static constexpr int kMinUnits = 16;  // units of a share below which fewer warps work
 };
 template <typename T> struct PaType;
 template <> struct PaType<__half> : PaShape {
@@ -89,6 +90,7 @@ template <> struct PaType<__nv_bfloat16> : PaShape {
 };
 template <> struct PaType<float> : PaShape {
   static constexpr int kKeys = 16, kRows = 16;
+  static constexpr int kMinUnits = 8;  // (16 requests of 13 rows over 448 tokens: 14.5 us, with 16 17.1)
 };
 
 template <typename T>

@@ -86,6 +86,8 @@ struct PaShares {
 template <typename C> WATTN_DEVINL PaShares pa_shares(int total, int max_parts) {
   PaShares s;
   s.parts = max(1, min(max_parts, total / C::kMinUnits));
+  // (whole CTAs: then a few items of one size are cut alike, and merged in one)
+  if (s.parts > C::kShares) s.parts -= s.parts % C::kShares;
   s.size = total / s.parts;
   s.more = total - s.size * s.parts;
   return s;
