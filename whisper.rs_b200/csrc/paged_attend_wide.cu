@@ -361,6 +361,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
           for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
           tmem_st32(t_o + 32 * h, o);
         }
+        if (special) tmem_wait_st();  // (below, O may be read back)
       }
       if (special) {
         // Thread k has value row k of the tile: one behind the last position
