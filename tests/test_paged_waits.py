@@ -1,0 +1,23 @@
+"""Waits of the device-planned cache's kernels, checked in their source: a
+bounded wait that runs out cannot be caused in them without a fault, so what
+keeps their warps from waiting for one another for ever is read here."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "whisper.rs_b200", "csrc")
+
+
+def source(name):
+    text = open(os.path.join(CSRC, name)).read()
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def test_softmax_warps_meet_with_a_limit():
+    """The wide kernel's softmax warps leave one by one where a wait runs out:
+    none may wait for the others at a barrier without a limit."""
+    text = source("paged_attend_wide.cu")
+    assert not re.search(r"\bbar(rier)?(\.cta)?\.(sync|red)", text)
+    body = text[text.index("void pw_softmax("):text.index("paged_attend_wide_kernel(")]
+    assert "__syncthreads" not in body
+    calls = re.findall(r"[^\n]*\bpw_sync\([^\n]*", body)
+    assert len(calls) == 6 and all(re.match(r"\s*if \(!pw_sync\(.*\) return;", c) for c in calls)

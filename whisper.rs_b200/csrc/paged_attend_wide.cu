@@ -61,7 +61,7 @@ struct PwSmem {
   uint64_t q_full, k_full[kPwK], k_empty[kPwK], v_full[kPwV], v_empty[kPwV];
   uint64_t s_full, s_free, p_full, o_done;
   uint64_t item_full[kPwQueue], item_empty[kPwQueue];
-  uint64_t drain, done;
+  uint64_t drain, done, meet;
   PaItem queue[kPwQueue];
   PaFind<PwShape> find;
   uint32_t odd[4];  // keys of a tile with values that are infinite or NaN
@@ -71,8 +71,14 @@ struct PwSmem {
 
 #define PW_SITE(role, what) ((5 << 24) | ((role) << 16) | ((what) << 8))
 
-// Barrier of the softmax warps.
-WATTN_DEVINL void pw_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Barrier of the softmax warps, `count` (of such barriers so far) being the
+// same in all of them. Bounded like all waits (a warp that gave up elsewhere
+// does not come): false if it ran out.
+WATTN_DEVINL bool pw_sync(const PagedAttendParams &p, PwSmem &s, uint32_t &count) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(&s.meet);
+  return __all_sync(0xffffffffu, mbar_wait(&s.meet, count++ & 1, &s.abort, p.status, PW_SITE(2, 5)));
+}
 
 // ---------------------------------------------------------------- load warp
 
@@ -251,7 +257,8 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
   const int wq = tid >> 5, lane = tid & 31;
   const int r = tid;  // row of the tile
   const uint32_t t_s = tmem + (uint32_t(wq * 32) << 16), t_p = t_s + 128, t_o = t_s + 192;
-  uint32_t n = 0;  // tiles so far
+  uint32_t n = 0;      // tiles so far
+  uint32_t met = 0;    // barriers of the softmax warps
 #pragma unroll 1
   for (uint32_t i = 0;; ++i) {
     const int islot = i % kPwQueue;
@@ -388,7 +395,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
         }
         const uint32_t flags = __ballot_sync(0xffffffffu, odd);
         if (lane == 0) s.odd[wq] = flags;
-        pw_sync();
+        if (!pw_sync(p, s, met)) return;
         if ((s.odd[0] | s.odd[1] | s.odd[2] | s.odd[3]) != 0) {
           if (warp_has) {
 #pragma unroll 1
@@ -414,14 +421,14 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
               tmem_st32(t_o + 32 * h, o);
             }
           }
-          pw_sync();  // all have read the values
+          if (!pw_sync(p, s, met)) return;  // all have read the values
           if (odd) {
             uint32_t *w = reinterpret_cast<uint32_t *>(vrow);
             for (int e = 0; e < 32; ++e) w[e] &= ~__vcmpeq2(w[e] & kInf2, kInf2);
           }
         }
         fence_proxy_async_smem();
-        pw_sync();  // (s.odd is used again; and the tile is clean for the product)
+        if (!pw_sync(p, s, met)) return;  // (s.odd is used again; and the tile is clean for the product)
       }
       if (warp_has) {
 #pragma unroll
@@ -466,7 +473,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
       part[64 * 128] = m;
       part[65 * 128] = l;
     }
-    pw_sync();
+    if (!pw_sync(p, s, met)) return;
     if (tid == 0) {
       // Release: the barrier orders the threads' partials before this
       // fence, and the fence orders them before the count.
@@ -477,7 +484,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
         p.count[c0] = 0;  // zeroed for the next call
       }
     }
-    pw_sync();
+    if (!pw_sync(p, s, met)) return;
     if (s.last && mine) {
       float M = -INFINITY, L = 0.f;
 #pragma unroll
@@ -495,7 +502,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
       }
       pw_store_row<OutT>(p, o, L == 0.f ? 0.f : __fdividef(1.f, L), it.row0 + r, it.head);
     }
-    pw_sync();  // s.last is used again
+    if (!pw_sync(p, s, met)) return;  // s.last is used again
   }
 }
 
@@ -529,6 +536,7 @@ __global__ void __launch_bounds__(kPwThreads, kPwCtasPerSm)
     }
     mbar_init(&s.drain, 1);
     mbar_init(&s.done, 128);
+    mbar_init(&s.meet, 4);
     s.abort = 0;
     fence_barrier_init();
   }
