@@ -21,3 +21,16 @@ def test_softmax_warps_meet_with_a_limit():
     assert "__syncthreads" not in body
     calls = re.findall(r"[^\n]*\bpw_sync\([^\n]*", body)
     assert len(calls) == 6 and all(re.match(r"\s*if \(!pw_sync\(.*\) return;", c) for c in calls)
+
+
+def test_lanes_leave_together():
+    """Where a wait's result decides what a whole warp does next, all its lanes
+    vote: it may run out for some of them only."""
+    text = source("paged_attend.cu")
+    assert len(re.findall(r"\bif \(!__all_sync\(0xffffffffu, mbar_wait\(", text)) == 1
+    assert not re.search(r"\bif \(!mbar_wait\(", text)
+    wide = source("paged_attend_wide.cu")
+    softmax = wide[wide.index("void pw_softmax("):wide.index("paged_attend_wide_kernel(")]
+    load = wide[wide.index("void pw_load("):wide.index("void pw_products(")]
+    for body in (softmax, load):
+        assert "mbar_wait(" in body and not re.search(r"\bif \(!mbar_wait\(", body)
