@@ -4,7 +4,7 @@ larger than the step, and what the device status word says of whom."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_paged import WIDE, W, bound, clean_status, wide_batch  # noqa: F401
+from tests.test_gpu_paged import WIDE, W, bound, clean_status, cu, tdt, wide_batch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +79,30 @@ def test_wide_value_that_is_not_finite_where_the_maximum_grows(W, value):
     got[hit, 64 + 37] = o[hit, 64 + 37]
     lim = bound("f16", "f32", o, mag, top, 1128, 6.0) + WIDE * mag
     assert (np.abs(got - o) <= lim).all()
+
+
+# ------------------------------------------------------------------ sizes
+
+@pytest.mark.parametrize("dtype,rows", [("f16", 130), ("f16", 3), ("bf16", 130), ("f32", 3)])
+def test_lengths_near_2_31(W, dtype, rows):
+    """A table of 2^31 positions and a length close to them: out of range, and
+    the other request's rows are written."""
+    import torch
+    P_, heads, ln = 4096, 2, 600
+    g = torch.Generator(device="cuda").manual_seed(69)
+    pool = torch.randn(2, 1, 2, heads, P_, 64, generator=g, device="cuda").to(tdt(dtype))
+    table = torch.zeros(2, (1 << 31) // P_, dtype=torch.int32, device="cuda")
+    table[0, 0] = 1
+    q = torch.randn(2 * rows, heads * 64, generator=g, device="cuda").to(tdt(dtype))
+    o = torch.full((2 * rows, heads * 64), 7.0, device="cuda")
+    W.paged_attend(pool, 0, table, cu(np.array([ln, 2 ** 31 - 1 - 64 - rows])),
+                   cu(np.array([0, rows, 2 * rows])), q, o)
+    torch.cuda.synchronize()
+    assert W.device_status() == -6
+    assert (o[rows:] == 7).all()
+    kv = pool[1, 0, :, :, :ln + rows].double()
+    z = torch.einsum("nhd,hkd->hnk", q[:rows].double().view(rows, heads, 64), kv[0]) / 8
+    z.masked_fill_(torch.arange(ln + rows, device="cuda") > ln + torch.arange(rows, device="cuda")[:, None],
+                   -torch.inf)
+    ref = torch.einsum("hnk,hkd->nhd", torch.softmax(z, -1), kv[1]).reshape(rows, -1)
+    assert float((o[:rows] - ref).abs().max()) <= (1e-5 if dtype == "f32" else 2e-3)

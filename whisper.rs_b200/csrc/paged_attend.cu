@@ -92,6 +92,7 @@ template <> struct PaType<float> : PaShape {
   static constexpr int kKeys = 16, kRows = 16;
   static constexpr int kMinUnits = 8;  // (16 requests of 13 rows over 448 tokens: 14.5 us, with 16 17.1)
 };
+static_assert(PaType<__half>::kKeys <= kPaMostKeys && PaType<float>::kKeys <= kPaMostKeys, "see kPaMostKeys");
 
 template <typename T>
 struct PaSmem {
@@ -1191,7 +1192,8 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.o_rs = o_row_stride;
   p.max_rows = max_rows;
   p.scale_log2 = scale * 1.4426950408889634f;
-  p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 64);
+  // (positions rounded up to a stage of either kernel stay within 32 bits)
+  p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 2 * kPaMostKeys);
   p.status = device_status_ptr();
   if (p.status == nullptr) return WATTN_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;

@@ -40,6 +40,7 @@ struct PagedAttendParams {
 };
 
 constexpr int kPaTail = 16;  // rows of a tail box: the pool's unit of page rows
+constexpr int kPaMostKeys = 128;  // keys of a stage, at most
 
 // One request as the kernel sees it. One whose arrays are out of range has
 // no rows here (and is reported).

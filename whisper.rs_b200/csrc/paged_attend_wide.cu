@@ -29,7 +29,7 @@ namespace wattn {
 
 namespace {
 
-constexpr int kPwKeys = 128;       // keys of a stage
+constexpr int kPwKeys = kPaMostKeys;  // keys of a stage
 constexpr int kPwTile = kPwKeys * 128;
 constexpr int kPwK = 2, kPwV = 3;  // ring depths
 constexpr int kPwThreads = 8 * 32;
