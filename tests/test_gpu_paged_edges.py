@@ -4,7 +4,7 @@ larger than the step, and what the device status word says of whom."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_paged import WIDE, W, bound, clean_status, cu, tdt, wide_batch  # noqa: F401
+from tests.test_gpu_paged import WIDE, Batch, W, bound, clean_status, cu, tdt, wide_batch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -79,6 +79,44 @@ def test_wide_value_that_is_not_finite_where_the_maximum_grows(W, value):
     got[hit, 64 + 37] = o[hit, 64 + 37]
     lim = bound("f16", "f32", o, mag, top, 1128, 6.0) + WIDE * mag
     assert (np.abs(got - o) <= lim).all()
+
+
+@pytest.mark.parametrize("dtype,wide", [("f16", True), ("f16", False), ("bf16", False), ("f32", False)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_key_that_is_not_finite_is_seen(W, dtype, wide, bad):
+    """One element of one draft's key, at each of nine neighbouring positions: a
+    row that sees it has a score that is NaN or +inf there and is NaN, or one
+    of -inf and does without that key; the others are as they were."""
+    lens, new = ([1000], [128]) if wide else ([70], [40])
+    b = wide_batch(67, lens, new, 2, 64, layers=1) if wide else Batch(
+        67, dtype, lens, new, 2, 64, [-1] + [max(0, i - 2) for i in range(1, new[0])], layers=1)
+    clean, mask = b.attend(W, 0, "f32"), b.mask.copy()
+    n_lost = n_without = 0
+    for j in range(3, 12):
+        page, row = place(b, 0, lens[0] + j)
+        keep = b.pool[page, 0, 0, 1, row, 5].clone()
+        b.pool[page, 0, 0, 1, row, 5] = bad
+        got = b.attend(W, 0, "f32")
+        sees = seen_by(b, 0)[:, j]
+        positive = (b.q[:new[0], 64 + 5] > 0).cpu().numpy()
+        lost = sees if bad != bad else sees & positive
+        n_lost += lost.sum()
+        assert not sees.all()
+        assert np.isnan(got[lost, 64:]).all(), j
+        same = ~sees
+        assert np.array_equal(got[same], clean[same])
+        assert np.array_equal(got[:, :64], clean[:, :64])
+        if bad == bad:  # without that key
+            without = sees & ~positive
+            b.pool[page, 0, 0, 1, row, 5] = keep
+            b.mask[:new[0], 0] &= ~np.int32(1 << j)
+            o, mag, top = formula(b, 0)
+            b.mask = mask.copy()
+            lim = bound(dtype, "f32", o, mag, top, 1200, 6.0) + (WIDE if wide else 0) * mag
+            n_without += without.sum()
+            assert (np.abs(got - o) <= lim)[without, 64:].all()
+        b.pool[page, 0, 0, 1, row, 5] = keep
+    assert n_lost > 0 and (n_without > 0 or bad != bad)
 
 
 # ------------------------------------------------------------------ sizes

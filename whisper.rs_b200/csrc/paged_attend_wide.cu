@@ -41,7 +41,10 @@ static_assert(kPwSoftmaxRegs + kPwOtherRegs <= 2 * kPwRegs, "a larger split neve
 constexpr int kPwCtasPerSm = 2;
 constexpr int kPwQueue = 2;        // items announced
 // One pair of exponentials in so many runs on the FMA pipe instead of the SFU
-// (7.5e-5 off at most, less than the weights' rounding to f16).
+// (7.5e-5 off at most, less than the weights' rounding to f16). The polynomial
+// does not give NaN for NaN, nor 0 for -inf but 2^-126: rows with such scores
+// are caught by their maximum, and 2^-126 is 0 in f16 and nothing in a sum that
+// has a key.
 constexpr int kPwFmaPairs = 4;
 constexpr uint32_t kPwCols = 256;  // TMEM: S 128, P 64, O 64
 constexpr int kPwPartFloats = 66 * 128;  // a partial: O [64][row], m, l
@@ -247,6 +250,13 @@ WATTN_DEVINL float *pw_part(const PagedAttendParams &p, int c, bool starts) {
   return p.part + ((int64_t)c * 2 + (starts ? 1 : 0)) * kPwPartFloats;
 }
 
+// max(a, b, c), NaN if one of them is.
+WATTN_DEVINL float pw_max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Which of 32 positions row r of the item's tile sees (pa_visible).
 WATTN_DEVINL uint32_t pw_visible(const PagedAttendParams &p, const PaItem &it, int r, int off, int left) {
   return left > 0 ? pa_visible(p, it.row0 + r, it.row + r, off, left) : 0u;
@@ -326,8 +336,8 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
 #pragma unroll
         for (int e = 0; e < 128; e += 8)
 #pragma unroll
-          for (int a = 0; a < 4; ++a) mx[a] = fmax3(mx[a], x(e + 2 * a), x(e + 2 * a + 1));
-        const float mc = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          for (int a = 0; a < 4; ++a) mx[a] = pw_max3(mx[a], x(e + 2 * a), x(e + 2 * a + 1));
+        const float mc = pw_max3(pw_max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * p.scale_log2;
         const bool need = mc > m + 8.0f;  // rescale only when the running max grows by more than 2^8
         rescale = __any_sync(0xffffffffu, need) && t > it.from;
         if (need) {
@@ -335,6 +345,9 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
           l *= alpha;
           m = mc;
         }
+        // A score that is NaN or +inf makes the row NaN (the polynomial below
+        // would take it for a small weight).
+        if (!(mc < INFINITY)) l = __int_as_float(0x7fffffff);
         const float mu = m == -INFINITY ? 0.f : m;
         const float2 c2 = make_float2(p.scale_log2, p.scale_log2), nmu2 = make_float2(-mu, -mu);
         float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
