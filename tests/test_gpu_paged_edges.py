@@ -119,6 +119,43 @@ def test_a_key_that_is_not_finite_is_seen(W, dtype, wide, bad):
     assert n_lost > 0 and (n_without > 0 or bad != bad)
 
 
+# ------------------------------------------------------------------ what 16-bit weights keep
+
+TAIL_KEYS = 131072
+
+
+@pytest.mark.parametrize("rows", [1, 12, 20, 128])
+def test_a_flat_tail_keeps_its_weight(W, rows):
+    """One key that outweighs each of 131072 others 2^25.5 times, whose values
+    are small where theirs are not: theirs are the output. (Requests of the
+    same pages, as many as give each share of the work a whole request's keys.)
+
+    Weights in f16 relative to 2^-7 of the largest: 2^-18.5 in steps of 2^-24,
+    off by 2^-6.5 of themselves at most and all alike; the sums of 131072 of
+    them on the tensor cores, which cut off, by 8192 * 2^-23."""
+    import torch
+    heads, page_rows, n = 8, 128, 40 if rows > 64 else 160
+    pages = TAIL_KEYS // page_rows + 1
+    pool = torch.zeros(pages, 1, 2, heads, page_rows, 64, dtype=torch.float16, device="cuda")
+    c = (0.5 + torch.arange(64, device="cuda") / 64).half()
+    pool[:, :, 1] = c
+    sink = 25.5 * float(np.log(2.0))
+    pool[0, 0, 0, :, 0, 0] = sink
+    pool[0, 0, 1, :, 0] = 0
+    q = torch.zeros(n * rows, heads, 64, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 8
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(n, pages).contiguous()
+    o = torch.empty(n * rows, heads * 64, device="cuda")
+    W.paged_attend(pool, 0, table, cu(np.full(n, TAIL_KEYS)), cu(np.arange(n + 1) * rows),
+                   q.view(n * rows, heads * 64), o)
+    r = float(np.exp(-float(pool[0, 0, 0, 0, 0, 0])))
+    tail = torch.arange(TAIL_KEYS, TAIL_KEYS + rows, device="cuda").double().repeat(n)[:, None, None] * r
+    want = (tail / (1 + tail) * c.double()).expand(n * rows, heads, 64).reshape(n * rows, -1)
+    assert 2e-3 < float(want.max()) < 6e-3
+    err = (o.double() - want).abs()
+    assert float((err / want).max()) <= 2.0 ** -6.5 + 2.0 ** -10 + 2 * 7.5e-5 + 2.0 ** -16
+
+
 # ------------------------------------------------------------------ sizes
 
 @pytest.mark.parametrize("dtype,rows", [("f16", 130), ("f16", 3), ("bf16", 130), ("f32", 3)])

@@ -82,11 +82,13 @@ template <> struct PaType<__half> : PaShape {
   static constexpr int kKeys = 32, kRows = 32;
   static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
   static constexpr bool kResidual = false;  // f16 weights: 2^-11 each, within the 2e-3 bar
+  static constexpr float kLower = kPaLower16;
 };
 template <> struct PaType<__nv_bfloat16> : PaShape {
   static constexpr int kKeys = 32, kRows = 32;
   static constexpr uint32_t kOne = 0x3f80u, kInf = 0x7f80u;
   static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
+  static constexpr float kLower = 0.f;      // (f32's range)
 };
 template <> struct PaType<float> : PaShape {
   static constexpr int kKeys = 16, kRows = 16;
@@ -178,7 +180,7 @@ template <typename OutT> WATTN_DEVINL void pa_store2(void *o, int64_t at, float 
 // A warp's 16 query rows over some keys: this lane's part of rows g and g + 8.
 struct PaTile {
   float o[8][4];     // dims 8 db + 2 t4 and + 1 of row g, then of row g + 8
-  float m[2], l[2];  // running max; sum of this lane's weights
+  float m[2], l[2];  // running max (less kLower); sum of this lane's weights
 };
 
 // Partials of cut items, in the lanes' layout: two slots per share (`starts`:
@@ -472,7 +474,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
         for (int nb = 0; nb < 4; ++nb) mx = fmax3(mx, sc[mt][nb][2 * h], sc[mt][nb][2 * h + 1]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mc[mt][h] = mx * p.scale_log2;
+        mc[mt][h] = fmaf(mx, p.scale_log2, -PaType<T>::kLower);
         grows |= mc[mt][h] > a[mt].m[h] + 8.0f;
       }
     }

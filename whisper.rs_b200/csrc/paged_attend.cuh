@@ -41,6 +41,12 @@ struct PagedAttendParams {
 
 constexpr int kPaTail = 16;  // rows of a tail box: the pool's unit of page rows
 constexpr int kPaMostKeys = 128;  // keys of a stage, at most
+// f16 weights are taken relative to a running maximum that is lowered by this
+// many powers of two: with the 2^8 that it may lag behind they reach 2^15, and
+// what is lost below f16's least (a weight under 2^-25, or up to 2^-25 of one
+// under 2^-14) is 2^-32 of the largest weight. Relative to the maximum itself it
+// would be 2^-25, and 131072 keys of such weights 2^-8 of the output.
+constexpr float kPaLower16 = 7.f;
 
 // One request as the kernel sees it. One whose arrays are out of range has
 // no rows here (and is reported).

@@ -10,8 +10,8 @@
 // registers, of which one warp loads (TMA through the block table, rings of
 // two 128-key K tiles and three V tiles) and one issues the products. S = Q
 // K^T lands in TMEM, the softmax writes the weights (f16: 2^-11 each, within
-// the 2e-3 bar) back to TMEM as the A operand of O += P V, and S of the next
-// tile runs under the softmax of this one.
+// the 2e-3 bar; small ones: kPaLower16) back to TMEM as the A operand of O += P
+// V, and S of the next tile runs under the softmax of this one.
 //
 // bf16 pools stay with the narrow kernel: bf16 weights (2^-8 each) need their
 // residuals in the product, here as a second set of 64 rows of the tile, and
@@ -300,7 +300,7 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
       tc_fence_before();
       mbar_arrive(&s.q_full);
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // running max (less kPaLower16), sum of the weights
 #pragma unroll 1
     for (int t = it.from; t < it.to; ++t, ++n) {
       if (!__all_sync(0xffffffffu, mbar_wait(&s.s_full, n & 1, &s.abort, p.status, PW_SITE(2, 1)))) return;
@@ -337,7 +337,8 @@ WATTN_DEVINL void pw_softmax(const PagedAttendParams &p, PwSmem &s, uint32_t tme
         for (int e = 0; e < 128; e += 8)
 #pragma unroll
           for (int a = 0; a < 4; ++a) mx[a] = pw_max3(mx[a], x(e + 2 * a), x(e + 2 * a + 1));
-        const float mc = pw_max3(pw_max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * p.scale_log2;
+        const float top = pw_max3(pw_max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY);
+        const float mc = fmaf(top, p.scale_log2, -kPaLower16);
         const bool need = mc > m + 8.0f;  // rescale only when the running max grows by more than 2^8
         rescale = __any_sync(0xffffffffu, need) && t > it.from;
         if (need) {

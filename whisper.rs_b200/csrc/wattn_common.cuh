@@ -100,7 +100,7 @@ WATTN_DEVINL float fmax3(float a, float b, float c) {
   return r;
 }
 
-// 2^x for a pair on the FMA pipe, for x <= 8 (x below -126 gives ~0).
+// 2^x for a pair on the FMA pipe, for x <= 16 (x below -126 gives ~0).
 // Range reduction x = j + f with j = rint(x) (the 1.5 * 2^23 rounding trick)
 // and f in [-1/2, 1/2]; 2^f from a cubic fitted for minimum relative error on
 // that interval (a discretised Chebyshev fit solved as a linear programme,
