@@ -156,6 +156,20 @@ def test_a_flat_tail_keeps_its_weight(W, rows):
     assert float((err / want).max()) <= 2.0 ** -6.5 + 2.0 ** -10 + 2 * 7.5e-5 + 2.0 ** -16
 
 
+@pytest.mark.parametrize("lens,new", [([5], [1]), ([448, 17, 300], [8, 1, 3]), ([40] * 30, [2] * 30),
+                                      ([9000], [5])])
+def test_up_to_8_rows_carry_the_weights_residuals(W, lens, new):
+    """f16 pools, f32 outputs, at most 8 rows to a request: the weights are two
+    f16 numbers and 22 bits, of which those below 2^-25 in the unit of 2^7
+    above the largest are lost."""
+    b = Batch(68, "f16", lens, new, 6, 64)
+    o, mag, top = formula(b, 1)
+    got = b.attend(W, 1, "f32")
+    keys = int((b.lens + b.new).max())
+    lim = (2 * 64 * 2.0 ** -24 * top + 2.0 ** -22 + 2.0 ** -18) * mag + keys * 2.0 ** -32 * 6 + 1e-7
+    assert (np.abs(got - o) <= lim + 2.0 ** -24 * np.abs(o)).all()
+
+
 # ------------------------------------------------------------------ sizes
 
 @pytest.mark.parametrize("dtype,rows", [("f16", 130), ("f16", 3), ("bf16", 130), ("f32", 3)])

@@ -81,7 +81,7 @@ template <typename T> struct PaType;
 template <> struct PaType<__half> : PaShape {
   static constexpr int kKeys = 32, kRows = 32;
   static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
-  static constexpr bool kResidual = false;  // f16 weights: 2^-11 each, within the 2e-3 bar
+  static constexpr bool kResidual = false;  // f16 weights of 9 rows or more: 2^-11 each, within the 2e-3 bar
   static constexpr float kLower = kPaLower16;
 };
 template <> struct PaType<__nv_bfloat16> : PaShape {
@@ -381,7 +381,8 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem<T> &s, const CUtens
 
 // The products of one item's stages: MT tiles of 16 query rows against 32
 // keys a stage. few (at most 8 rows): rows 8..15 of the tile carry the
-// weights' rounding residuals and cost no further products. (One body for
+// weights' rounding residuals and cost no further products, so f16 has them
+// there too (4.8e-7 off instead of 3.3e-4, as in the host-planned decode). (One body for
 // both MT is 14 % slower over single rows, its branches being predicated
 // products; one more for few rows costs more instruction fetches than it saves.)
 template <typename T, typename OutT, int MT>
@@ -596,7 +597,7 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        // (of a tile of few rows the residuals are rows 8..15, where T needs them)
+        // (of a tile of few rows the residuals are rows 8..15)
         uint32_t pa[4], pr[4];
 #pragma unroll
         for (int n2 = 0; n2 < 2; ++n2) {
@@ -605,12 +606,12 @@ WATTN_DEVINL void pa_item(const PagedAttendParams &p, PaSmem<T> &s, const PaItem
           const float e1 = ex2(fmaf(x[1], p.scale_log2, -mu[mt][0]));
           a[mt].l[0] += e0 + e1;
           pa[2 * n2] = pack2<T>(e0, e1);
-          if (PaType<T>::kResidual) {
+          if (PaType<T>::kResidual || few) {
             const float2 r = unpack2<T>(pa[2 * n2]);
             pr[2 * n2] = pack2<T>(e0 - r.x, e1 - r.y);
           }
           if (few) {
-            pa[2 * n2 + 1] = PaType<T>::kResidual ? pr[2 * n2] : 0u;
+            pa[2 * n2 + 1] = pr[2 * n2];
           } else {
             const float f0 = ex2(fmaf(x[2], p.scale_log2, -mu[mt][1]));
             const float f1 = ex2(fmaf(x[3], p.scale_log2, -mu[mt][1]));
