@@ -66,7 +66,9 @@ int wattn_last_error(char *buf, size_t len);
 /* Reads and clears the device status word of `device` (the current device
  * if device < 0): WATTN_OK, WATTN_ERR_TIMEOUT if a kernel's bounded wait ran
  * out since the last call, or WATTN_ERR_RANGE if a kernel found a device array
- * out of range (the first of them is kept). Synchronises that device. */
+ * out of range. A timeout goes first; the range report is then the next call's.
+ * The host-buffer entry points return (and clear) timeouts only. Synchronises
+ * that device. */
 int wattn_device_status(int device, int *status);
 
 /* ======================================================================

@@ -195,3 +195,29 @@ def test_lengths_near_2_31(W, dtype, rows):
                    -torch.inf)
     ref = torch.einsum("hnk,hkd->nhd", torch.softmax(z, -1), kv[1]).reshape(rows, -1)
     assert float((o[:rows] - ref).abs().max()) <= (1e-5 if dtype == "f32" else 2e-3)
+
+
+# ------------------------------------------------------------------ the status word
+
+def bad_length(W):
+    b = Batch(71, "f16", [100, 40], [3, 2], 2, 16)
+    b.lens[1] = 2 ** 31 - 1
+    b.attend(W, 1, "f32")
+
+
+def test_a_range_report_is_its_callers_alone(W, oracle):
+    """A length out of range in a paged call, then a call of host buffers:
+    that one succeeds, and the report is still there for who asks."""
+    bad_length(W)
+    r = np.random.default_rng(0)
+    q, k, v = (r.standard_normal(100 * 128).astype(np.float32) for _ in range(3))
+    out = np.empty_like(q)
+    W.flash_attention_2(q, k, v, 100, 100, 2, 128, False, out)
+    assert np.abs(out - oracle.flash_attention_2(q, k, v, 100, 100, 2, 128, False)).max() <= 1e-5
+    assert W.device_status() == -6 and W.device_status() == 0
+
+
+def test_a_range_report_does_not_hide_a_timeout(W):
+    bad_length(W)
+    assert W.selftest_bounded_wait(2000) == -4   # a flag that nothing sets: 2 ms
+    assert W.device_status() == -6 and W.device_status() == 0

@@ -16,8 +16,9 @@
 
 namespace wattn {
 
-// [0] status word, [1] site of the first bounded wait that ran out.
-__device__ int g_status[2] = {WATTN_OK, 0};
+// [0] status word, [1] site of the first bounded wait that ran out; [2], [3] of
+// the first device array found out of range.
+__device__ int g_status[4] = {WATTN_OK, 0, WATTN_OK, 0};
 
 namespace {
 
@@ -251,7 +252,8 @@ int finish_host(HostCtx *h, int rc) {
 }
 
 // After the device's work is complete: reports (and clears) a bounded wait
-// that ran out, from the current device's status word.
+// that ran out, from the current device's status word. (An array out of range
+// is not this call's, which has none on the device: that report stays.)
 int consume_status() {
   int *sp = device_status_ptr();
   int s[2] = {WATTN_OK, 0};
@@ -260,10 +262,7 @@ int consume_status() {
     const int zero[2] = {WATTN_OK, 0};
     cudaMemcpy(sp, zero, sizeof(zero), cudaMemcpyHostToDevice);
     reset_split_counters();
-    return set_error(s[0], "%s (site 0x%08x)",
-                     s[0] == WATTN_ERR_RANGE ? "a kernel found a device array out of range"
-                                             : "a kernel's bounded wait ran out",
-                     s[1]);
+    return set_error(s[0], "a kernel's bounded wait ran out (site 0x%08x)", s[1]);
   }
   return WATTN_OK;
 }
@@ -594,18 +593,20 @@ int wattn_device_status(int device, int *status) {
   int *sp = device_status_ptr();
   if (!sp) rc = WATTN_ERR_CUDA;
   if (rc == WATTN_OK && cudaDeviceSynchronize() != cudaSuccess) rc = check_launch("cudaDeviceSynchronize");
-  int s[2] = {WATTN_OK, 0};
-  if (rc == WATTN_OK && cudaMemcpy(s, sp, sizeof(s), cudaMemcpyDeviceToHost) != cudaSuccess)
+  int words[4] = {WATTN_OK, 0, WATTN_OK, 0};
+  if (rc == WATTN_OK && cudaMemcpy(words, sp, sizeof(words), cudaMemcpyDeviceToHost) != cudaSuccess)
     rc = check_launch("read status word");
+  // A timeout goes before an array out of range, whose report then stays.
+  const int which = words[0] == WATTN_OK && words[2] != WATTN_OK ? 2 : 0;
+  const int *s = words + which;
   const int zero[2] = {WATTN_OK, 0};
-  if (rc == WATTN_OK && cudaMemcpy(sp, zero, sizeof(zero), cudaMemcpyHostToDevice) != cudaSuccess)
+  if (rc == WATTN_OK && cudaMemcpy(sp + which, zero, sizeof(zero), cudaMemcpyHostToDevice) != cudaSuccess)
     rc = check_launch("clear status word");
-  if (rc == WATTN_OK && s[0] != WATTN_OK) reset_split_counters();
+  if (rc == WATTN_OK && words[0] != WATTN_OK) reset_split_counters();
   if (device >= 0 && device != prev) cudaSetDevice(prev);
   *status = s[0];
   if (rc == WATTN_OK && s[0] != WATTN_OK)
-    set_error(s[0], "%s at site 0x%08x",
-              s[0] == WATTN_ERR_RANGE ? "device array out of range" : "bounded wait ran out", s[1]);
+    set_error(s[0], "%s at site 0x%08x", which ? "device array out of range" : "bounded wait ran out", s[1]);
   return rc;
 }
 

@@ -348,7 +348,7 @@ WATTN_DEVINL void pa_load(const PagedAttendParams &p, PaSmem<T> &s, const CUtens
       if (lane == 0) {
         if (b == 0) mbar_arrive_expect_tx(bar, boxes * step * 4 * 32 * sizeof(T));  // (releases the announcement too)
         if ((unsigned)page >= (unsigned)p.n_pages) {
-          report_error(p.status, WATTN_ERR_RANGE, (4 << 24) | (3 << 16));
+          report_range(p.status, (4 << 24) | (3 << 16));
           page = 0;
         }
         const int c1 = w.head * p.page_rows + ld.in_page, c3 = page * p.n_layers + p.layer;

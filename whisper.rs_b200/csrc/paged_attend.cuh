@@ -161,7 +161,7 @@ template <typename C, bool QUEUE = false> WATTN_DEVINL void pa_find_shares(const
   for (int i = s0; i < s1; ++i) {
     bool bad;
     const PaSeq q = pa_seq(p, i, &bad);
-    if (bad) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
+    if (bad) report_range(p.status, 4 << 24);
     mine += pa_head_units<C>(p, q) * p.n_heads;
     if constexpr (QUEUE) {
       items += pa_tiles<C>(q) * p.n_heads;
@@ -191,7 +191,7 @@ template <typename C, bool QUEUE = false> WATTN_DEVINL void pa_find_shares(const
     total += s.warp_sums[w];
   }
   if (total > INT_MAX) {  // more than a call may ask for
-    if (tid == 0) report_error(p.status, WATTN_ERR_RANGE, 4 << 24);
+    if (tid == 0) report_range(p.status, 4 << 24);
     total = 0;
   }
   if constexpr (QUEUE) {

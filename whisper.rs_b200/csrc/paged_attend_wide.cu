@@ -138,7 +138,7 @@ WATTN_DEVINL void pw_load(const PagedAttendParams &p, PwSmem &s, const CUtensorM
       const int at = ld.t * kPwKeys + lane * step, pi = at / p.page_rows;
       int page = p.table[w.s * p.table_stride + pi];
       if ((unsigned)page >= (unsigned)p.n_pages) {
-        report_error(p.status, WATTN_ERR_RANGE, PW_SITE(0, 1));
+        report_range(p.status, PW_SITE(0, 1));
         page = 0;
       }
       c1 = w.head * p.page_rows + at - pi * p.page_rows;

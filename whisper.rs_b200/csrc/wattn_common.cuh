@@ -37,12 +37,17 @@ WATTN_DEVINL unsigned long long globaltimer_ns() {
 }
 
 // status[0]: status word; status[1]: site of the first wait that ran out
-// (kernel << 24 | role << 16 | barrier << 8 | iteration & 0xff).
+// (kernel << 24 | role << 16 | barrier << 8 | iteration & 0xff). status[2],
+// status[3]: the same of a device array found out of range, apart because it is
+// the affair of the caller who passed it, and hides no timeout.
 WATTN_DEVINL void report_error(int *status, int code, int site) {
   if (atomicCAS(status, WATTN_OK, code) == WATTN_OK) atomicExch(status + 1, site);
 }
 WATTN_DEVINL void report_timeout(int *status, int site) {
   report_error(status, WATTN_ERR_TIMEOUT, site);
+}
+WATTN_DEVINL void report_range(int *status, int site) {
+  report_error(status + 2, WATTN_ERR_RANGE, site);
 }
 
 // ------------------------------------------------------------ element types
