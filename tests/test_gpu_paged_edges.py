@@ -4,7 +4,7 @@ larger than the step, and what the device status word says of whom."""
 import numpy as np
 import pytest
 
-from tests.test_gpu_paged import WIDE, Batch, W, bound, clean_status, cu, tdt, wide_batch  # noqa: F401
+from tests.test_gpu_paged import WIDE, Batch, W, bound, clean_status, cu, tdt, tree  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -36,13 +36,37 @@ def formula(b, layer, scale=0.125):
         seen[:, ln:] = torch.as_tensor(seen_by(b, s), device="cuda")
         z = torch.einsum("nhd,khd->hnk", q, kv[:, 0]) * scale
         z = z.masked_fill(~seen, -torch.inf)
-        p = torch.softmax(z, -1)
+        p = torch.softmax(z, -1).masked_fill(~seen.any(-1)[:, None], 0)
         big = torch.einsum("nhd,khd->hnk", q.abs(), kv[:, 0].abs()).masked_fill(~seen, 0) * scale
         for i, x in enumerate((torch.einsum("hnk,khd->nhd", p, kv[:, 1]),
                                torch.einsum("hnk,khd->nhd", p, kv[:, 1].abs()),
                                big.amax(-1).T[:, :, None].expand(n, b.heads, 64))):
             out[i, a:a + n] = x.reshape(n, w).cpu().numpy()
     return out
+
+
+def units(lens, new, heads, words):
+    """(units of the narrow, of the wide kernel) that a step of f16 counts for;
+    words: mask words, 0 without masks."""
+    total = [0, 0]
+    for k, (keys, rows, stage, item) in enumerate(((32, 32, 5, 12), (128, 128, 2, 3))):
+        for ln, n in zip(lens, new):
+            for first in range(0, n, rows):
+                end = ln + min(n, 32 * words if words else first + rows)
+                total[k] += -(-end // keys) * (4 if k == 0 and n - first <= 16 else stage) + item
+    return total[0] * heads, total[1] * heads
+
+
+def wide(seed, lens, new, heads, page_rows, kind="tree", dead=0.0, **kw):
+    """A step that the kernel for many rows takes, as the numbers of its work say."""
+    rng = np.random.default_rng(seed)
+    par = sum((tree(rng, k, dead) for k in new), []) if kind == "tree" else None
+    words = -(-max(new) // 32)
+    kw = {"layers": 1, **kw}
+    b = Batch(seed, "f16", lens, new, heads, page_rows, par, words=words, **kw)
+    narrow, many = units(lens, new, heads, words if par else 0)
+    assert narrow > 33 * many and narrow >= 150 * 148 * 8 and b.max_rows // len(lens) > 96
+    return b
 
 
 def place(b, s, at):
@@ -57,38 +81,38 @@ def test_wide_value_that_is_not_finite_where_the_maximum_grows(W, value):
     """Tiles in which the running maximum grows by more than 2^8 and a draft's
     value is not finite: the sums so far are rescaled once, in all dimensions
     but the value's own."""
-    b = wide_batch(66, [1000], [128], 2, 64, layers=1)
+    b = wide(66, [15000], [128], 20, 64)
     b.q += 1
     # scores of about 32 in the tile of the first drafts, of about 64 in the next
     # (every row sees that draft)
-    jumps = [(999, 4.0), (1030, 8.0)]
+    jumps = [(14999, 4.0), (15110, 8.0)]
     for at, k in jumps:
         page, row = place(b, 0, at)
         b.pool[page, 0, 0, :, row] = k
-    b.mask[:128, 0] |= np.int32(1 << 30)
+    b.mask[:128, 3] |= np.int32(1 << 14)
     o, mag, top = formula(b, 0)
     sees = seen_by(b, 0)
-    hit = sees[:, 4] | sees[:, 40]
+    hit = sees[:, 4] | sees[:, 108]
     assert hit.any() and not hit.all()
-    for at in (1004, 1040):
+    for at in (15004, 15108):
         page, row = place(b, 0, at)
-        b.pool[page, 0, 1, 1, row, 37] = value
+        b.pool[page, 0, 1, :, row, 37] = value
     got = b.attend(W, 0, "f32")
-    want = got[hit, 64 + 37]
+    want = got[hit, 37::64]
     assert np.isnan(want).all() if value != value else (want == value).all()
-    got[hit, 64 + 37] = o[hit, 64 + 37]
-    lim = bound("f16", "f32", o, mag, top, 1128, 6.0) + WIDE * mag
+    got[hit, 37::64] = o[hit, 37::64]
+    lim = bound("f16", "f32", o, mag, top, 15128, 6.0) + WIDE * mag
     assert (np.abs(got - o) <= lim).all()
 
 
-@pytest.mark.parametrize("dtype,wide", [("f16", True), ("f16", False), ("bf16", False), ("f32", False)])
+@pytest.mark.parametrize("dtype,many", [("f16", True), ("f16", False), ("bf16", False), ("f32", False)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_a_key_that_is_not_finite_is_seen(W, dtype, wide, bad):
+def test_a_key_that_is_not_finite_is_seen(W, dtype, many, bad):
     """One element of one draft's key, at each of nine neighbouring positions: a
     row that sees it has a score that is NaN or +inf there and is NaN, or one
     of -inf and does without that key; the others are as they were."""
-    lens, new = ([1000], [128]) if wide else ([70], [40])
-    b = wide_batch(67, lens, new, 2, 64, layers=1) if wide else Batch(
+    lens, new = ([15000], [128]) if many else ([70], [40])
+    b = wide(67, lens, new, 20, 64) if many else Batch(
         67, dtype, lens, new, 2, 64, [-1] + [max(0, i - 2) for i in range(1, new[0])], layers=1)
     clean, mask = b.attend(W, 0, "f32"), b.mask.copy()
     n_lost = n_without = 0
@@ -102,19 +126,19 @@ def test_a_key_that_is_not_finite_is_seen(W, dtype, wide, bad):
         lost = sees if bad != bad else sees & positive
         n_lost += lost.sum()
         assert not sees.all()
-        assert np.isnan(got[lost, 64:]).all(), j
+        assert np.isnan(got[lost, 64:128]).all(), j
         same = ~sees
         assert np.array_equal(got[same], clean[same])
-        assert np.array_equal(got[:, :64], clean[:, :64])
+        assert np.array_equal(got[:, :64], clean[:, :64]) and np.array_equal(got[:, 128:], clean[:, 128:])
         if bad == bad:  # without that key
             without = sees & ~positive
             b.pool[page, 0, 0, 1, row, 5] = keep
             b.mask[:new[0], 0] &= ~np.int32(1 << j)
             o, mag, top = formula(b, 0)
             b.mask = mask.copy()
-            lim = bound(dtype, "f32", o, mag, top, 1200, 6.0) + (WIDE if wide else 0) * mag
+            lim = bound(dtype, "f32", o, mag, top, 1200, 6.0) + (WIDE if many else 0) * mag
             n_without += without.sum()
-            assert (np.abs(got - o) <= lim)[without, 64:].all()
+            assert (np.abs(got - o) <= lim)[without, 64:128].all()
         b.pool[page, 0, 0, 1, row, 5] = keep
     assert n_lost > 0 and (n_without > 0 or bad != bad)
 
@@ -195,6 +219,91 @@ def test_lengths_near_2_31(W, dtype, rows):
                    -torch.inf)
     ref = torch.einsum("hnk,hkd->nhd", torch.softmax(z, -1), kv[1]).reshape(rows, -1)
     assert float((o[:rows] - ref).abs().max()) <= (1e-5 if dtype == "f32" else 2e-3)
+
+
+@pytest.mark.parametrize("n,heads", [(4, 6), (64, 20)])
+def test_row_buffers_larger_than_the_step(W, n, heads):
+    """Single rows in a buffer for 120 rows a request (a graph captured once
+    for steps of every length) are computed as in a buffer of their own."""
+    import torch
+    lens = ([1000, 300, 700, 80] * n)[:n]
+    b = Batch(70, "f16", lens, [1] * n, heads, 64, spare_rows=n * 119)
+    table, seq, start, _ = b.device()
+    small = torch.zeros(n, heads * 64, device="cuda")
+    large = torch.zeros(b.max_rows, heads * 64, device="cuda")
+    W.paged_attend(b.pool, 1, table, seq, start, b.q[:n], small)
+    W.paged_attend(b.pool, 1, table, seq, start, b.q, large)
+    assert torch.equal(small, large[:n])
+    assert (large[n:] == 0).all()
+
+
+# ------------------------------------------------------------------ steps that the wide kernel takes
+
+WIDE_STEPS = [
+    # lens, new, heads, page_rows
+    ([15000], [128], 20, 64), ([9000, 0, 33, 1000], [256, 1, 2, 127], 20, 128),
+    ([2500] * 8, [120] * 8, 16, 48), ([4000], [1000], 16, 16), ([7000, 1, 6501, 513], [124, 0, 253, 113], 20, 80),
+    ([0, 0], [2040, 2048], 20, 32),
+]
+
+
+@pytest.mark.parametrize("step", range(len(WIDE_STEPS)))
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+@pytest.mark.parametrize("out", ["f16", "f32"])
+def test_wide_steps(W, step, kind, out):
+    """Rows that fill tiles of 128 nearly, next to requests that do not."""
+    b = wide(80 + step, *WIDE_STEPS[step], kind, dead=0.02, stride=8 * step)
+    got = b.attend(W, 0, out, stride=8 * step)
+    o, mag, top = formula(b, 0)
+    lim = bound("f16", out, o, mag, top, int((b.lens + b.new).max()), 6.0) + WIDE * mag
+    assert (np.abs(got - o) <= lim).all()
+    assert np.array_equal(got, b.attend(W, 0, out, stride=8 * step))
+
+
+def test_the_work_decides_which_kernel(W):
+    """The same request alone, and beside so many that rest that the buffers
+    cannot be full: other sums, to their rounding the same."""
+    import torch
+    b = wide(90, [15000], [128], 20, 64, "chain")
+    alone = b.attend(W, 0, "f32")
+    table, _, _, _ = b.device()
+    o = torch.zeros(b.max_rows, 1280, device="cuda")
+    W.paged_attend(b.pool, 0, table.expand(9, -1).contiguous(), cu(np.array([15000] + [0] * 8)),
+                   cu(np.array([0] + [128] * 9)), b.q, o)
+    o = o[:128].cpu().numpy()
+    assert not np.array_equal(o, alone)
+    ref, mag, top = formula(b, 0)
+    assert (np.abs(o - ref) <= bound("f16", "f32", ref, mag, top, 15128, 6.0)).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), "lowest"])
+def test_wide_steps_masked_places_have_no_influence(W, bad):
+    """Drafts that hold NaN, infinities or the lowest value reach only the rows that see them."""
+    import torch
+    bad = torch.finfo(torch.float16).min if bad == "lowest" else bad
+    b = wide(91, [9000, 0, 33, 1000], [256, 1, 2, 127], 20, 128)
+    clean = b.attend(W, 0, "f32")
+    hit = np.zeros(int(b.start[-1]), bool)
+    for s, j in [(0, 5), (0, 250), (3, 60), (2, 1)]:
+        page, row = place(b, s, int(b.lens[s]) + j)
+        b.pool[page, :, :, :, row] = bad
+        a = int(b.start[s])
+        hit[a:a + b.new[s]] |= seen_by(b, s)[:, j]
+    got = b.attend(W, 0, "f32")
+    assert hit.any() and not hit.all()
+    assert np.array_equal(got[~hit], clean[~hit])
+    if not np.isfinite(bad):
+        assert np.isnan(got[hit]).any(axis=1).all()
+
+
+def test_wide_steps_rows_that_see_nothing_are_zero(W):
+    b = wide(92, [9000, 0], [256, 120], 20, 128)
+    b.mask[[256, 300, 375]] = 0        # rows of the request without context
+    b.mask[40] = 0                     # this one still sees its context
+    got = b.attend(W, 0, "f32")
+    o, mag, top = formula(b, 0)
+    assert (got[[256, 300, 375]] == 0).all() and (got[40] != 0).any()
+    assert (np.abs(got - o) <= bound("f16", "f32", o, mag, top, 9256, 6.0) + WIDE * mag).all()
 
 
 # ------------------------------------------------------------------ the status word

@@ -38,54 +38,32 @@ namespace {
 
 constexpr int kPaStageBytes = 8192;  // keys, then values
 constexpr int kPaStages = 3;      // stages of a warp's ring
-constexpr int kPaWarps = 4;       // compute warps (one warpgroup), and as many load warps
-constexpr int kPaThreads = 2 * kPaWarps * 32;
-constexpr int kPaCtasPerSm = 2;
 // Registers per thread: what the block is launched with, then after the
 // warpgroups' split (whose sum may not exceed twice the launch's).
 constexpr int kPaRegs = 128, kPaComputeRegs = 216, kPaLoadRegs = 40;
 static_assert(kPaComputeRegs + kPaLoadRegs <= 2 * kPaRegs, "a larger split never gets its registers");
-// Whether the wide kernel is the faster one, from what the host knows: the
-// rows of a request, averaged over the row buffer, fill tiles of 128 to 7/8
-// (8 rows of padding aside), over this many cached positions. f16, wide /
-// narrow: 16 requests of 8 heads, 4096 cached: 64 rows 66 us / 74, 112 rows 70
-// / 96, 128 rows 70 / 104, 160 rows 111 / 129, 256 rows 111 / 188. 16 requests
-// of 16 heads: 500 cached, 96 rows 47 / 41, 112 rows 45 / 55, 128 rows 47 / 53,
-// 160 rows 86 / 59, 256 rows 88 / 94; 2000 cached, 96 rows 84 / 84, 112 rows 80
-// / 111, 160 rows 137 / 129, 224 rows 158 / 174. 64 requests of 20 heads, 300
-// cached, 128 rows 129 / 119; 32 of them, nothing cached, 45 / 35.
-constexpr int kPaWideKeys = 448;
-inline bool pa_wide(int64_t max_rows, int n_seqs, int cap) {
-  const int64_t rows = max_rows / n_seqs, tiles = (rows + 119) / 128;
-  return tiles > 0 && rows * 8 >= tiles * 128 * 7 && cap - rows >= kPaWideKeys;
+// Whether a step of these sizes can be one for the wide kernel (pa_takes_wide):
+// else only the narrow one is launched. What the requests hold is on the
+// device; the buffers bound it.
+inline bool pa_may_be_wide(const PagedAttendParams &p) {
+  const int64_t tiles = (int64_t)p.max_rows / PaNarrow16::kRows + p.n_seqs;
+  const int64_t stages = (p.cap + PaNarrow16::kKeys - 1) / PaNarrow16::kKeys;
+  const int64_t units = tiles * (stages * PaNarrow16::kWideUnits + PaNarrow16::kItemUnits);
+  return p.max_rows / p.n_seqs > PwShape::kRows - PaNarrow16::kRows && p.cap >= kPaWideCap &&
+         units >= kPaWideUnits * p.n_sm * kPaCtasPerSm * kPaWarps / p.n_heads;
 }
 constexpr int kPaMergeAll = 8;    // CTAs beyond the first from which all warps merge an item
 constexpr int kPaQueue = 8;       // items a warp may have loads for, and one more
 constexpr int kPaTileFloats = 32 * 36;  // a partial's tile of 16 rows: 36 floats a lane
 static_assert(kPaStages * kPaStageBytes >= kPaWarps * kPaTileFloats * 4, "a ring holds the warps' sums");
 
-// A stage is 8 KB of keys and values. Units, measured: two tiles of 16 rows
-// cost a quarter more than one, an item as much as three stages (with 2, 3 and
-// 2 units trees of 64 rows over 32768 tokens take 82 us instead of 77).
-struct PaShape {
-  static constexpr int kShares = kPaWarps, kThreads = kPaThreads;
-  // Items to a compute warp from which they are taken one by one (cached
-  // lengths from 1 to 440, f16, taken / in equal shares: 400 requests of 12
-  // heads 68.6 us / 76.8, 600 88.3 / 103.4, 300 of 20 heads and 40 new rows
-  // 235 / 273; of 200 or 300 requests of 12 heads the lookup alone costs 2 us).
-  static constexpr int kQueueItems = 4;
-  static constexpr int kStageUnits = 4, kWideUnits = 5, kItemUnits = 12;
-  static constexpr int kMinUnits = 16;  // units of a share below which fewer warps work
-};
 template <typename T> struct PaType;
-template <> struct PaType<__half> : PaShape {
-  static constexpr int kKeys = 32, kRows = 32;
+template <> struct PaType<__half> : PaNarrow16 {
   static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
   static constexpr bool kResidual = false;  // f16 weights of 9 rows or more: 2^-11 each, within the 2e-3 bar
   static constexpr float kLower = kPaLower16;
 };
-template <> struct PaType<__nv_bfloat16> : PaShape {
-  static constexpr int kKeys = 32, kRows = 32;
+template <> struct PaType<__nv_bfloat16> : PaNarrow16 {
   static constexpr uint32_t kOne = 0x3f80u, kInf = 0x7f80u;
   static constexpr bool kResidual = true;   // bf16's 2^-8 alone would not be: its rounding goes in too
   static constexpr float kLower = 0.f;      // (f32's range)
@@ -103,6 +81,7 @@ struct PaSmem {
   PaItem queue[kPaWarps][kPaQueue];
   PaItem cut[kPaWarps][2];  // items cut by the share's begin and by its end (stages 0: none)
   PaFind<PaType<T>> find;
+  PaChoice choice;
   int merge_first[2 * kPaWarps], merge_last[2 * kPaWarps];  // shares to merge, per cut item
   int final[2 * kPaWarps];  // this CTA merges the parts of them all
   int abort;
@@ -1032,6 +1011,8 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
   }
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
+  if constexpr (__is_same(T, __half))
+    if (p.choose && pa_takes_wide(p, s.choice)) return;
   pa_find_shares<PaType<T>, QUEUE>(p, s.find);
   if (warp >= kPaWarps) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPaLoadRegs));
@@ -1122,11 +1103,17 @@ int launch_stream(const PagedAttendParams &p, int dtype, cudaStream_t st) {
 
 int launch_attend(const PagedAttendParams &p, int dtype, int out_dtype, cudaStream_t st) {
   if (dtype == WATTN_F32) return launch_stream<float, float>(p, dtype, st);
-  if (dtype == WATTN_F16 && pa_wide(p.max_rows, p.n_seqs, p.cap))
-    return launch_paged_attend_wide(p, out_dtype, st);
-  if (dtype == WATTN_F16)
-    return out_dtype == WATTN_F32 ? launch_stream<__half, float>(p, dtype, st)
-                                  : launch_stream<__half, __half>(p, dtype, st);
+  if (dtype == WATTN_F16) {
+    // The narrow kernel, or both, of which the one that is not for the step
+    // leaves at once: 4 to 7 us. (320 single rows of 20 heads over up to 1000
+    // tokens, in buffers for 128 rows each: 133 us, in buffers of their own 127;
+    // in the wide kernel they would take 552.)
+    PagedAttendParams q = p;
+    q.choose = pa_may_be_wide(p);
+    const int rc = out_dtype == WATTN_F32 ? launch_stream<__half, float>(q, dtype, st)
+                                          : launch_stream<__half, __half>(q, dtype, st);
+    return rc == WATTN_OK && q.choose ? launch_paged_attend_wide(q, out_dtype, st) : rc;
+  }
   return out_dtype == WATTN_F32 ? launch_stream<__nv_bfloat16, float>(p, dtype, st)
                                 : launch_stream<__nv_bfloat16, __nv_bfloat16>(p, dtype, st);
 }

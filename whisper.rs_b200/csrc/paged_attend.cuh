@@ -37,8 +37,12 @@ struct PagedAttendParams {
   int *taken;    // items taken from the queue
   int *status;
   int n_sm;
+  bool choose;   // f16: the kernels' work decides which of the two does it
 };
 
+constexpr int kPaWarps = 4;      // narrow kernel: compute warps (one warpgroup), and as many load warps
+constexpr int kPaThreads = 2 * kPaWarps * 32;
+constexpr int kPaCtasPerSm = 2;
 constexpr int kPaTail = 16;  // rows of a tail box: the pool's unit of page rows
 constexpr int kPaMostKeys = 128;  // keys of a stage, at most
 // f16 weights are taken relative to a running maximum that is lowered by this
@@ -47,6 +51,31 @@ constexpr int kPaMostKeys = 128;  // keys of a stage, at most
 // under 2^-14) is 2^-32 of the largest weight. Relative to the maximum itself it
 // would be 2^-25, and 131072 keys of such weights 2^-8 of the output.
 constexpr float kPaLower16 = 7.f;
+
+// The narrow kernel's configuration (16-bit pools). A stage is 8 KB of keys and
+// values. Units, measured: two tiles of 16 rows cost a quarter more than one, an
+// item as much as three stages (with 2, 3 and 2 units trees of 64 rows over
+// 32768 tokens take 82 us instead of 77).
+struct PaShape {
+  static constexpr int kShares = kPaWarps, kThreads = kPaThreads;
+  // Items to a compute warp from which they are taken one by one (cached
+  // lengths from 1 to 440, f16, taken / in equal shares: 400 requests of 12
+  // heads 68.6 us / 76.8, 600 88.3 / 103.4, 300 of 20 heads and 40 new rows
+  // 235 / 273; of 200 or 300 requests of 12 heads the lookup alone costs 2 us).
+  static constexpr int kQueueItems = 4;
+  static constexpr int kStageUnits = 4, kWideUnits = 5, kItemUnits = 12;
+  static constexpr int kMinUnits = 16;  // units of a share below which fewer warps work
+};
+struct PaNarrow16 : PaShape {
+  static constexpr int kKeys = 32, kRows = 32;
+};
+// The wide kernel's.
+struct PwShape {
+  static constexpr int kKeys = kPaMostKeys, kRows = 128;
+  static constexpr int kShares = 1, kThreads = kPaThreads;
+  static constexpr int kStageUnits = 2, kWideUnits = 2, kItemUnits = 3;
+  static constexpr int kMinUnits = 4;
+};
 
 // One request as the kernel sees it. One whose arrays are out of range has
 // no rows here (and is reported).
@@ -83,6 +112,49 @@ template <typename C> WATTN_DEVINL long long pa_head_units(const PagedAttendPara
   long long stages = full * pa_stages<C>(p, q, 0);
   if (p.row_mask == nullptr) stages += full * (full - 1) / 2;  // one more from tile to tile
   return stages * pa_weight<C>(q, 0) + full * C::kItemUnits + pa_units<C>(p, q, (int)full);
+}
+
+// Whether a step (f16) is for the wide kernel: the narrow one's units are more
+// than kPaWideRatio times the wide one's, and kPaWideUnits or more to each of
+// its compute warps (below, the wide kernel's start of 20 us shows). Narrow /
+// wide, us, trees of 128 rows unless said: 16 requests of 8 heads, 4096 cached
+// 92 / 68, 64 rows 58 / 66, 100 rows 87 / 69, 160 rows 115 / 111, 256 rows
+// 181 / 112; 16 of 16 heads, 2000 cached 101 / 83, 500 cached 47 / 46; 64 of 20
+// heads, 300 cached 127 / 135, 384 cached 121 / 109; chains of 512 rows over
+// 4000, 4 of 20 heads 208 / 146; 60 mixed requests of 20 heads, most with one
+// row 150 / 273; one of one head, 1000 rows over 4000 26 / 39. Of 73 such points
+// the rule takes the slower kernel by 9 % at most.
+constexpr int kPaWideRatio = 33;
+constexpr long long kPaWideUnits = 150;
+constexpr int kPaWideCap = 512;  // positions of a table below which no point was the wide kernel's
+struct PaChoice {
+  long long narrow[kPaThreads / 32], wide[kPaThreads / 32];
+};
+WATTN_DEVINL bool pa_takes_wide(const PagedAttendParams &p, PaChoice &s) {
+  long long narrow = 0, wide = 0;
+  for (int i = threadIdx.x; i < p.n_seqs; i += kPaThreads) {
+    const PaSeq q = pa_seq(p, i, nullptr);
+    narrow += pa_head_units<PaNarrow16>(p, q);
+    wide += pa_head_units<PwShape>(p, q);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    narrow += __shfl_xor_sync(0xffffffffu, narrow, d);
+    wide += __shfl_xor_sync(0xffffffffu, wide, d);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    s.narrow[threadIdx.x >> 5] = narrow;
+    s.wide[threadIdx.x >> 5] = wide;
+  }
+  __syncthreads();
+  narrow = wide = 0;
+#pragma unroll
+  for (int w = 0; w < kPaThreads / 32; ++w) {
+    narrow += s.narrow[w];
+    wide += s.wide[w];
+  }
+  return narrow > kPaWideRatio * wide &&
+         narrow * p.n_heads >= kPaWideUnits * p.n_sm * kPaCtasPerSm * kPaWarps;
 }
 
 // `total` units (below 2^31) in `parts` shares, in order: the first `more` of

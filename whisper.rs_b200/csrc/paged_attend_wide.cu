@@ -29,10 +29,10 @@ namespace wattn {
 
 namespace {
 
-constexpr int kPwKeys = kPaMostKeys;  // keys of a stage
+constexpr int kPwKeys = PwShape::kKeys;  // keys of a stage
 constexpr int kPwTile = kPwKeys * 128;
 constexpr int kPwK = 2, kPwV = 3;  // ring depths
-constexpr int kPwThreads = 8 * 32;
+constexpr int kPwThreads = PwShape::kThreads;
 constexpr int kPwLoadWarp = 4, kPwMmaWarp = 5;
 // Registers per thread: at the launch, then after the warpgroups' split
 // (whose sum may not exceed twice the launch's).
@@ -49,14 +49,6 @@ constexpr int kPwFmaPairs = 4;
 constexpr uint32_t kPwCols = 256;  // TMEM: S 128, P 64, O 64
 constexpr int kPwPartFloats = 66 * 128;  // a partial: O [64][row], m, l
 
-struct PwShape {
-  static constexpr int kKeys = kPwKeys, kRows = 128;
-  static constexpr int kShares = 1, kThreads = kPwThreads;
-  static constexpr int kQueueItems = 0;  // (no queue)
-  static constexpr int kStageUnits = 2, kWideUnits = 2, kItemUnits = 3;
-  static constexpr int kMinUnits = 4;
-};
-
 struct PwSmem {
   uint8_t q[kPwTile];
   uint8_t k[kPwK][kPwTile];
@@ -67,6 +59,7 @@ struct PwSmem {
   uint64_t drain, done, meet;
   PaItem queue[kPwQueue];
   PaFind<PwShape> find;
+  PaChoice choice;
   uint32_t odd[4];  // keys of a tile with values that are infinite or NaN
   uint32_t tmem;
   int abort, last;
@@ -568,8 +561,12 @@ __global__ void __launch_bounds__(kPwThreads, kPwCtasPerSm)
   tc_fence_after();
   grid_dep_wait();  // (launched with programmatic serialisation)
   grid_dep_launch();
-  pa_find_shares<PwShape>(p, s.find);
   const uint32_t tmem = s.tmem;
+  if (!pa_takes_wide(p, s.choice)) {
+    if (warp == kPwMmaWarp) tmem_dealloc(tmem, kPwCols);
+    return;
+  }
+  pa_find_shares<PwShape>(p, s.find);
   if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPwOtherRegs));
     if (warp == kPwLoadWarp) pw_load(p, s, map, map_tail, lane);
