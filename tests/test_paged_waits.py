@@ -28,9 +28,12 @@ def test_lanes_leave_together():
     the same way: it may run out for some of them only. They vote, or those
     end the warp's share in what all of them read next."""
     text = source("paged_attend.cu")
-    left = re.sub(r"\bif \(!mbar_wait\([^;]*\)\)\s*s\.queue\[warp\]\[i % kPaQueue\]\.nr = 0;\s*__syncwarp\(\);"
-                  r"\s*const PaItem it = s\.queue\[warp\]\[i % kPaQueue\];\s*if \(it\.nr == 0\) break;", "", text)
-    assert left != text and not re.search(r"\bif \(!mbar_wait\(", left)
+    kernel = text[text.index("paged_attend_stream_kernel("):text.index("int pa_sms()")]
+    assert kernel.count("mbar_wait(") == 2
+    assert re.search(r"if \(!__all_sync\(0xffffffffu, mbar_wait\([^;]*\)\)\)\s*break;", kernel)
+    assert re.search(r"if \(!mbar_wait\([^;]*\)\)\s*s\.queue\[warp\]\[i % kPaQueue\]\.nr = 0;\s*__syncwarp\(\);"
+                     r"\s*\}\s*const PaItem it = s\.queue\[warp\]\[i % kPaQueue\];\s*if \(it\.nr == 0\) break;", kernel)
+    assert len(re.findall(r"\bif \(!mbar_wait\(", text)) == 1
     wide = source("paged_attend_wide.cu")
     softmax = wide[wide.index("void pw_softmax("):wide.index("paged_attend_wide_kernel(")]
     load = wide[wide.index("void pw_load("):wide.index("void pw_products(")]

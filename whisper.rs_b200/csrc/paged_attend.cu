@@ -1024,12 +1024,19 @@ __global__ void __launch_bounds__(kPaThreads, kPaCtasPerSm)
 #pragma unroll 1
     for (uint32_t i = 0;; ++i) {
       // The next stage's barrier covers the announcement of its item. A wait
-      // may run out for some lanes only, and all of them stay or leave: such
-      // a lane ends the share for the others. (A vote of the lanes costs trees
-      // of 64 rows over 32768 tokens 5 %, in registers.)
-      if (!mbar_wait(&s.full[warp][pos & 3], pos >> 31, &s.abort, p.status, (4 << 24) | (2 << 16)))
-        s.queue[warp][i % kPaQueue].nr = 0;
-      __syncwarp();
+      // may run out for some lanes only, and all of them stay or leave: they
+      // vote, or such a lane ends the share for the others. (Which of the two
+      // costs no registers: by vote, trees of 64 rows over 32768 tokens take
+      // 5 % longer, by mark 320 single rows of f16 2 %.)
+      uint64_t *const full = &s.full[warp][pos & 3];
+      if constexpr (QUEUE) {
+        if (!__all_sync(0xffffffffu, mbar_wait(full, pos >> 31, &s.abort, p.status, (4 << 24) | (2 << 16))))
+          break;
+      } else {
+        if (!mbar_wait(full, pos >> 31, &s.abort, p.status, (4 << 24) | (2 << 16)))
+          s.queue[warp][i % kPaQueue].nr = 0;
+        __syncwarp();
+      }
       const PaItem it = s.queue[warp][i % kPaQueue];
       if (it.nr == 0) break;
       if constexpr (sizeof(T) == 4) pa_item_f32(p, s, it, pos, warp, lane);
