@@ -306,6 +306,87 @@ def test_wide_steps_rows_that_see_nothing_are_zero(W):
     assert (np.abs(got - o) <= bound("f16", "f32", o, mag, top, 9256, 6.0) + WIDE * mag).all()
 
 
+def either_kernel():
+    """A step for the wide kernel, and one of single rows in buffers for many."""
+    many = wide(93, [9000, 0, 33, 1000], [256, 1, 2, 127], 20, 128)
+    single = Batch(94, "f16", [1000, 300, 700, 80] * 16, [1] * 64, 20, 64, spare_rows=64 * 119, layers=1)
+    return many, single
+
+
+def test_either_kernel_repeats_beside_another(W):
+    """The same calls 100 times while attention of its own runs on another stream."""
+    import torch
+    x = torch.randn(4 * 700 * 384, device="cuda").half()
+    y = torch.empty_like(x)
+    ws = torch.zeros(W.paged_attend_workspace_bytes(1, 1, 1), dtype=torch.uint8, device="cuda")
+    work = []
+    for b in either_kernel():
+        a = dict(zip(("block_table", "seq_lens", "row_start", "row_mask"), b.device()))
+        want = torch.zeros(b.max_rows, b.heads * 64, device="cuda")
+        W.paged_attend(b.pool, 0, q=b.q, o=want, **a)
+        work.append((b, a, want, torch.empty_like(want)))
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    side, main = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(100):
+        W.attention_fwd(x, x, x, y, batch=4, t_q=700, t_kv=700, n_heads=6, scale=0.125, stream=side)
+        with torch.cuda.stream(main):
+            for b, a, want, o in work:
+                o.zero_()
+                W.paged_attend(b.pool, 0, q=b.q, o=o, workspace=ws, **a)
+                differ += (o != want).any()
+    torch.cuda.synchronize()
+    assert int(differ) == 0
+    assert (ws[:65536 * 4] == 0).all()
+
+
+def test_either_kernel_from_one_graph(W):
+    """A graph captured once, without a workspace, replayed with lengths for
+    the one kernel and for the other, on two streams at once."""
+    import torch
+    long = Batch(95, "f16", [9000, 1000], [256, 127], 20, 64, layers=1)
+    single, n = either_kernel()[1], 64
+    rows, pages = single.max_rows, long.st.table.shape[1]
+    narrow, many = units(long.lens, long.new, 20, 0)
+    assert narrow > 33 * many and narrow >= 150 * 148 * 8 and rows // n > 96
+    graphs = []
+    for _ in range(2):
+        g = dict(pool=torch.zeros(max(long.n_pages, single.n_pages), 1, 2, 20, 64, 64,
+                                  dtype=torch.float16, device="cuda"),
+                 block_table=torch.zeros(n, pages, dtype=torch.int32, device="cuda"),
+                 seq_lens=torch.zeros(n, dtype=torch.int32, device="cuda"),
+                 row_start=torch.zeros(n + 1, dtype=torch.int32, device="cuda"),
+                 q=torch.zeros(rows, 1280, dtype=torch.float16, device="cuda"),
+                 o=torch.zeros(rows, 1280, device="cuda"))
+        s, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            W.paged_attend(layer=0, **g)
+        graphs.append((g, s, graph))
+    for steps in ((long, single), (single, long), (long, long)):
+        for (g, s, graph), b in zip(graphs, steps):
+            k = len(b.lens)
+            g["pool"][:b.n_pages] = b.pool
+            g["block_table"][:k, :b.st.table.shape[1]] = cu(b.st.table)
+            g["seq_lens"][:k] = cu(b.lens)
+            g["row_start"][:k + 1] = cu(b.start)
+            g["row_start"][k + 1:] = int(b.start[-1])
+            g["q"][:b.max_rows] = b.q
+            g["o"].fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s, graph in graphs:
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for (g, s, graph), b in zip(graphs, steps):
+            end = int(b.start[-1])
+            o, mag, top = formula(b, 0)
+            lim = bound("f16", "f32", o, mag, top, 9300, 6.0) + WIDE * mag
+            assert (np.abs(g["o"][:end].cpu().numpy() - o) <= lim).all()
+            assert (g["o"][end:] == 7).all()
+
+
 # ------------------------------------------------------------------ the status word
 
 def bad_length(W):
