@@ -1154,8 +1154,9 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
     return set_error(WATTN_ERR_INVALID, "paged_attend: invalid sizes");
   if (row_mask != nullptr && mask_words <= 0)
     return set_error(WATTN_ERR_INVALID, "paged_attend: mask_words must be positive");
-  if (!(scale > 0.f) || scale > 3.0e38f)
-    return set_error(WATTN_ERR_INVALID, "paged_attend: scale must be finite and positive");
+  const float scale_log2 = scale * 1.4426950408889634f;  // (in the kernels' base: may be infinite where scale is not)
+  if (!(scale > 0.f) || !(scale_log2 < INFINITY))
+    return set_error(WATTN_ERR_INVALID, "paged_attend: scale must be positive and below 2.3e38");
   const int64_t w = (int64_t)n_heads * 64;
   if (q_row_stride < w || o_row_stride < w)
     return set_error(WATTN_ERR_INVALID, "paged_attend: row stride below width");
@@ -1190,7 +1191,7 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
   p.q_rs = q_row_stride;
   p.o_rs = o_row_stride;
   p.max_rows = max_rows;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   // (positions rounded up to a stage of either kernel stay within 32 bits)
   p.cap = (int)std::min((int64_t)max_pages * page_rows, (int64_t)INT32_MAX - 2 * kPaMostKeys);
   p.status = device_status_ptr();
