@@ -1,6 +1,8 @@
-"""Waits of the device-planned cache's kernels, checked in their source: a
-bounded wait that runs out cannot be caused in them without a fault, so what
-keeps their warps from waiting for one another for ever is read here."""
+"""What the device-planned cache does when something fails, checked in its
+source: a bounded wait that runs out in its kernels, or a captured call whose
+workspace cannot be cleared, cannot be caused without a fault, so what keeps
+warps from waiting for one another for ever, and memory from staying, is read
+here."""
 import os
 import re
 
@@ -39,3 +41,13 @@ def test_lanes_leave_together():
     load = wide[wide.index("void pw_load("):wide.index("void pw_products(")]
     for body in (softmax, load):
         assert "mbar_wait(" in body and not re.search(r"\bif \(!mbar_wait\(", body)
+
+
+def test_a_captured_workspace_is_freed_on_every_way_out():
+    """After its allocation joins a graph, a call ends by freeing it."""
+    text = source("paged_attend.cu")
+    rest = text[text.index("cudaMallocAsync(&own"):]
+    failed = rest[rest.index("cudaMemsetAsync(own"):]
+    assert failed.index("cudaFreeAsync(own, st)") < failed.index("return")
+    done = rest[rest.index("rc = launch_attend("):]
+    assert done.index("cudaFreeAsync(own, st)") < done.index("return")

@@ -1206,9 +1206,13 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();
     if (capture == cudaStreamCaptureStatusActive) {
-      if (cudaMallocAsync(&own, need, st) != cudaSuccess ||
-          cudaMemsetAsync(own, 0, kCounterBytes, st) != cudaSuccess)
+      if (cudaMallocAsync(&own, need, st) != cudaSuccess)
         return check_launch("paged_attend: a captured call's workspace");
+      if (cudaMemsetAsync(own, 0, kCounterBytes, st) != cudaSuccess) {
+        rc = check_launch("paged_attend: a captured call's workspace");
+        cudaFreeAsync(own, st);
+        return rc;
+      }
       workspace = own;
     } else {
       workspace = thread_workspace(need, st);
