@@ -422,15 +422,23 @@ int wattn_paged_write(void *pool, int dtype, int n_pages, int n_layers, int n_he
  * every row: one that is infinite or NaN may make any of its request's outputs
  * NaN. A table entry outside the pool, lengths beyond max_pages pages or row
  * starts outside [0, max_rows] make that request's rows unspecified, and
- * wattn_device_status() reports WATTN_ERR_RANGE; so does a call of 2^31 units
- * of work or more (about five for every 16 keys of each head and tile of 16
- * rows), which writes no rows. workspace as for wattn_decode_fwd
- * (wattn_paged_attend_workspace_bytes(), zero-filled before its first use),
- * or NULL. Calls that may overlap, captured graphs among them, need one each;
- * a call that is captured with NULL gets one of its graph's own, at the price
- * of a memset in it. After WATTN_ERR_TIMEOUT a workspace is zero-filled again
- * before its next use (wattn_device_status() does so for the calling thread's
- * own). */
+ * wattn_device_status() reports WATTN_ERR_RANGE; so does a request of more than
+ * 2^31 - 257 positions, and a call of 2^31 units of work or more, which writes
+ * no rows (f16 and bf16: up to 5 units for every 32 keys of each head and tile
+ * of 32 rows, and 12 for the tile; f32: 4 for every 16 keys of a tile of 16
+ * rows, and 12). A row that sees a draft whose score is NaN or +inf is NaN.
+ * The softmax weights enter the second product with 22 bits in f16 pools where
+ * the request has up to 8 new rows, with 11 where it has more (in steps of
+ * 2^-31 of the row's largest at the finest), with 16 in bf16 pools, and as two
+ * tf32 parts in f32 pools.
+ * workspace as for wattn_decode_fwd (wattn_paged_attend_workspace_bytes(),
+ * zero-filled before its first use), or NULL. Calls that may overlap, captured
+ * graphs among them, need one each; a call that is captured with NULL gets one
+ * of its graph's own, at the price of a memset and of an allocation in it (some
+ * 27 MB, shared by the calls of a graph that follow each other): such a graph
+ * can be instantiated once at a time only, and be no other's child. After
+ * WATTN_ERR_TIMEOUT a workspace is zero-filled again before its next use
+ * (wattn_device_status() does so for the calling thread's own). */
 size_t wattn_paged_attend_workspace_bytes(int n_seqs, int max_rows, int n_heads);
 int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, int n_heads,
                        int page_rows, int layer, const int *block_table, int64_t table_stride,
@@ -452,7 +460,9 @@ int wattn_paged_attend(const void *pool, int dtype, int n_pages, int n_layers, i
  * A request without new rows, or whose row 0 is no root, accepts nothing
  * (next_token -1). parents, row_start, row_slot as in wattn_paged_plan
  * (parents NULL: each row's parent is the one before it). The pages beyond the
- * new length are given back or used by the next plan. */
+ * new length are given back or used by the next plan. With n_seqs 0 nothing is
+ * written. (Rows that are kept without a check, a prompt's, need no call: their
+ * K/V are in place, and the caller adds n_new to seq_lens.) */
 int wattn_paged_accept(void *pool, int dtype, int n_pages, int n_layers, int n_heads,
                        int page_rows, const int *row_start, int n_seqs, int max_rows,
                        const int *parents, const int *row_slot, const int *tokens,

@@ -231,7 +231,8 @@ int consume_status();
 // After a bounded wait ran out, a kernel may have left split counters
 // counted up: zero the counter regions of the calling thread's workspaces on
 // the current device, so that the next launch's last-part detection starts
-// clean. (Caller-owned workspaces are zeroed by the launches that use them.)
+// clean. (Caller-owned workspaces are zeroed by the attention launches that use
+// them; those of wattn_paged_attend by the caller.)
 void reset_split_counters() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return;

@@ -19,13 +19,14 @@
 // Many small items (a step of 320 beams x 20 heads) are not cut but taken one
 // by one from a counter: the warps of an SM share what it can read, so equal
 // shares end unequally, and taken ones even that out. 370 MB of keys and
-// values: 71 us (5.2 TB/s) against 87.5 in equal shares.
+// values: bf16 70 us (5.3 TB/s); 320 beams over up to 440 tokens, f16: 61.7 us
+// against 71.2 in equal shares.
 //
 // Elsewhere the chain of one stage bounds (scores, maximum, weights, products,
 // with eight compute warps on an SM): 64 trees of up to 33 rows over up to 448
-// tokens, 20 heads, f16 37 us (82 MB); 8 trees of up to 64 rows over up to
-// 32768 tokens, 8 heads, bf16 77 us (238 MB); one tree of 16 rows 11 us, of
-// which 3 are the launch.
+// tokens, 20 heads, f16 36 us (82 MB); 8 trees of up to 64 rows over up to
+// 32768 tokens, 8 heads, bf16 76 us (238 MB); one tree of 16 rows 10.6 us, of
+// which 3 are the launch. (Replayed graphs.)
 #include <algorithm>
 
 #include "paged_attend.cuh"
@@ -60,7 +61,10 @@ static_assert(kPaStages * kPaStageBytes >= kPaWarps * kPaTileFloats * 4, "a ring
 template <typename T> struct PaType;
 template <> struct PaType<__half> : PaNarrow16 {
   static constexpr uint32_t kOne = 0x3c00u, kInf = 0x7c00u;
-  static constexpr bool kResidual = false;  // f16 weights of 9 rows or more: 2^-11 each, within the 2e-3 bar
+  // f16 weights of 9 rows or more: 2^-11 each, within the 2e-3 bar (with their
+  // residuals one tree of 16 rows takes 12.9 us instead of 10.6, 64 of up to 33
+  // 40.9 instead of 35.9).
+  static constexpr bool kResidual = false;
   static constexpr float kLower = kPaLower16;
 };
 template <> struct PaType<__nv_bfloat16> : PaNarrow16 {
@@ -70,7 +74,10 @@ template <> struct PaType<__nv_bfloat16> : PaNarrow16 {
 };
 template <> struct PaType<float> : PaShape {
   static constexpr int kKeys = 16, kRows = 16;
-  static constexpr int kMinUnits = 8;  // (16 requests of 13 rows over 448 tokens: 14.5 us, with 16 17.1)
+  // (8 / 16 units, 13 rows a request: 1 request of 6 heads over 448 tokens 12.2
+  // us / 13.7, 4 of them 13.4 / 15.7, 16 of 8 heads over 224 tokens 13.9 / 16.4,
+  // 1 of 8 heads over 4000 17.2 / 18.4; 4 units as 8, 32 up to 45 % longer.)
+  static constexpr int kMinUnits = 8;
 };
 static_assert(PaType<__half>::kKeys <= kPaMostKeys && PaType<float>::kKeys <= kPaMostKeys, "see kPaMostKeys");
 

@@ -59,9 +59,10 @@ constexpr float kPaLower16 = 7.f;
 struct PaShape {
   static constexpr int kShares = kPaWarps, kThreads = kPaThreads;
   // Items to a compute warp from which they are taken one by one (cached
-  // lengths from 1 to 440, f16, taken / in equal shares: 400 requests of 12
-  // heads 68.6 us / 76.8, 600 88.3 / 103.4, 300 of 20 heads and 40 new rows
-  // 235 / 273; of 200 or 300 requests of 12 heads the lookup alone costs 2 us).
+  // lengths from 1 to 440, f16, taken / in equal shares: 200 requests of 12
+  // heads 39.5 us / 35.4, 300 52.8 / 47.8, 400 53.0 / 60.6, 600 70.2 / 79.8, 320
+  // of 20 heads 61.7 / 71.2, 2000 of 3 heads 65.5 / 72.3; 300 of 20 heads and 40
+  // new rows 197 / 196).
   static constexpr int kQueueItems = 4;
   static constexpr int kStageUnits = 4, kWideUnits = 5, kItemUnits = 12;
   static constexpr int kMinUnits = 16;  // units of a share below which fewer warps work
