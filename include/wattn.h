@@ -426,7 +426,10 @@ int wattn_paged_write(void *pool, int dtype, int n_pages, int n_layers, int n_he
  * 2^31 - 257 positions, and a call of 2^31 units of work or more, which writes
  * no rows (f16 and bf16: up to 5 units for every 32 keys of each head and tile
  * of 32 rows, and 12 for the tile; f32: 4 for every 16 keys of a tile of 16
- * rows, and 12). A row that sees a draft whose score is NaN or +inf is NaN.
+ * rows, and 12). A row that sees a draft whose score is NaN or +inf is NaN; one
+ * whose score is -inf counts nothing, and where its value is not finite either,
+ * the row may or may not be. A finite score's value that is not finite makes its
+ * dimension what the formula does.
  * The softmax weights enter the second product with 22 bits in f16 pools where
  * the request has up to 8 new rows, with 11 where it has more (in steps of
  * 2^-31 of the row's largest at the finest), with 16 in bf16 pools, and as two

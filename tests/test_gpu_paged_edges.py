@@ -237,6 +237,20 @@ def test_row_buffers_larger_than_the_step(W, n, heads):
     assert (large[n:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_masks_narrower_than_the_step(W, dtype):
+    """Mask words for fewer drafts than the request has rows: those behind are seen by none."""
+    import torch
+    b = Batch(72, dtype, [40, 0, 5], [70, 33, 3], 3, 32, sum((tree(np.random.default_rng(72), k) for k in (70, 33, 3)), []),
+              words=3, layers=1)
+    b.mask[:, 1:] = 0
+    table, seq, start, _ = b.device()
+    o = torch.zeros(b.max_rows, 192, device="cuda")
+    W.paged_attend(b.pool, 0, table, seq, start, b.q, o, row_mask=cu(b.mask[:, :1]))
+    ref, mag, top = formula(b, 0)
+    assert (np.abs(o[:106].cpu().numpy() - ref) <= bound(dtype, "f32", ref, mag, top, 110, 6.0)).all()
+
+
 # ------------------------------------------------------------------ steps that the wide kernel takes
 
 WIDE_STEPS = [
