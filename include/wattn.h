@@ -431,9 +431,10 @@ int wattn_paged_write(void *pool, int dtype, int n_pages, int n_layers, int n_he
  * the row may or may not be. A finite score's value that is not finite makes its
  * dimension what the formula does.
  * The softmax weights enter the second product with 22 bits in f16 pools where
- * the request has up to 8 new rows, with 11 where it has more (in steps of
- * 2^-31 of the row's largest at the finest), with 16 in bf16 pools, and as two
- * tf32 parts in f32 pools.
+ * the request has up to 8 new rows, with 11 where it has more or where the
+ * call's rows fill tiles of 128 over long contexts (in steps of 2^-31 of the
+ * row's largest at the finest), with 16 in bf16 pools, and as two tf32 parts in
+ * f32 pools.
  * workspace as for wattn_decode_fwd (wattn_paged_attend_workspace_bytes(),
  * zero-filled before its first use), or NULL. Calls that may overlap, captured
  * graphs among them, need one each; a call that is captured with NULL gets one
